@@ -27,8 +27,10 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "librans_hip.so")
 SOURCES = [os.path.join(CSRC, f) for f in ("rans_gemv.hip", "rans_decode.hip", "rans_linear.hip", "rans_matmul.hip",
-                                           "ref32_gemv.hip", "w64_host.cpp")]
-HEADERS = [os.path.join(INCLUDE, "vramc_rans.h"), os.path.join(CSRC, "rans_device.h")]
+                                           "ref32_gemv.hip", "kv_append.hip", "kv_attend.hip",
+                                           "kv_evict.hip", "w64_host.cpp")]
+HEADERS = [os.path.join(INCLUDE, "vramc_rans.h"), os.path.join(INCLUDE, "vramc_kv.h"),
+           os.path.join(CSRC, "rans_device.h"), os.path.join(CSRC, "kv_device.h")]
 
 SCALE_BITS = 12
 M = 1 << SCALE_BITS
