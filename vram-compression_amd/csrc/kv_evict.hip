@@ -1,158 +1,312 @@
 // Eviction of a cache's tokens by accumulated weight.
 //
 // A kv head of a sequence ranks its tokens by a 32-bit key that sorts as the
-// order of eviction does.  The budget-th largest key is found by radix
-// selection, eight bits at a time; every token above it is kept, and of those
-// equal to it as many as there is room for, lowest index first.  What moves
-// where is then two ordered lists, and moving is a copy of rows that are all
-// different places.
+// order of eviction does.  One workgroup reads the keys of up to 32768 tokens
+// into LDS once, finds the budget-th largest by radix selection (11, 11 and 10
+// bits, histograms in LDS too), and keeps every token above it and of those
+// equal to it as many as there is room for, lowest index first.  A wave goes
+// over neighbouring tokens, so that ranks within it are counts of ballot bits,
+// and the order of indices costs one exchange between the waves.  Longer
+// sequences go through in pieces of 32768 tokens, read again for every step.
+//
+// What moves is then two ordered lists of places, all different, and moving a
+// copy of rows.  In place a kept token moves only if it lies beyond the budget:
+// a decode step's eviction moves one token, not the cache.
 #include "kv_device.h"
 
 namespace {
 
-constexpr int kSelect = 1024;  // threads that select
-constexpr int kMove = 256;     // threads that move
+constexpr int kSelect = 1024;          // threads that select
+constexpr int kWaves = kSelect / 64;
+constexpr int kBatch = 8;              // keys that a lane loads at once
+constexpr int kKeys = 32;              // keys of a lane
+constexpr int kPiece = kSelect * kKeys;
+constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
+constexpr int kMove = 256;             // threads that move
+constexpr int kRows = 16;              // tokens that a wave moves at once
+// With at most this many moves a kv head (known from the table's width and the
+// budget) the selecting workgroup makes them itself, a wave's worth each:
+// a launch less.
+constexpr int kMovesHere = kWaves * kRows;
 
 struct Evict {
     vramc_kv_cache c;
+    int page_shift;
     const int32_t* table;
     int64_t table_row;
-    int table_width;
+    int bound;                   // tokens that a row of the table has room for
     const int32_t *lengths, *seen;
-    int batch, budget, recent;
+    int budget, recent;
     const int32_t* into;
     int64_t into_row;
-    int into_width;
     int32_t* new_lengths;
-    int32_t *from, *to, *count;  // [batch * kv_heads][most] places, and how many
+    int32_t *from, *to, *count;  // [batch * kv_heads][most] indices, and how many
     int most;
 };
 
 // The place of token j: slot of the cache for a kv head, -1 for none.
 __device__ __forceinline__ int64_t place(const Evict& e, const int32_t* row, int h, int j) {
-    const int page = row[j / e.c.page_size];
+    const int page = row[j >> e.page_shift];
     if (page < 0 || page >= e.c.pages) return -1;
-    return ((int64_t)page * e.c.kv_heads + h) * e.c.page_size + j % e.c.page_size;
+    return ((((int64_t)page * e.c.kv_heads + h) << e.page_shift) + (j & (e.c.page_size - 1)));
 }
 
 // Sorts as the order in which tokens are kept: 0 for a token that is nowhere,
 // the mass's bits made monotonic (NaN as -infinity), all ones for a recent one.
-__device__ __forceinline__ uint32_t rank_of(const Evict& e, int64_t at, int from_position) {
-    if (at < 0) return 0;
-    if (e.c.position[at] >= from_position) return 0xffffffffu;
-    float m = e.c.mass[at];
+__device__ __forceinline__ uint32_t rank_of(float m, int position, bool there, int recent) {
     if (m != m) m = -__builtin_inff();
     const uint32_t bits = __float_as_uint(m + 0.f);  // -0 as 0
-    return bits >> 31 ? ~bits : bits | 0x80000000u;
+    const uint32_t sorted = bits >> 31 ? ~bits : bits | 0x80000000u;
+    return !there ? 0 : position >= recent ? 0xffffffffu : sorted;
 }
 
-// Exclusive sum over the workgroup's threads; total in *sum.
-__device__ int scan(int x, int* buf, int* sum) {
-    const int t = threadIdx.x;
-    buf[t] = x;
-    __syncthreads();
-    for (int n = 1; n < kSelect; n *= 2) {
-        const int y = t >= n ? buf[t - n] : 0;
-        __syncthreads();
-        buf[t] += y;
-        __syncthreads();
+// Copies the tokens of list entries first .. first + kRows - 1, below count, of
+// a kv head, by one wave: 16 bytes a lane, four loads of keys and four of
+// values before the first store.
+__device__ __forceinline__ void move_rows(const Evict& e, int group, int first, int count, int64_t* from_at,
+                          int64_t* to_at) {
+    const int lane = threadIdx.x & 63, b = group / e.c.kv_heads, h = group % e.c.kv_heads;
+    const int n = min(kRows, count - first);
+    if (lane < kRows) {
+        int64_t from = -1, to = -1;
+        if (lane < n) {
+            const int64_t i = (int64_t)group * e.most + first + lane;
+            const int32_t* row = e.table + b * e.table_row;
+            from = place(e, row, h, e.from[i]);
+            to = place(e, e.into ? e.into + b * e.into_row : row, h, e.to[i]);
+        }
+        const bool moves = from >= 0 && to >= 0;
+        from_at[lane] = moves ? from : -1;
+        to_at[lane] = to;
+        if (moves) {
+            const float m = e.c.mass[from];
+            const int p = e.c.position[from];
+            e.c.mass[to] = m;
+            e.c.position[to] = p;
+        }
     }
-    *sum = buf[kSelect - 1];
-    const int before = buf[t] - x;
-    __syncthreads();
-    return before;
+    __builtin_amdgcn_wave_barrier();
+    const int wide = e.c.mx ? e.c.head_dim / 32 : e.c.head_dim * (e.c.dtype == RANS_X_F32 ? 4 : 2) / 16;
+    auto* k = static_cast<vec<uint32_t, 4>*>(e.c.k);
+    auto* v = static_cast<vec<uint32_t, 4>*>(e.c.v);
+    constexpr int U = 4;
+    for (int at = lane; at < n * wide; at += 64 * U) {
+        vec<uint32_t, 4> x[U], y[U];
+        int64_t to[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = at + 64 * u, r = i / wide;
+            to[u] = -1;
+            if (r < n && from_at[r] >= 0) {
+                const int64_t from = from_at[r] * wide + (i - r * wide);
+                to[u] = to_at[r] * wide + (i - r * wide);
+                x[u] = k[from];
+                y[u] = v[from];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (to[u] >= 0) {
+                k[to[u]] = x[u];
+                v[to[u]] = y[u];
+            }
+    }
+    if (e.c.mx) {
+        const int scales = e.c.head_dim / kMxBlock;
+        for (int i = lane; i < n * scales; i += 64) {
+            const int r = i / scales;
+            if (from_at[r] < 0) continue;
+            const int64_t from = from_at[r] * scales + (i - r * scales);
+            const int64_t to = to_at[r] * scales + (i - r * scales);
+            const uint8_t x = e.c.k_scale[from], y = e.c.v_scale[from];
+            e.c.k_scale[to] = x;
+            e.c.v_scale[to] = y;
+        }
+    }
 }
 
-__global__ void __launch_bounds__(kSelect) select_kernel(Evict e) {
-    __shared__ int hist[256], buf[kSelect], found[2];
+// Counts of the waves before this one, and of all, for three kinds of token.
+struct Sums {
+    int before[3], all[3];
+};
+__device__ __forceinline__ Sums across_waves(const int (&mine)[3], int (*buf)[kWaves]) {
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < 3; k++) buf[k][wave] = mine[k];
+    __syncthreads();
+    Sums s = {};
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            s.before[k] += w < wave ? buf[k][w] : 0;
+            s.all[k] += buf[k][w];
+        }
+    return s;
+}
+
+__global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
+    extern __shared__ uint32_t piece_keys[];
+    __shared__ int hist[kBins], waves[3][kWaves], found[3];
+    __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
-    const int bound = e.table_width * e.c.page_size;
-    const int n = min(max(e.lengths[b], 0), bound);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = min(max(e.lengths[b], 0), e.bound);
     const int32_t* row = e.table + b * e.table_row;
-    const int64_t from_position = (int64_t)e.seen[b] - e.recent;
-    const int recent = (int)max(from_position, (int64_t)INT32_MIN);
+    const int recent = (int)max((int64_t)e.seen[b] - e.recent, (int64_t)INT32_MIN);
     if (h == 0 && threadIdx.x == 0) e.new_lengths[b] = min(n, e.budget);
     int32_t* from = e.from + (int64_t)blockIdx.x * e.most;
     int32_t* to = e.to + (int64_t)blockIdx.x * e.most;
+    int count = 0;
     if (n <= e.budget) {  // everything is kept
-        if (threadIdx.x == 0) e.count[blockIdx.x] = e.into ? n : 0;
-        if (e.into)
+        if (e.into) {
+            count = n;
             for (int j = threadIdx.x; j < n; j += kSelect) from[j] = to[j] = j;
+        }
+    } else {
+        const int pieces = (n + kPiece - 1) / kPiece;
+        const int each = pieces > 1 ? kKeys : (n + kSelect - 1) / kSelect;  // keys of a lane
+        int first, limit;  // the wave's tokens in the piece at hand, and its keys
+        uint32_t* keys = piece_keys + wave * 64 * each + lane;
+        const auto load = [&](int piece) {
+            first = piece * kPiece + wave * 64 * each;
+            limit = min(n, first + 64 * each);
+            for (int i = 0; i < each; i += kBatch) {
+                int64_t at[kBatch];
+                float m[kBatch];
+                int p[kBatch];
+#pragma unroll
+                for (int u = 0; u < kBatch; u++)
+                    at[u] = place(e, row, h, min(first + 64 * (i + u) + lane, n - 1));
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    m[u] = e.c.mass[max(at[u], (int64_t)0)];
+                    p[u] = e.c.position[max(at[u], (int64_t)0)];
+                }
+#pragma unroll
+                for (int u = 0; u < kBatch; u++)
+                    if (i + u < each) keys[64 * (i + u)] = rank_of(m[u], p[u], at[u] >= 0, recent);
+            }
+        };
+        const auto each_key = [&](auto f) {  // f(key, index, whether the index is the wave's)
+            for (int i = 0; first + 64 * i < limit; i++) {
+                const int j = first + 64 * i + lane;
+                f(keys[64 * i], j, j < limit);
+            }
+        };
+        uint32_t above = 0;  // the digits found so far
+        int room = e.budget; // tokens to keep of those that share them
+        hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
+        __syncthreads();
+        if (pieces == 1) load(0);
+        for (int shift = 21, bits = 11; bits; shift = shift == 21 ? 10 : 0) {
+            for (int piece = 0; piece < pieces; piece++) {
+                if (pieces > 1) load(piece);
+                each_key([&](uint32_t r, int, bool mine) {
+                    if (mine && (shift == 21 || (r ^ above) >> (shift + bits) == 0))
+                        atomicAdd(&hist[r >> shift & ((1 << bits) - 1)], 1);
+                });
+            }
+            __syncthreads();
+            // the bin that holds the room-th largest: a sum from the top over
+            // the threads, two bins each
+            const int low = hist[2 * threadIdx.x], high = hist[2 * threadIdx.x + 1];
+            int sum = low + high;
+            for (int d = 1; d < 64; d *= 2) {
+                const int x = __shfl_down(sum, d);
+                sum += lane + d < 64 ? x : 0;
+            }
+            if (lane == 0) waves[0][wave] = sum;
+            __syncthreads();
+            hist[2 * threadIdx.x] = hist[2 * threadIdx.x + 1] = 0;
+            int over = sum - low - high;  // in the bins above these two
+            for (int w = wave + 1; w < kWaves; w++) over += waves[0][w];
+            if (over < room && room <= over + low + high) {
+                const bool upper = room <= over + high;
+                found[0] = 2 * threadIdx.x + upper;
+                found[1] = room - over - (upper ? 0 : high);
+                found[2] = upper ? high : low;
+            }
+            __syncthreads();
+            above |= (uint32_t)found[0] << shift;
+            room = found[1];
+            if (room == found[2]) break;  // all that share these digits are kept
+            if (shift == 0) break;
+            bits = shift == 21 ? 11 : 10;
+        }
+        // Kept: what exceeds `above`, which has the digits found and zeros behind
+        // them, and `room` of those that share its digits.  If the search ended
+        // early those are all that there are, else they are equal to it.
+        const bool all = room == found[2];
+        int done[3] = {0, 0, 0};  // ties, kept (or holes), moves of the pieces so far
+        for (int piece = 0; piece < pieces; piece++) {
+            if (pieces > 1) load(piece);
+            int mine[3] = {0, 0, 0};
+            if (!all) {
+                each_key([&](uint32_t r, int, bool ok) { mine[0] += __popcll(__ballot(ok && r == above)); });
+                const Sums s = across_waves(mine, waves);
+                mine[0] = done[0] + s.before[0];
+                done[0] += s.all[0];
+            }
+            const auto kept = [&](uint32_t r, bool ok, int* ties) {
+                if (all) return ok && r >= above;
+                const uint64_t same = __ballot(ok && r == above);
+                const int before = *ties + __popcll(same & ((1ull << lane) - 1));
+                *ties += __popcll(same);
+                return ok && (r > above || (r == above && before < room));
+            };
+            int ties = mine[0];
+            each_key([&](uint32_t r, int j, bool ok) {
+                const bool keep = kept(r, ok, &ties);
+                mine[1] += __popcll(__ballot(e.into ? keep : ok && !keep && j < e.budget));
+                mine[2] += __popcll(__ballot(keep && j >= e.budget));
+            });
+            const Sums s = across_waves(mine, waves);
+            int at[2] = {done[1] + s.before[1], done[2] + s.before[2]};
+            done[1] += s.all[1];
+            done[2] += s.all[2];
+            ties = mine[0];
+            each_key([&](uint32_t r, int j, bool ok) {
+                const bool keep = kept(r, ok, &ties);
+                const uint64_t below = (1ull << lane) - 1;
+                const bool one = e.into ? keep : ok && !keep && j < e.budget;
+                const uint64_t ones = __ballot(one);
+                const int i = at[0] + __popcll(ones & below);
+                at[0] += __popcll(ones);
+                if (one) to[i] = e.into ? i : j;
+                if (one && e.into) from[i] = j;
+                if (!e.into) {
+                    const bool moves = keep && j >= e.budget;
+                    const uint64_t twos = __ballot(moves);
+                    if (moves) from[at[1] + __popcll(twos & below)] = j;
+                    at[1] += __popcll(twos);
+                }
+            });
+        }
+        count = e.into ? done[1] : done[2];
+    }
+    if (!moves_here) {
+        if (threadIdx.x == 0) e.count[blockIdx.x] = count;
         return;
     }
-    uint32_t above = 0;     // the digits found so far
-    int room = e.budget;    // tokens to keep of those that share them
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kSelect) hist[i] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kSelect) {
-            const uint32_t r = rank_of(e, place(e, row, h, j), recent);
-            if (shift == 24 || r >> (shift + 8) == above >> (shift + 8))
-                atomicAdd(&hist[r >> shift & 255], 1);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int digit = 255, left = room;
-            while (hist[digit] < left) left -= hist[digit--];
-            found[0] = digit;
-            found[1] = left;
-        }
-        __syncthreads();
-        above |= (uint32_t)found[0] << shift;
-        room = found[1];
-        __syncthreads();
-    }
-    // `above` is the budget-th largest rank, `room` of its tokens are kept
-    int ties = 0, holes = 0, kept_above = 0, kept = 0;
-    for (int first = 0; first < n; first += kSelect) {
-        const int j = first + threadIdx.x;
-        const uint32_t r = j < n ? rank_of(e, place(e, row, h, j), recent) : 0;
-        int sum;
-        const bool tie = j < n && r == above;
-        const int tied = ties + scan(tie, buf, &sum);
-        ties += sum;
-        const bool keep = j < n && (r > above || (tie && tied < room));
-        if (e.into) {
-            const int i = kept + scan(keep, buf, &sum);
-            kept += sum;
-            if (keep) from[i] = j, to[i] = i;
-        } else {
-            const bool hole = j < e.budget && !keep;
-            int i = holes + scan(hole, buf, &sum);
-            holes += sum;
-            if (hole) to[i] = j;
-            const bool moves = keep && j >= e.budget;
-            i = kept_above + scan(moves, buf, &sum);
-            kept_above += sum;
-            if (moves) from[i] = j;
-        }
-    }
-    if (threadIdx.x == 0) e.count[blockIdx.x] = e.into ? kept : kept_above;
+    __syncthreads();  // the lists are this workgroup's own
+    if (wave * kRows < count) move_rows(e, blockIdx.x, wave * kRows, count, rows[wave][0], rows[wave][1]);
 }
 
-// One wave moves a token of a kv head.
 __global__ void __launch_bounds__(kMove) move_kernel(Evict e) {
-    const int group = blockIdx.y, b = group / e.c.kv_heads, h = group % e.c.kv_heads;
-    const int i = blockIdx.x * (kMove / 64) + threadIdx.x / 64, lane = threadIdx.x & 63;
-    if (i >= e.count[group]) return;
-    const int64_t from = place(e, e.table + b * e.table_row, h, e.from[(int64_t)group * e.most + i]);
-    const int64_t to = place(e, e.into ? e.into + b * e.into_row : e.table + b * e.table_row, h,
-                             e.to[(int64_t)group * e.most + i]);
-    if (from < 0 || to < 0) return;
-    const int size = e.c.dtype == RANS_X_F32 ? 4 : 2;
-    const int bytes = e.c.mx ? e.c.head_dim / 2 : e.c.head_dim * size;
-    for (int which = 0; which < 2; which++) {
-        auto* p = static_cast<uint32_t*>(which ? e.c.v : e.c.k);
-        for (int j = lane; j < bytes / 4; j += 64) p[to * (bytes / 4) + j] = p[from * (bytes / 4) + j];
-        if (e.c.mx && lane < e.c.head_dim / kMxBlock) {
-            uint8_t* s = which ? e.c.v_scale : e.c.k_scale;
-            s[to * (e.c.head_dim / kMxBlock) + lane] = s[from * (e.c.head_dim / kMxBlock) + lane];
-        }
-    }
-    if (lane == 0) {
-        e.c.mass[to] = e.c.mass[from];
-        e.c.position[to] = e.c.position[from];
-    }
+    __shared__ int64_t rows[kMove / 64][2][kRows];
+    const int wave = threadIdx.x >> 6, group = blockIdx.y;
+    const int first = (blockIdx.x * (kMove / 64) + wave) * kRows, count = e.count[group];
+    if (first < count) move_rows(e, group, first, count, rows[wave][0], rows[wave][1]);
+}
+
+// Lets the selecting workgroup have more LDS than 64 KB, once a process.
+int allow_lds() {
+    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(select_kernel),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kPiece * 4);
+    return (int)rc;
 }
 
 // Tokens of a kv head that one call can move.
@@ -188,12 +342,17 @@ extern "C" int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int
     if (!workspace || workspace_bytes < need) return RANS_EWORKSPACE;
     const int64_t heads = (int64_t)batch * c->kv_heads;
     auto* count = static_cast<int32_t*>(workspace);
-    Evict e{*c, table, table_row, table_width, lengths, seen, batch, budget, recent, into, into_row,
-            into_width, new_lengths, count + heads, count + heads + heads * most, count, (int)most};
-    hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), 0, stream, e);
+    Evict e{*c, __builtin_ctz(c->page_size), table, table_row, table_width * c->page_size, lengths,
+            seen, budget, recent, into, into_row, new_lengths, count + heads,
+            count + heads + heads * most, count, (int)most};
+    const bool here = most <= kMovesHere;
+    const int64_t keys = e.bound < kPiece ? e.bound : kPiece;
+    const size_t lds = (size_t)((keys + kSelect - 1) / kSelect * kSelect * 4);
+    if (const int rc = allow_lds()) return rc;
+    hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), lds, stream, e, here);
     if (const int rc = (int)hipGetLastError()) return rc;
-    if (!most) return 0;
-    const int rows = kMove / 64;
+    if (here) return 0;
+    const int rows = kMove / 64 * kRows;
     hipLaunchKernelGGL(move_kernel, dim3((unsigned)((most + rows - 1) / rows), (unsigned)heads),
                        dim3(kMove), 0, stream, e);
     return (int)hipGetLastError();
