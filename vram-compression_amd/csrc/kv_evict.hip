@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kSelect = 1024;          // threads that select
 constexpr int kWaves = kSelect / 64;
-constexpr int kBatch = 8;              // keys that a lane loads at once
+constexpr int kBatch = 16;             // keys that a lane loads at once
 constexpr int kKeys = 32;              // keys of a lane
 constexpr int kPiece = kSelect * kKeys;
 constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
@@ -125,31 +125,54 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
     }
 }
 
-// Counts of the waves before this one, and of all, for three kinds of token.
-struct Sums {
-    int before[3], all[3];
-};
-__device__ __forceinline__ Sums across_waves(const int (&mine)[3], int (*buf)[kWaves]) {
-    const int wave = threadIdx.x >> 6;
+// The sum over a wave's lanes below this one, and over the workgroup's waves
+// below this one; the workgroup's whole sum in *all.
+__device__ __forceinline__ uint32_t before_of(uint32_t x, uint32_t* waves, uint32_t* all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t y = __shfl_up(sum, d);
+        sum += lane >= d ? y : 0;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-        for (int k = 0; k < 3; k++) buf[k][wave] = mine[k];
+    if (lane == 63) waves[wave] = sum;
     __syncthreads();
-    Sums s = {};
+    uint32_t below = 0, total = 0;
 #pragma unroll
-    for (int k = 0; k < 3; k++)
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            s.before[k] += w < wave ? buf[k][w] : 0;
-            s.all[k] += buf[k][w];
-        }
-    return s;
+    for (int w = 0; w < kWaves; w++) {
+        below += w < wave ? waves[w] : 0;
+        total += waves[w];
+    }
+    *all = total;
+    return below + sum - x;
+}
+
+// The n lowest bits of a word, and of those that are set in x.
+__device__ __forceinline__ uint64_t low_bits(int n) {
+    return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1;
+}
+__device__ __forceinline__ uint64_t lowest_set(uint64_t x, int n) {
+    if (n >= (int)__popcll(x)) return x;
+    uint64_t got = 0;
+    for (; n > 0; n--) {
+        got |= x & -x;
+        x &= x - 1;
+    }
+    return got;
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ int bits_below(uint64_t x) {  // this lane
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, 0));
 }
 
 __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
     extern __shared__ uint32_t piece_keys[];
-    __shared__ int hist[kBins], waves[3][kWaves], found[3];
+    __shared__ int hist[kBins], found[3];
+    __shared__ uint32_t waves[kWaves];
     __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -190,12 +213,6 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                     if (i + u < each) keys[64 * (i + u)] = rank_of(m[u], p[u], at[u] >= 0, recent);
             }
         };
-        const auto each_key = [&](auto f) {  // f(key, index, whether the index is the wave's)
-            for (int i = 0; first + 64 * i < limit; i++) {
-                const int j = first + 64 * i + lane;
-                f(keys[64 * i], j, j < limit);
-            }
-        };
         uint32_t above = 0;  // the digits found so far
         int room = e.budget; // tokens to keep of those that share them
         hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
@@ -204,10 +221,11 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         for (int shift = 21, bits = 11; bits; shift = shift == 21 ? 10 : 0) {
             for (int piece = 0; piece < pieces; piece++) {
                 if (pieces > 1) load(piece);
-                each_key([&](uint32_t r, int, bool mine) {
-                    if (mine && (shift == 21 || (r ^ above) >> (shift + bits) == 0))
+                for (int i = 0; first + 64 * i < limit; i++) {
+                    const uint32_t r = keys[64 * i];
+                    if (first + 64 * i + lane < limit && (shift == 21 || (r ^ above) >> (shift + bits) == 0))
                         atomicAdd(&hist[r >> shift & ((1 << bits) - 1)], 1);
-                });
+                }
             }
             __syncthreads();
             // the bin that holds the room-th largest: a sum from the top over
@@ -218,11 +236,11 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                 const int x = __shfl_down(sum, d);
                 sum += lane + d < 64 ? x : 0;
             }
-            if (lane == 0) waves[0][wave] = sum;
+            if (lane == 0) waves[wave] = sum;
             __syncthreads();
             hist[2 * threadIdx.x] = hist[2 * threadIdx.x + 1] = 0;
             int over = sum - low - high;  // in the bins above these two
-            for (int w = wave + 1; w < kWaves; w++) over += waves[0][w];
+            for (int w = wave + 1; w < kWaves; w++) over += waves[w];
             if (over < room && room <= over + low + high) {
                 const bool upper = room <= over + high;
                 found[0] = 2 * threadIdx.x + upper;
@@ -240,52 +258,42 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         // them, and `room` of those that share its digits.  If the search ended
         // early those are all that there are, else they are equal to it.
         const bool all = room == found[2];
-        int done[3] = {0, 0, 0};  // ties, kept (or holes), moves of the pieces so far
+        // Lane i of a wave decides about its i-th 64 tokens, all bits at once.
+        uint32_t ties = 0, lists[2] = {0, 0};  // of the pieces so far
         for (int piece = 0; piece < pieces; piece++) {
             if (pieces > 1) load(piece);
-            int mine[3] = {0, 0, 0};
-            if (!all) {
-                each_key([&](uint32_t r, int, bool ok) { mine[0] += __popcll(__ballot(ok && r == above)); });
-                const Sums s = across_waves(mine, waves);
-                mine[0] = done[0] + s.before[0];
-                done[0] += s.all[0];
+            uint64_t more = 0, same = 0;
+            for (int i = 0; first + 64 * i < limit; i++) {
+                const uint32_t r = keys[64 * i];
+                const bool mine = first + 64 * i + lane < limit;
+                const uint64_t x = __ballot(mine && r > above), y = __ballot(mine && r == above);
+                if (lane == i) more = x, same = y;
             }
-            const auto kept = [&](uint32_t r, bool ok, int* ties) {
-                if (all) return ok && r >= above;
-                const uint64_t same = __ballot(ok && r == above);
-                const int before = *ties + __popcll(same & ((1ull << lane) - 1));
-                *ties += __popcll(same);
-                return ok && (r > above || (r == above && before < room));
-            };
-            int ties = mine[0];
-            each_key([&](uint32_t r, int j, bool ok) {
-                const bool keep = kept(r, ok, &ties);
-                mine[1] += __popcll(__ballot(e.into ? keep : ok && !keep && j < e.budget));
-                mine[2] += __popcll(__ballot(keep && j >= e.budget));
-            });
-            const Sums s = across_waves(mine, waves);
-            int at[2] = {done[1] + s.before[1], done[2] + s.before[2]};
-            done[1] += s.all[1];
-            done[2] += s.all[2];
-            ties = mine[0];
-            each_key([&](uint32_t r, int j, bool ok) {
-                const bool keep = kept(r, ok, &ties);
-                const uint64_t below = (1ull << lane) - 1;
-                const bool one = e.into ? keep : ok && !keep && j < e.budget;
-                const uint64_t ones = __ballot(one);
-                const int i = at[0] + __popcll(ones & below);
-                at[0] += __popcll(ones);
-                if (one) to[i] = e.into ? i : j;
-                if (one && e.into) from[i] = j;
-                if (!e.into) {
-                    const bool moves = keep && j >= e.budget;
-                    const uint64_t twos = __ballot(moves);
-                    if (moves) from[at[1] + __popcll(twos & below)] = j;
-                    at[1] += __popcll(twos);
-                }
-            });
+            uint32_t sum;
+            if (!all) {
+                const uint32_t before = ties + before_of(__popcll(same), waves, &sum);
+                ties += sum;
+                same = lowest_set(same, room - (int)before);
+            }
+            const int start = first + 64 * lane;  // of the lane's 64 tokens
+            const uint64_t kept = more | same, low = low_bits(e.budget - start);
+            const uint64_t listed[2] = {e.into ? kept : low_bits(limit - start) & low & ~kept,
+                                        e.into ? 0 : kept & ~low};
+            // at most 32768 of each in a piece: both sums in one word
+            const uint32_t before = before_of(__popcll(listed[0]) | __popcll(listed[1]) << 16, waves, &sum);
+            const uint32_t at[2] = {lists[0] + (before & 0xffff), lists[1] + (before >> 16)};
+            lists[0] += sum & 0xffff;
+            lists[1] += sum >> 16;
+            for (int i = 0; first + 64 * i < limit; i++) {
+                const int j = first + 64 * i + lane;
+                const uint64_t one = of_lane(listed[0], i), two = of_lane(listed[1], i);
+                const int k = __builtin_amdgcn_readlane((int)at[0], i) + bits_below(one);
+                const int l = __builtin_amdgcn_readlane((int)at[1], i) + bits_below(two);
+                if (one >> lane & 1) to[k] = e.into ? k : j;
+                if (e.into ? one >> lane & 1 : two >> lane & 1) from[e.into ? k : l] = j;
+            }
         }
-        count = e.into ? done[1] : done[2];
+        count = lists[0];
     }
     if (!moves_here) {
         if (threadIdx.x == 0) e.count[blockIdx.x] = count;
