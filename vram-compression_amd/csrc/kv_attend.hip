@@ -119,25 +119,6 @@ __device__ __forceinline__ vec<float, 4> mma(Half8<_Float16> a, Half8<_Float16> 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Two values of a byte of codes (the lower half first) times 2^(scale - 127).
-template <typename T, int BYTE>
-__device__ __forceinline__ uint32_t mx_pair(uint32_t codes, uint32_t scale) {
-    const float unit = __uint_as_float(scale << 23);  // the conversion reads the exponent alone
-    if constexpr (std::is_same_v<T, __bf16>)
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, BYTE));
-    else
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, unit, BYTE));
-}
-template <typename T>
-__device__ __forceinline__ uint32_t mx_pair_at(uint32_t codes, uint32_t scale, int byte) {
-    switch (byte) {  // constant after unrolling
-        case 0: return mx_pair<T, 0>(codes, scale);
-        case 1: return mx_pair<T, 1>(codes, scale);
-        case 2: return mx_pair<T, 2>(codes, scale);
-        default: return mx_pair<T, 3>(codes, scale);
-    }
-}
-
 // The keys of a step as a wave holds them: per tile of 16, lane (key = lane %
 // 16, g) has a quarter of its key's columns.  Values: 16 bytes of every 64, so
 // that four lanes read 64 neighbouring bytes.  Codes: a quarter of the row.

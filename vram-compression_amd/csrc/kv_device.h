@@ -20,25 +20,28 @@ constexpr int64_t kMaxTokens = 1 << 30;  // that a row of the table has room for
 template <typename T, int N>
 using vec = T __attribute__((ext_vector_type(N)));
 
-// 2^(s-127) of a scale byte, whose bits are a float's exponent: 0 is the
-// subnormal 2^-127, 255 NaN.
-__device__ __forceinline__ float mx_power(uint32_t s) {
-    const uint32_t bits = s == 0 ? 0x00400000u : s == 255 ? 0x7fc00000u : s << 23;
-    return __uint_as_float(bits);
+// Two values of a byte of codes (the lower half first) times 2^(scale - 127).
+template <typename T, int BYTE>
+__device__ __forceinline__ uint32_t mx_pair(uint32_t codes, uint32_t scale) {
+    const float unit = __uint_as_float(scale << 23);  // the conversion reads the exponent alone
+    if constexpr (std::is_same_v<T, __bf16>)
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, unit, BYTE));
+    else
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, unit, BYTE));
 }
-
-// The value of a 4-bit code: 2^(e-1) * (1 + m/2), or m/2 where e is 0.
-__device__ __forceinline__ float mx_value(uint32_t code) {
-    const uint32_t e = code >> 1 & 3, m = code & 1;
-    const float a = e ? __uint_as_float((e + 126) << 23 | m << 22) : 0.5f * (float)m;
-    return code & 8 ? -a : a;
+template <typename T>
+__device__ __forceinline__ uint32_t mx_pair_at(uint32_t codes, uint32_t scale, int byte) {
+    switch (byte) {  // constant after unrolling
+        case 0: return mx_pair<T, 0>(codes, scale);
+        case 1: return mx_pair<T, 1>(codes, scale);
+        case 2: return mx_pair<T, 2>(codes, scale);
+        default: return mx_pair<T, 3>(codes, scale);
+    }
 }
-
-inline int size_of(int dtype) { return dtype == RANS_X_F32 ? 4 : 2; }
 
 // The checks of every entry point.
 inline int check_cache(const vramc_kv_cache* c) {
-    if (!c || !c->k || !c->v || c->pages <= 0 || c->kv_heads <= 0) return RANS_EARG;
+    if (!c || !c->k || !c->v || c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535) return RANS_EARG;
     switch (c->page_size) {
         case 16: case 32: case 64: case 128: case 256: break;
         default: return RANS_EUNSUPPORTED;

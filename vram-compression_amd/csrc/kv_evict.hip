@@ -22,6 +22,7 @@ constexpr int kBatch = 16;             // keys that a lane loads at once
 constexpr int kKeys = 32;              // keys of a lane
 constexpr int kPiece = kSelect * kKeys;
 constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
+constexpr int kFew = 256;              // keys that a search by bits takes over
 constexpr int kMove = 256;             // threads that move
 constexpr int kRows = 16;              // tokens that a wave moves at once
 // With at most this many moves a kv head (known from the table's width and the
@@ -51,13 +52,14 @@ __device__ __forceinline__ int64_t place(const Evict& e, const int32_t* row, int
     return ((((int64_t)page * e.c.kv_heads + h) << e.page_shift) + (j & (e.c.page_size - 1)));
 }
 
-// Sorts as the order in which tokens are kept: 0 for a token that is nowhere,
+// Sorts as the order in which tokens are kept: 1 for a token that is nowhere,
 // the mass's bits made monotonic (NaN as -infinity), all ones for a recent one.
+// 0 stands behind a sequence's last token and is never among the kept.
 __device__ __forceinline__ uint32_t rank_of(float m, int position, bool there, int recent) {
     if (m != m) m = -__builtin_inff();
     const uint32_t bits = __float_as_uint(m + 0.f);  // -0 as 0
     const uint32_t sorted = bits >> 31 ? ~bits : bits | 0x80000000u;
-    return !there ? 0 : position >= recent ? 0xffffffffu : sorted;
+    return !there ? 1 : position >= recent ? 0xffffffffu : sorted;
 }
 
 // Copies the tokens of list entries first .. first + kRows - 1, below count, of
@@ -128,7 +130,7 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
 // The sum over a wave's lanes below this one, and over the workgroup's waves
 // below this one; the workgroup's whole sum in *all.
 __device__ __forceinline__ uint32_t before_of(uint32_t x, uint32_t* waves, uint32_t* all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t sum = x;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -153,29 +155,24 @@ __device__ __forceinline__ uint64_t low_bits(int n) {
     return n >= 64 ? ~0ull : n <= 0 ? 0 : (1ull << n) - 1;
 }
 __device__ __forceinline__ uint64_t lowest_set(uint64_t x, int n) {
+    if (n <= 0) return 0;
     if (n >= (int)__popcll(x)) return x;
-    uint64_t got = 0;
-    for (; n > 0; n--) {
-        got |= x & -x;
-        x &= x - 1;
+    int at = 0;  // of the n-th set bit, found by halves
+#pragma unroll
+    for (int half = 32; half; half /= 2) {
+        const int in = __popcll(x >> at & low_bits(half));
+        if (in < n) n -= in, at += half;
     }
-    return got;
-}
-__device__ __forceinline__ uint64_t of_lane(uint64_t x, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
-}
-__device__ __forceinline__ int bits_below(uint64_t x) {  // this lane
-    return __builtin_amdgcn_mbcnt_hi((uint32_t)(x >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)x, 0));
+    return x & low_bits(at + 1);
 }
 
 __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
     extern __shared__ uint32_t piece_keys[];
-    __shared__ int hist[kBins], found[3];
-    __shared__ uint32_t waves[kWaves];
+    __shared__ int hist[kBins], found[4];
+    __shared__ uint32_t waves[kWaves], few[kFew];
     __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = min(max(e.lengths[b], 0), e.bound);
     const int32_t* row = e.table + b * e.table_row;
     const int recent = (int)max((int64_t)e.seen[b] - e.recent, (int64_t)INT32_MIN);
@@ -190,42 +187,77 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         }
     } else {
         const int pieces = (n + kPiece - 1) / kPiece;
-        const int each = pieces > 1 ? kKeys : (n + kSelect - 1) / kSelect;  // keys of a lane
+        // keys of a lane, in fours
+        const int each = pieces > 1 ? kKeys : (n + 4 * kSelect - 1) / (4 * kSelect) * 4;
         int first, limit;  // the wave's tokens in the piece at hand, and its keys
         uint32_t* keys = piece_keys + wave * 64 * each + lane;
         const auto load = [&](int piece) {
             first = piece * kPiece + wave * 64 * each;
             limit = min(n, first + 64 * each);
+            // the wave's pages: at most 2048 tokens, 16 or more to a page
+            const int page0 = first >> e.page_shift, pages = (max(limit, 1) - 1) >> e.page_shift;
+            int page[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                page[u] = page0 + 64 * u + lane <= pages ? row[page0 + 64 * u + lane] : -1;
+                if ((uint32_t)page[u] >= (uint32_t)e.c.pages) page[u] = -1;
+            }
             for (int i = 0; i < each; i += kBatch) {
-                int64_t at[kBatch];
+                if (first + 64 * i >= limit) {  // nothing there
+                    for (int u = i; u < each; u++) keys[64 * u] = 0;
+                    break;
+                }
                 float m[kBatch];
                 int p[kBatch];
-#pragma unroll
-                for (int u = 0; u < kBatch; u++)
-                    at[u] = place(e, row, h, min(first + 64 * (i + u) + lane, n - 1));
+                bool there[kBatch];
 #pragma unroll
                 for (int u = 0; u < kBatch; u++) {
-                    m[u] = e.c.mass[max(at[u], (int64_t)0)];
-                    p[u] = e.c.position[max(at[u], (int64_t)0)];
+                    const int j = min(first + 64 * (i + u) + lane, limit - 1);
+                    const int k = (j >> e.page_shift) - page0;
+                    const int x = __shfl(page[0], k & 63), y = __shfl(page[1], k & 63);
+                    const int in = k < 64 ? x : y;
+                    there[u] = in >= 0;
+                    const int64_t at = ((((int64_t)max(in, 0) * e.c.kv_heads + h) << e.page_shift) +
+                                        (j & (e.c.page_size - 1)));
+                    m[u] = e.c.mass[at];
+                    p[u] = e.c.position[at];
                 }
 #pragma unroll
                 for (int u = 0; u < kBatch; u++)
-                    if (i + u < each) keys[64 * (i + u)] = rank_of(m[u], p[u], at[u] >= 0, recent);
+                    if (i + u < each)
+                        keys[64 * (i + u)] = first + 64 * (i + u) + lane < limit
+                                                 ? rank_of(m[u], p[u], there[u], recent)
+                                                 : 0;
+            }
+        };
+        const auto over_keys = [&](auto f) {  // f(i, key): the wave's tokens 64 * i..
+            for (int i = 0; i < each; i += 4) {
+                uint32_t r[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) r[u] = keys[64 * (i + u)];
+#pragma unroll
+                for (int u = 0; u < 4; u++) f(i + u, r[u]);
             }
         };
         uint32_t above = 0;  // the digits found so far
         int room = e.budget; // tokens to keep of those that share them
+        int in_bin = 0;      // and how many do
         hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
         __syncthreads();
         if (pieces == 1) load(0);
-        for (int shift = 21, bits = 11; bits; shift = shift == 21 ? 10 : 0) {
+        if (threadIdx.x == 0) found[3] = 0;
+        for (int shift = 21, bits = 11;; shift = shift == 21 ? 10 : 0) {
             for (int piece = 0; piece < pieces; piece++) {
                 if (pieces > 1) load(piece);
-                for (int i = 0; first + 64 * i < limit; i++) {
-                    const uint32_t r = keys[64 * i];
-                    if (first + 64 * i + lane < limit && (shift == 21 || (r ^ above) >> (shift + bits) == 0))
-                        atomicAdd(&hist[r >> shift & ((1 << bits) - 1)], 1);
-                }
+                if (shift == 21)
+                    over_keys([&](int, uint32_t r) {
+                        if (r) atomicAdd(&hist[r >> 21], 1);
+                    });
+                else
+                    over_keys([&](int, uint32_t r) {
+                        if (r && (r ^ above) >> (shift + bits) == 0)
+                            atomicAdd(&hist[r >> shift & ((1 << bits) - 1)], 1);
+                    });
             }
             __syncthreads();
             // the bin that holds the room-th largest: a sum from the top over
@@ -250,25 +282,51 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             __syncthreads();
             above |= (uint32_t)found[0] << shift;
             room = found[1];
-            if (room == found[2]) break;  // all that share these digits are kept
-            if (shift == 0) break;
+            in_bin = found[2];
+            if (room == in_bin || shift == 0) break;  // all that share these digits are kept
+            if (in_bin <= kFew && pieces == 1) {
+                // few are left: one wave looks at all of them, bit by bit
+                over_keys([&](int, uint32_t r) {
+                    if (r && (r ^ above) >> shift == 0) few[atomicAdd(&found[3], 1)] = r;
+                });
+                __syncthreads();
+                if (wave == 0) {
+                    uint32_t left[kFew / 64];
+#pragma unroll
+                    for (int u = 0; u < kFew / 64; u++) left[u] = 64 * u + lane < in_bin ? few[64 * u + lane] : 0;
+                    for (int bit = shift - 1; bit >= 0; bit--) {
+                        const uint32_t next = above >> bit | 1;
+                        int ones = 0;
+#pragma unroll
+                        for (int u = 0; u < kFew / 64; u++)
+                            if (64 * u < in_bin) ones += __popcll(__ballot(left[u] >> bit == next));
+                        if (room <= ones) above |= 1u << bit;
+                        else room -= ones;
+                    }
+                    if (lane == 0) found[0] = (int)above, found[1] = room;
+                }
+                __syncthreads();
+                above = (uint32_t)found[0];
+                room = found[1];
+                in_bin = -1;  // equal keys, as many as there may be
+                break;
+            }
             bits = shift == 21 ? 11 : 10;
         }
         // Kept: what exceeds `above`, which has the digits found and zeros behind
         // them, and `room` of those that share its digits.  If the search ended
         // early those are all that there are, else they are equal to it.
-        const bool all = room == found[2];
+        const bool all = room == in_bin;
+        above = max(above, 1u);  // not what stands behind the last token
         // Lane i of a wave decides about its i-th 64 tokens, all bits at once.
         uint32_t ties = 0, lists[2] = {0, 0};  // of the pieces so far
         for (int piece = 0; piece < pieces; piece++) {
             if (pieces > 1) load(piece);
             uint64_t more = 0, same = 0;
-            for (int i = 0; first + 64 * i < limit; i++) {
-                const uint32_t r = keys[64 * i];
-                const bool mine = first + 64 * i + lane < limit;
-                const uint64_t x = __ballot(mine && r > above), y = __ballot(mine && r == above);
+            over_keys([&](int i, uint32_t r) {
+                const uint64_t x = __ballot(r > above), y = __ballot(r == above);
                 if (lane == i) more = x, same = y;
-            }
+            });
             uint32_t sum;
             if (!all) {
                 const uint32_t before = ties + before_of(__popcll(same), waves, &sum);
@@ -284,13 +342,23 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             const uint32_t at[2] = {lists[0] + (before & 0xffff), lists[1] + (before >> 16)};
             lists[0] += sum & 0xffff;
             lists[1] += sum >> 16;
-            for (int i = 0; first + 64 * i < limit; i++) {
-                const int j = first + 64 * i + lane;
-                const uint64_t one = of_lane(listed[0], i), two = of_lane(listed[1], i);
-                const int k = __builtin_amdgcn_readlane((int)at[0], i) + bits_below(one);
-                const int l = __builtin_amdgcn_readlane((int)at[1], i) + bits_below(two);
-                if (one >> lane & 1) to[k] = e.into ? k : j;
-                if (e.into ? one >> lane & 1 : two >> lane & 1) from[e.into ? k : l] = j;
+            // and writes its own down, each half of the wave 32 bits of the 64
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                if (k && e.into) break;
+                const uint32_t x = __shfl((int)(uint32_t)listed[k], lane & 31);
+                const uint32_t y = __shfl((int)(uint32_t)(listed[k] >> 32), lane & 31);
+                uint32_t left = lane < 32 ? x : y;
+                int i = __shfl((int)at[k], lane & 31) + (lane < 32 ? 0 : __popc(x));
+                for (int j = first + 64 * (lane & 31) + (lane & 32); left; left &= left - 1, i++) {
+                    const int token = j + __builtin_ctz(left);
+                    if (e.into) {
+                        to[i] = i;
+                        from[i] = token;
+                    } else {
+                        (k ? from : to)[i] = token;
+                    }
+                }
             }
         }
         count = lists[0];
@@ -355,7 +423,7 @@ extern "C" int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int
             count + heads + heads * most, count, (int)most};
     const bool here = most <= kMovesHere;
     const int64_t keys = e.bound < kPiece ? e.bound : kPiece;
-    const size_t lds = (size_t)((keys + kSelect - 1) / kSelect * kSelect * 4);
+    const size_t lds = (size_t)((keys + 4 * kSelect - 1) / (4 * kSelect) * (4 * kSelect) * 4);
     if (const int rc = allow_lds()) return rc;
     hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), lds, stream, e, here);
     if (const int rc = (int)hipGetLastError()) return rc;
