@@ -51,12 +51,68 @@ struct Row {
 __device__ __forceinline__ Row row_of(const vramc_kv_cache& c, int page_shift,
                                       const int64_t* __restrict__ slots, int64_t tokens) {
     Row r;
-    r.token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    r.head = blockIdx.y;
+    const uint32_t block = blockIdx.x / c.kv_heads;
+    r.token = (int64_t)block * blockDim.y + threadIdx.y;
+    r.head = blockIdx.x - block * c.kv_heads;
     const int64_t slot = r.token < tokens ? slots[r.token] : -1;
     r.there = slot >= 0 && slot < (int64_t)c.pages << page_shift;
     r.at = (((slot >> page_shift) * c.kv_heads + r.head) << page_shift) + (slot & (c.page_size - 1));
     return r;
+}
+
+// Eight values of a row of the cache, written.
+template <typename T, bool MX>
+__device__ __forceinline__ void store(vec<T, kPer> x, void* held, uint8_t* scales, int64_t at, int per_row,
+                                      int seg) {
+    if constexpr (!MX) {
+        *reinterpret_cast<vec<T, kPer>*>(static_cast<T*>(held) + (at * per_row + seg) * kPer) = x;
+    } else {
+        // a block's threads are four neighbours of a wave
+        uint32_t most = largest(x);
+        most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+        // the scale's byte, floor(log2(most)) - 2 + 127, from the exponent's bits
+        const int bits = (int)(most >> 23);
+        const int byte = bits == 255 ? 255 : max(bits - 2, 0);
+        const uint32_t codes = mx_codes(x, __uint_as_float((uint32_t)byte << 23));
+        static_cast<uint32_t*>(held)[at * per_row + seg] = byte == 255 ? 0 : codes;
+        if (seg % 4 == 0) scales[at * (per_row / 4) + seg / 4] = (uint8_t)byte;
+    }
+}
+
+// Eight values of a row of the cache, read.
+template <typename T, bool MX>
+struct Held {
+    vec<T, kPer> x;
+    uint32_t codes, scale;
+    __device__ __forceinline__ void load(const void* held, const uint8_t* scales, int64_t at, int per_row,
+                                         int seg) {
+        if constexpr (!MX) {
+            x = *reinterpret_cast<const vec<T, kPer>*>(static_cast<const T*>(held) + (at * per_row + seg) * kPer);
+        } else {
+            codes = static_cast<const uint32_t*>(held)[at * per_row + seg];
+            scale = scales[at * (per_row / 4) + seg / 4];
+        }
+    }
+    __device__ __forceinline__ vec<T, kPer> values() const {
+        if constexpr (!MX) {
+            return x;
+        } else {
+            vec<uint32_t, 4> pairs;
+#pragma unroll
+            for (int i = 0; i < 4; i++) pairs[i] = mx_pair_at<T>(codes, scale, i);
+            return __builtin_bit_cast(vec<T, kPer>, pairs);
+        }
+    }
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ vec<T, kPer> load(const T* in) {
+    if constexpr (WIDE) return *reinterpret_cast<const vec<T, kPer>*>(in);
+    vec<T, kPer> x;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) x[j] = in[j];
+    return x;
 }
 
 template <typename T, bool MX, bool WIDE>
@@ -67,34 +123,14 @@ __global__ void __launch_bounds__(kThreads)
                      int64_t tokens) {
     const int per_row = blockDim.x, seg = threadIdx.x;
     const Row r = row_of(c, page_shift, slots, tokens);
+    if (r.token >= tokens) return;
+    // before the slot is known, so that one wait covers both
+    const auto x = load<T, WIDE>(k + r.token * k_token + r.head * k_head + seg * kPer);
+    const auto y = load<T, WIDE>(v + r.token * v_token + r.head * v_head + seg * kPer);
     if (!r.there) return;  // the threads of a block of 32 columns share a row
-    const bool values = blockIdx.z;
-    const T* in = (values ? v + r.token * v_token + r.head * v_head
-                          : k + r.token * k_token + r.head * k_head) + seg * kPer;
-    vec<T, kPer> x;
-    if (WIDE) {
-        x = *reinterpret_cast<const vec<T, kPer>*>(in);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kPer; j++) x[j] = in[j];
-    }
-    if constexpr (!MX) {
-        auto* out = static_cast<T*>(values ? c.v : c.k) + (r.at * per_row + seg) * kPer;
-        *reinterpret_cast<vec<T, kPer>*>(out) = x;
-    } else {
-        // a block's threads are four neighbours of a wave
-        uint32_t most = largest(x);
-        most = max(most, (uint32_t)__shfl_xor((int)most, 1));
-        most = max(most, (uint32_t)__shfl_xor((int)most, 2));
-        // the scale's byte, floor(log2(most)) - 2 + 127, from the exponent's bits
-        const int bits = (int)(most >> 23);
-        const int byte = bits == 255 ? 255 : max(bits - 2, 0);
-        const uint32_t codes = mx_codes(x, __uint_as_float((uint32_t)byte << 23));
-        static_cast<uint32_t*>(values ? c.v : c.k)[r.at * per_row + seg] = byte == 255 ? 0 : codes;
-        if (seg % 4 == 0)
-            (values ? c.v_scale : c.k_scale)[r.at * (per_row / 4) + seg / 4] = (uint8_t)byte;
-    }
-    if (c.mass && !values && seg == 0) {
+    store<T, MX>(x, c.k, c.k_scale, r.at, per_row, seg);
+    store<T, MX>(y, c.v, c.v_scale, r.at, per_row, seg);
+    if (c.mass && seg == 0) {
         c.mass[r.at] = 0.f;
         c.position[r.at] = positions[r.token];
     }
@@ -107,24 +143,17 @@ __global__ void __launch_bounds__(kThreads)
     const int per_row = blockDim.x, seg = threadIdx.x;
     const Row r = row_of(c, page_shift, slots, tokens);
     if (r.token >= tokens) return;
-    const bool values = blockIdx.z;
-    vec<T, kPer> x = {};
+    vec<T, kPer> x = {}, y = {};
     if (r.there) {
-        const void* held = values ? c.v : c.k;
-        const int64_t at = r.at * per_row + seg;
-        if constexpr (!MX) {
-            x = *reinterpret_cast<const vec<T, kPer>*>(static_cast<const T*>(held) + at * kPer);
-        } else {
-            const uint32_t codes = static_cast<const uint32_t*>(held)[at];
-            const uint32_t scale = (values ? c.v_scale : c.k_scale)[r.at * (per_row / 4) + seg / 4];
-            vec<uint32_t, 4> pairs;
-#pragma unroll
-            for (int i = 0; i < 4; i++) pairs[i] = mx_pair_at<T>(codes, scale, i);
-            x = __builtin_bit_cast(vec<T, kPer>, pairs);
-        }
+        Held<T, MX> kh, vh;
+        kh.load(c.k, c.k_scale, r.at, per_row, seg);
+        vh.load(c.v, c.v_scale, r.at, per_row, seg);
+        x = kh.values();
+        y = vh.values();
     }
-    T* out = (values ? v : k) + ((r.token * c.kv_heads + r.head) * per_row + seg) * kPer;
-    *reinterpret_cast<vec<T, kPer>*>(out) = x;
+    const int64_t to = ((r.token * c.kv_heads + r.head) * per_row + seg) * kPer;
+    *reinterpret_cast<vec<T, kPer>*>(k + to) = x;
+    *reinterpret_cast<vec<T, kPer>*>(v + to) = y;
 }
 
 // Whether rows at these strides can be read eight values at a time.
@@ -134,14 +163,15 @@ bool wide(const void* p, int64_t token, int64_t head) {
             (uintptr_t)(head * (int64_t)sizeof(T))) % (kPer * sizeof(T)) == 0;
 }
 
-// Workgroups of whole rows of one head, neighbouring tokens each.
+// Workgroups of whole rows of one head, neighbouring tokens each, the heads of
+// a token next to each other in time, as they lie in memory; 0 for too many.
 struct Shape {
     dim3 grid, block;
 };
 Shape shape_of(const vramc_kv_cache& c, int64_t tokens) {
     const int per_row = c.head_dim / kPer, rows = kThreads / per_row;
-    return {dim3((unsigned)((tokens + rows - 1) / rows), (unsigned)c.kv_heads, 2),
-            dim3((unsigned)per_row, (unsigned)rows)};
+    const int64_t n = (tokens + rows - 1) / rows * c.kv_heads;
+    return {dim3(n > INT32_MAX ? 0 : (unsigned)n), dim3((unsigned)per_row, (unsigned)rows)};
 }
 
 template <typename T, bool MX>
@@ -150,6 +180,7 @@ int append(const vramc_kv_cache& c, const void* k, int64_t k_token, int64_t k_he
            int64_t tokens, hipStream_t stream) {
     const auto *kp = static_cast<const T*>(k), *vp = static_cast<const T*>(v);
     const Shape s = shape_of(c, tokens);
+    if (!s.grid.x) return RANS_EARG;
     const int shift = __builtin_ctz(c.page_size);
     if (wide<T>(k, k_token, k_head) && wide<T>(v, v_token, v_head))
         hipLaunchKernelGGL((kv_append_kernel<T, MX, true>), s.grid, s.block, 0, stream, c, shift, kp,
@@ -164,6 +195,7 @@ template <typename T, bool MX>
 int read(const vramc_kv_cache& c, const int64_t* slots, int64_t tokens, void* k, void* v,
          hipStream_t stream) {
     const Shape s = shape_of(c, tokens);
+    if (!s.grid.x) return RANS_EARG;
     hipLaunchKernelGGL((kv_read_kernel<T, MX>), s.grid, s.block, 0, stream, c,
                        __builtin_ctz(c.page_size), slots, static_cast<T*>(k), static_cast<T*>(v), tokens);
     return (int)hipGetLastError();
@@ -176,7 +208,7 @@ extern "C" int vramc_kv_append(const vramc_kv_cache* c, const void* k, int64_t k
                                const int64_t* slots, const int32_t* positions, int64_t tokens,
                                hipStream_t stream) {
     if (const int rc = check_cache(c)) return rc;
-    if (tokens < 0 || tokens > INT32_MAX) return RANS_EARG;
+    if (tokens < 0 || tokens > INT64_MAX / 65536) return RANS_EARG;
     if (tokens == 0) return 0;
     if (!k || !v || !slots || (c->mass && !positions)) return RANS_EARG;
     const auto go = [&](auto fn) {
@@ -190,7 +222,7 @@ extern "C" int vramc_kv_append(const vramc_kv_cache* c, const void* k, int64_t k
 extern "C" int vramc_kv_read(const vramc_kv_cache* c, const int64_t* slots, int64_t tokens,
                              void* k_out, void* v_out, hipStream_t stream) {
     if (const int rc = check_cache(c)) return rc;
-    if (tokens < 0 || tokens > INT32_MAX) return RANS_EARG;
+    if (tokens < 0 || tokens > INT64_MAX / 65536) return RANS_EARG;
     if (tokens == 0) return 0;
     if (!slots || !k_out || !v_out || ((uintptr_t)k_out | (uintptr_t)v_out) % 32) return RANS_EARG;
     const auto go = [&](auto fn) { return fn(*c, slots, tokens, k_out, v_out, stream); };

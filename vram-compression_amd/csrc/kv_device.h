@@ -41,7 +41,7 @@ __device__ __forceinline__ uint32_t mx_pair_at(uint32_t codes, uint32_t scale, i
 
 // The checks of every entry point.
 inline int check_cache(const vramc_kv_cache* c) {
-    if (!c || !c->k || !c->v || c->pages <= 0 || c->kv_heads <= 0 || c->kv_heads > 65535) return RANS_EARG;
+    if (!c || !c->k || !c->v || c->pages <= 0 || c->kv_heads <= 0) return RANS_EARG;
     switch (c->page_size) {
         case 16: case 32: case 64: case 128: case 256: break;
         default: return RANS_EUNSUPPORTED;
