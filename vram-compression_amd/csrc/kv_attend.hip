@@ -62,6 +62,7 @@ struct Attend {
     void* out;
     int chunk, splits;       // keys of a part, parts of the longest possible sequence
     int head_tiles;
+    int page_shift;
     int bound;               // tokens that a row of the table has room for
     float* scores;           // [batch * q_heads][bound], log2, where weights are tracked
     float* parts;            // [batch * q_heads][splits][dim]
@@ -130,21 +131,23 @@ struct Keys {
     Raw<BYTES> x[N];
     uint32_t scale[BLOCKS ? BLOCKS : 1];
 
+    // row0: the tile's first row, the same for all lanes
     __device__ __forceinline__ void load(const vramc_kv_cache& c, int64_t row0, int lane) {
-        const int g = lane >> 4;
-        const int64_t row = row0 + (lane & 15);
+        const uint32_t g = lane >> 4, n = lane & 15;
         if constexpr (MX) {
-            x[0] = load_raw<BYTES, BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : 4>(
-                static_cast<const uint8_t*>(c.k) + row * (D / 2) + g * BYTES);
-            const uint8_t* s = c.k_scale + row * (D / kMxBlock) + g * (D / 4) / kMxBlock;
-            scale[0] = s[0];
+            const uint8_t* p = static_cast<const uint8_t*>(c.k) + row0 * (D / 2);
+            x[0] = load_raw<BYTES, BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : 4>(p + (n * (D / 2) + g * BYTES));
+            const uint8_t* s = c.k_scale + row0 * (D / kMxBlock);
+            const uint32_t at = n * (D / kMxBlock) + g * (D / 4) / kMxBlock;
+            scale[0] = s[at];
             // the last lanes of 96 and 192 columns end in their first block
             if constexpr (BLOCKS == 2)
-                scale[1] = s[(g * (D / 4) + D / 4 - 1) / kMxBlock - g * (D / 4) / kMxBlock];
+                scale[1] = s[at + ((g * (D / 4) + D / 4 - 1) / kMxBlock - g * (D / 4) / kMxBlock)];
         } else {
-            const uint8_t* p = static_cast<const uint8_t*>(c.k) + row * (D * (int)sizeof(T)) + g * 16;
+            const uint8_t* p = static_cast<const uint8_t*>(c.k) + row0 * (D * (int)sizeof(T));
 #pragma unroll
-            for (int s = 0; s < N; s++) x[s] = load_raw<16, 16>(p + s * 64);
+            for (int s = 0; s < N; s++)
+                x[s] = load_raw<16, 16>(p + (n * (uint32_t)(D * sizeof(T)) + g * 16) + s * 64);
         }
     }
     // The first column of the lane's chunk s.
@@ -180,18 +183,19 @@ struct Values {
     uint32_t scale0[MX ? KEYS : 1], scale1[MX && B1 ? KEYS : 1];
 
     __device__ __forceinline__ void load(const vramc_kv_cache& c, const int64_t* row0, int lane) {
-        const int n = lane & 15, g = lane >> 4;
+        const uint32_t n = lane & 15, g = lane >> 4;
+        constexpr int ROW = D * SIZE / 2, SCALES = D / kMxBlock;
         constexpr int A0 = B0 < 16 ? B0 : 16, A1 = B1 ? B1 : 1;
 #pragma unroll
         for (int j = 0; j < KEYS; j++) {
-            const int64_t row = row0[j >> 2] + 4 * g + (j & 3);
-            const uint8_t* p = static_cast<const uint8_t*>(c.v) + row * (D * SIZE / 2);
-            x0[j] = load_raw<B0, A0>(p + n * B0);
-            if constexpr (B1 > 0) x1[j] = load_raw<B1, A1>(p + 16 * B0 + n * B1);
+            const uint8_t* p = static_cast<const uint8_t*>(c.v) + row0[j >> 2] * ROW;
+            x0[j] = load_raw<B0, A0>(p + (g * (4 * ROW) + n * B0) + (j & 3) * ROW);
+            if constexpr (B1 > 0) x1[j] = load_raw<B1, A1>(p + (g * (4 * ROW) + n * B1) + ((j & 3) * ROW + 16 * B0));
             if constexpr (MX) {
-                const uint8_t* s = c.v_scale + row * (D / kMxBlock);
-                scale0[j] = s[n * C::L0 / kMxBlock];
-                if constexpr (B1 > 0) scale1[j] = s[(C::P0 + n * C::L1) / kMxBlock];
+                const uint8_t* s = c.v_scale + row0[j >> 2] * SCALES;
+                scale0[j] = *(s + (g * (4 * SCALES) + n * C::L0 / kMxBlock) + (j & 3) * SCALES);
+                if constexpr (B1 > 0)
+                    scale1[j] = *(s + (g * (4 * SCALES) + (C::P0 + n * C::L1) / kMxBlock) + (j & 3) * SCALES);
             }
         }
     }
@@ -227,12 +231,19 @@ struct Values {
     }
 };
 
+// Waves of a SIMD that the registers are to allow.  Two cap them at 256, which
+// also keeps the sums in ordinary registers instead of accumulation registers,
+// from where every rescaling would have to copy them.
+template <typename T, int D>
+constexpr int kWavesOfSimd = D <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
+
 template <typename T, bool MX, int D>
-__global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
+__global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(Attend a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int TILES = F32 ? 1 : 2;       // of 16 keys in a step
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
     constexpr int NT = D / 16;               // tiles of the output
+    constexpr int AHEAD = !MX ? 1 : D == 96 ? 3 : D <= 128 ? 4 : 2;
     using C = Deal<D>;
     const int split = blockIdx.x % a.splits;
     int rest = blockIdx.x / a.splits;
@@ -270,38 +281,47 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
     int pages = -1;
     {
         const int key = start + (wave + kWaves * (lane / TILES)) * STEP + lane % TILES * 16;
-        if (key < end) pages = a.table[b * a.table_row + key / a.c.page_size];
+        if (key < end) pages = a.table[b * a.table_row + (key >> a.page_shift)];
         if ((uint32_t)pages >= (uint32_t)a.c.pages) pages = -1;
     }
-    int page[TILES];
-    int64_t row[TILES];
-    const auto find = [&](int t) {  // the rows of step t; page 0 stands in for a missing one
+    // A step's keys and values as they arrive: AHEAD steps are in flight, so that
+    // a wave has some 8 KB on the way whatever the type.
+    struct Step {
+        Keys<T, MX, D> k[TILES];
+        Values<T, MX, D, KEYS> v;
+        int page[TILES];
+        int64_t row[TILES];
+    } step[AHEAD];
+    const auto find = [&](Step& x, int t) {  // page 0 stands in for a missing one
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            page[i] = __builtin_amdgcn_readlane(pages, t / kWaves * TILES + i);
-            row[i] = ((int64_t)max(page[i], 0) * a.c.kv_heads + h) * a.c.page_size +
-                     (start + t * STEP + i * 16) % a.c.page_size;
+            x.page[i] = __builtin_amdgcn_readlane(pages, t / kWaves * TILES + i);
+            x.row[i] = (((int64_t)max(x.page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
+                       ((start + t * STEP + i * 16) & (a.c.page_size - 1));
         }
     };
+    const auto load_keys = [&](Step& x) {
+#pragma unroll
+        for (int i = 0; i < TILES; i++) x.k[i].load(a.c, x.row[i], lane);
+    };
 
-    Keys<T, MX, D> k[TILES];
-    Values<T, MX, D, KEYS> v;
     vec<float, 4> o[NT] = {};
     float m = -__builtin_inff(), from = 0.f, l = 0.f;
     const float scale = a.scale * kLog2e;
-    if (wave < steps) {
-        find(wave);
 #pragma unroll
-        for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
-        v.load(a.c, row, lane);
-    }
-    for (int t = wave; t < steps; t += kWaves) {
+    for (int u = 0; u < AHEAD; u++)
+        if (wave + u * kWaves < steps) {
+            find(step[u], wave + u * kWaves);
+            load_keys(step[u]);
+            step[u].v.load(a.c, step[u].row, lane);
+        }
+    const auto compute = [&](Step& x, int t) {
         const int key0 = start + t * STEP;
         bool whole = key0 + STEP <= end;
         bool there[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            there[i] = page[i] >= 0;
+            there[i] = x.page[i] >= 0;
             whole &= there[i];
         }
         vec<float, 4> s[TILES] = {};
@@ -312,20 +332,18 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
                 for (int c = 0; c < D / 16; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
+                        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[i].x[c].w[e]),
                                                                     qf[c][e], s[i], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) s[i] = mma(k[i].operand(c, g), q[c], s[i]);
+                for (int c = 0; c < D / 32; c++) s[i] = mma(x.k[i].operand(c, g), q[c], s[i]);
             }
         }
-        const bool more = t + kWaves < steps;
-        if (more) {
-            find(t + kWaves);
-#pragma unroll
-            for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
+        const int next = t + AHEAD * kWaves;
+        if (next < steps) {
+            find(x, next);
+            load_keys(x);
         }
-        float top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < TILES; i++)
 #pragma unroll
@@ -337,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
                 for (int e = 0; e < 4; e++) {
                     const bool gone = !there[i] || key0 + 16 * i + 4 * g + e >= end;
                     if (gone) s[i][e] = -__builtin_inff();
-                    v.clear(4 * i + e, gone);
+                    x.v.clear(4 * i + e, gone);
                 }
         }
         if (a.scores && live) {
@@ -346,11 +364,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
                 if (key0 + 16 * i < a.bound)
                     *reinterpret_cast<vec<float, 4>*>(a.scores + q_row * a.bound + key0 + 16 * i + 4 * g) = s[i];
         }
+        float top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < TILES; i++)
 #pragma unroll
             for (int e = 0; e < 4; e++) top = fmaxf(top, s[i][e]);
-        if (__any(top > m + kSlack<T>)) {
+        if (__builtin_expect(__any(top > m + kSlack<T>), 0)) {
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             if (top > m + kSlack<T>) {
@@ -373,29 +392,36 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(Attend a) {
             for (int j = 0; j < KEYS; j++)
 #pragma unroll
                 for (int i = 0; i < NT; i++)
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[j], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v.value(i, j), p[j], o[i], 0, 0, 0);
         } else {
-            Half8<T> hi, lo;
+            vec<T, 2> hi2[4], lo2[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                hi[j] = (T)p[j];
-                lo[j] = (T)(p[j] - (float)hi[j]);
+            for (int j = 0; j < 4; j++) {
+                const vec<float, 2> w = {p[2 * j], p[2 * j + 1]};
+                hi2[j] = __builtin_convertvector(w, vec<T, 2>);
+                lo2[j] = __builtin_convertvector(w - __builtin_convertvector(hi2[j], vec<float, 2>), vec<T, 2>);
             }
+            const auto hi = __builtin_bit_cast(Half8<T>, hi2), lo = __builtin_bit_cast(Half8<T>, lo2);
 #pragma unroll
             for (int i = 0; i < NT / 2; i++) {
                 vec<uint32_t, 4> even, odd;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t x = v.pair(i, 2 * j), y = v.pair(i, 2 * j + 1);
-                    even[j] = __builtin_amdgcn_perm(y, x, 0x05040100);
-                    odd[j] = __builtin_amdgcn_perm(y, x, 0x07060302);
+                    const uint32_t y = x.v.pair(i, 2 * j), z = x.v.pair(i, 2 * j + 1);
+                    even[j] = __builtin_amdgcn_perm(z, y, 0x05040100);
+                    odd[j] = __builtin_amdgcn_perm(z, y, 0x07060302);
                 }
                 const auto e = __builtin_bit_cast(Half8<T>, even), f = __builtin_bit_cast(Half8<T>, odd);
                 o[2 * i] = mma(e, lo, mma(e, hi, o[2 * i]));
                 o[2 * i + 1] = mma(f, lo, mma(f, hi, o[2 * i + 1]));
             }
         }
-        if (more) v.load(a.c, row, lane);
+        if (next < steps) x.v.load(a.c, x.row, lane);
+    };
+    for (int t = wave; t < steps; t += AHEAD * kWaves) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++)
+            if (t + u * kWaves < steps) compute(step[u], t + u * kWaves);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
@@ -519,9 +545,9 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins) {
             }
     }
     if (key >= n) return;
-    const int page = a.table[b * a.table_row + key / a.c.page_size];
+    const int page = a.table[b * a.table_row + (key >> a.page_shift)];
     if (page < 0 || page >= a.c.pages) return;
-    float* mass = a.c.mass + ((int64_t)page * a.c.kv_heads + h) * a.c.page_size + key % a.c.page_size;
+    float* mass = a.c.mass + ((int64_t)page * a.c.kv_heads + h) * a.c.page_size + (key & (a.c.page_size - 1));
     for (int e = 0; e < 4; e++)
         if (key + e < n) unsafeAtomicAdd(mass + e, w[e]);
 }
@@ -601,7 +627,7 @@ extern "C" int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q
     const int64_t rows = (int64_t)batch * q_heads;
     Attend a{*c, q, q_seq, q_head, q_heads, q_heads / c->kv_heads, table, table_row, table_width,
              lengths, batch, scale, out, p.chunk, p.splits, p.head_tiles,
-             table_width * c->page_size, nullptr, nullptr, nullptr};
+             __builtin_ctz(c->page_size), table_width * c->page_size, nullptr, nullptr, nullptr};
     auto* work = static_cast<float*>(workspace);
     if (p.splits > 1) {
         a.parts = work;
