@@ -26,9 +26,11 @@
 //    rounded weight and the rounding's remainder, 16 or more bits together:
 //    one alone would make the weights' rounding as large as the output's own.
 //
-// The length is split over workgroups, whose waves take turns of 32 keys (16
-// in f32); parts are joined in a second launch, which also adds the weights to
-// the tokens' mass where that is tracked.
+// The work is all tokens of all kv heads behind each other, in units of 128 keys,
+// and every workgroup that the card holds at once takes an equal share of it:
+// the lengths, which only the GPU knows, decide how many workgroups a sequence
+// gets.  A share that ends inside a sequence leaves a part; a second launch joins
+// the parts, and adds the weights to the tokens' mass where that is tracked.
 #include "kv_device.h"
 
 namespace {
@@ -36,7 +38,8 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kHeadTile = 16;     // query heads of a workgroup
-constexpr int kMaxChunk = 4096;   // keys of a workgroup: its waves keep their page ids in lanes
+constexpr int kUnit = 128;        // keys that work is dealt in: a step of every wave
+constexpr int kMinUnits = 1;      // of a workgroup's share
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The reference is set this far below the largest score so far, and again when
@@ -52,6 +55,7 @@ struct Attend {
     vramc_kv_cache c;
     const void* q;
     int64_t q_seq, q_head;
+    bool q_wide;             // rows of q can be read 16 bytes at a time
     int q_heads, group;
     const int32_t* table;
     int64_t table_row;
@@ -60,40 +64,79 @@ struct Attend {
     int batch;
     float scale;
     void* out;
-    int chunk, splits;       // keys of a part, parts of the longest possible sequence
-    int head_tiles;
+    int head_tiles, groups;  // tiles of a kv head's queries; tiles of all kv heads
     int page_shift;
     int bound;               // tokens that a row of the table has room for
+    // Workgroup w leaves the part that starts a group in slot 2w + 1 and one
+    // that goes on from the workgroup before it in 2w.
+    float* parts;            // [slots][16][dim]
+    float2* part_sums;       // [slots][16]: reference (log2) and sum
+    int2* spans;             // [batch][groups]: first workgroup of a group, number of parts
     float* scores;           // [batch * q_heads][bound], log2, where weights are tracked
-    float* parts;            // [batch * q_heads][splits][dim]
-    float2* sums;            // [batch * q_heads][splits]: reference (log2) and sum
+    float2* sums;            // [batch * q_heads], of groups in one part, where they are
 };
 
 __device__ __forceinline__ int length_of(const Attend& a, int b) {
     return min(max(a.lengths[b], 0), a.bound);
 }
 
+__device__ __forceinline__ int units_of(int n) { return (n + kUnit - 1) / kUnit; }
+
+// How units are dealt to workgroups: `rest` of them get one more than the others.
+struct Shares {
+    uint32_t workers, each, rest;
+    __device__ __forceinline__ Shares(uint32_t units, uint32_t most) {
+        workers = min(most, (units + kMinUnits - 1) / kMinUnits);
+        each = workers ? units / workers : 0;
+        rest = units - each * workers;
+    }
+    __device__ __forceinline__ uint32_t start(uint32_t w) const { return w * each + min(w, rest); }
+    __device__ __forceinline__ uint32_t worker_of(uint32_t unit) const {
+        const uint32_t longer = rest * (each + 1);
+        return unit < longer ? unit / (each + 1) : rest + (unit - longer) / each;
+    }
+};
+
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 0 in the place of a reference for nothing, so that differences stay numbers.
 __device__ __forceinline__ float or_zero(float m) { return m == -__builtin_inff() ? 0.f : m; }
 
-// BYTES bytes of memory in registers, from an address aligned to ALIGN.
+// An address that all lanes share, kept apart from what a lane adds to it: loads
+// then take it from scalar registers and the lane's 32 bits beside it.
+using global_ptr = const __attribute__((address_space(1))) uint8_t*;
+__device__ __forceinline__ global_ptr shared_address(const void* p, int64_t off) {
+    uint64_t at = (uint64_t)p + off;
+    asm("" : "+s"(at));
+    return (global_ptr)at;
+}
+
+// BYTES bytes of memory in registers, from an address aligned to 4 or to BYTES.
 template <int BYTES>
 struct Raw {
     uint32_t w[BYTES < 4 ? 1 : BYTES / 4];
 };
-template <int BYTES, int ALIGN>
-__device__ __forceinline__ Raw<BYTES> load_raw(const uint8_t* p) {
+template <int N>
+using words = uint32_t __attribute__((ext_vector_type(N), aligned(4)));
+template <int BYTES>
+__device__ __forceinline__ Raw<BYTES> load_raw(global_ptr p) {
     Raw<BYTES> r;
     if constexpr (BYTES == 0) {
         r.w[0] = 0;
     } else if constexpr (BYTES == 1) {
         r.w[0] = *p;
     } else if constexpr (BYTES == 2) {
-        r.w[0] = *reinterpret_cast<const uint16_t*>(p);
+        r.w[0] = *reinterpret_cast<const __attribute__((address_space(1))) uint16_t*>(p);
+    } else if constexpr (BYTES == 4) {
+        r.w[0] = *reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(p);
     } else {
-        __builtin_memcpy(r.w, __builtin_assume_aligned(p, ALIGN), BYTES);
+        constexpr int N = BYTES / 4 <= 4 ? BYTES / 4 : BYTES % 16 == 0 ? 4 : 2;  // words of a load
+#pragma unroll
+        for (int i = 0; i < BYTES / 4; i += N) {
+            const auto x = *reinterpret_cast<const __attribute__((address_space(1))) words<N>*>(p + 4 * i);
+#pragma unroll
+            for (int j = 0; j < N; j++) r.w[i + j] = x[j];
+        }
     }
     return r;
 }
@@ -135,19 +178,18 @@ struct Keys {
     __device__ __forceinline__ void load(const vramc_kv_cache& c, int64_t row0, int lane) {
         const uint32_t g = lane >> 4, n = lane & 15;
         if constexpr (MX) {
-            const uint8_t* p = static_cast<const uint8_t*>(c.k) + row0 * (D / 2);
-            x[0] = load_raw<BYTES, BYTES % 16 == 0 ? 16 : BYTES % 8 == 0 ? 8 : 4>(p + (n * (D / 2) + g * BYTES));
-            const uint8_t* s = c.k_scale + row0 * (D / kMxBlock);
+            x[0] = load_raw<BYTES>(shared_address(c.k, row0 * (D / 2)) + (n * (D / 2) + g * BYTES));
+            const global_ptr s = shared_address(c.k_scale, row0 * (D / kMxBlock));
             const uint32_t at = n * (D / kMxBlock) + g * (D / 4) / kMxBlock;
             scale[0] = s[at];
             // the last lanes of 96 and 192 columns end in their first block
             if constexpr (BLOCKS == 2)
                 scale[1] = s[at + ((g * (D / 4) + D / 4 - 1) / kMxBlock - g * (D / 4) / kMxBlock)];
         } else {
-            const uint8_t* p = static_cast<const uint8_t*>(c.k) + row0 * (D * (int)sizeof(T));
+            const global_ptr p = shared_address(c.k, row0 * (D * (int)sizeof(T)));
 #pragma unroll
             for (int s = 0; s < N; s++)
-                x[s] = load_raw<16, 16>(p + (n * (uint32_t)(D * sizeof(T)) + g * 16) + s * 64);
+                x[s] = load_raw<16>(p + (n * (uint32_t)(D * sizeof(T)) + g * 16) + s * 64);
         }
     }
     // The first column of the lane's chunk s.
@@ -185,17 +227,22 @@ struct Values {
     __device__ __forceinline__ void load(const vramc_kv_cache& c, const int64_t* row0, int lane) {
         const uint32_t n = lane & 15, g = lane >> 4;
         constexpr int ROW = D * SIZE / 2, SCALES = D / kMxBlock;
-        constexpr int A0 = B0 < 16 ? B0 : 16, A1 = B1 ? B1 : 1;
 #pragma unroll
-        for (int j = 0; j < KEYS; j++) {
-            const uint8_t* p = static_cast<const uint8_t*>(c.v) + row0[j >> 2] * ROW;
-            x0[j] = load_raw<B0, A0>(p + (g * (4 * ROW) + n * B0) + (j & 3) * ROW);
-            if constexpr (B1 > 0) x1[j] = load_raw<B1, A1>(p + (g * (4 * ROW) + n * B1) + ((j & 3) * ROW + 16 * B0));
+        for (int i = 0; i < KEYS / 4; i++) {
+            const global_ptr p = shared_address(c.v, row0[i] * ROW);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x0[4 * i + e] = load_raw<B0>(p + (g * (4 * ROW) + n * B0) + e * ROW);
+                if constexpr (B1 > 0) x1[4 * i + e] = load_raw<B1>(p + (g * (4 * ROW) + n * B1) + (e * ROW + 16 * B0));
+            }
             if constexpr (MX) {
-                const uint8_t* s = c.v_scale + row0[j >> 2] * SCALES;
-                scale0[j] = *(s + (g * (4 * SCALES) + n * C::L0 / kMxBlock) + (j & 3) * SCALES);
-                if constexpr (B1 > 0)
-                    scale1[j] = *(s + (g * (4 * SCALES) + (C::P0 + n * C::L1) / kMxBlock) + (j & 3) * SCALES);
+                const global_ptr s = shared_address(c.v_scale, row0[i] * SCALES);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    scale0[4 * i + e] = *(s + (g * (4 * SCALES) + n * C::L0 / kMxBlock) + e * SCALES);
+                    if constexpr (B1 > 0)
+                        scale1[4 * i + e] = *(s + (g * (4 * SCALES) + (C::P0 + n * C::L1) / kMxBlock) + e * SCALES);
+                }
             }
         }
     }
@@ -235,7 +282,7 @@ struct Values {
 // also keeps the sums in ordinary registers instead of accumulation registers,
 // from where every rescaling would have to copy them.
 template <typename T, int D>
-constexpr int kWavesOfSimd = D <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
+constexpr int kWavesOfSimd = D <= (sizeof(T) == 4 ? 96 : 128) ? 3 : D <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
 
 template <typename T, bool MX, int D>
 __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(Attend a) {
@@ -243,18 +290,63 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
     constexpr int TILES = F32 ? 1 : 2;       // of 16 keys in a step
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
     constexpr int NT = D / 16;               // tiles of the output
-    constexpr int AHEAD = !MX ? 1 : D == 96 ? 3 : D <= 128 ? 4 : 2;
+    constexpr int AHEAD = !MX ? 1 : 2;
     using C = Deal<D>;
-    const int split = blockIdx.x % a.splits;
-    int rest = blockIdx.x / a.splits;
-    const int first_head = rest % a.head_tiles * kHeadTile;
-    rest /= a.head_tiles;
-    const int h = rest % a.c.kv_heads, b = rest / a.c.kv_heads;
-    const int n = length_of(a, b), start = split * a.chunk;
-    if (start >= n && split) return;
-    const int end = min(n, start + a.chunk);
+    __shared__ int wave_units[kWaves], place[2];
+    __shared__ float part[2][NT * 4 + 2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g = lane >> 4, head = first_head + (lane & 15);
+    const int g = lane >> 4;
+
+    // this workgroup's share: each thread counts some sequences' units
+    const int each = (a.batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
+    int mine = 0;
+    for (int i = b0; i < min(b0 + each, a.batch); i++) mine += units_of(length_of(a, i));
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(sum, d);
+        sum += lane >= d ? x : 0;
+    }
+    if (lane == 63) wave_units[wave] = sum;
+    __syncthreads();
+    int before = sum - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        before += w < wave ? wave_units[w] : 0;
+        total += wave_units[w];
+    }
+    const Shares shares(__builtin_amdgcn_readfirstlane(total) * (uint32_t)a.groups, gridDim.x);
+    for (int i = blockIdx.x; i < a.batch; i += gridDim.x)  // nothing to attend to
+        if (length_of(a, i) == 0) {
+            T* to = static_cast<T*>(a.out) + (int64_t)i * a.q_heads * D;
+            for (int x = threadIdx.x; x < a.q_heads * D; x += kThreads) to[x] = (T)0.f;
+            for (int x = threadIdx.x; x < a.groups; x += kThreads) a.spans[(int64_t)i * a.groups + x] = make_int2(0, 0);
+        }
+    if (blockIdx.x >= shares.workers) return;
+    uint32_t unit = shares.start(blockIdx.x);
+    const uint32_t stop = shares.start(blockIdx.x + 1);
+    if (unit >= (uint32_t)before * a.groups && unit < (uint32_t)(before + mine) * a.groups) {
+        uint32_t off = unit - (uint32_t)before * a.groups;
+        int i = b0;
+        for (uint32_t x; off >= (x = (uint32_t)units_of(length_of(a, i)) * a.groups); i++) off -= x;
+        place[0] = i;
+        place[1] = (int)off;
+    }
+    __syncthreads();
+    int b = __builtin_amdgcn_readfirstlane(place[0]), off = __builtin_amdgcn_readfirstlane(place[1]);
+    const float scale = a.scale * kLog2e;
+
+    while (unit < stop) {
+    const int n = __builtin_amdgcn_readfirstlane(length_of(a, b)), units = units_of(n);
+    const int group = off / units, first_unit = off - group * units;
+    const int here = min((uint32_t)(units - first_unit), stop - unit);
+    const int h = group / a.head_tiles, first_head = group % a.head_tiles * kHeadTile;
+    const int start = first_unit * kUnit, end = min(n, (first_unit + here) * kUnit);
+    const bool opens = first_unit == 0, alone = here == units;
+    if (opens && threadIdx.x == 0)
+        a.spans[(int64_t)b * a.groups + group] =
+            make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + units - 1) - blockIdx.x + 1);
+    const int head = first_head + (lane & 15);
     const bool live = head < a.group;
     const int64_t q_row = (int64_t)b * a.q_heads + h * a.group + head;
 
@@ -262,30 +354,42 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
     Half8<T> q[F32 ? 1 : D / 32];
     vec<float, 4> qf[F32 ? D / 16 : 1];
     {
-        const T* p = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)(h * a.group + head) * a.q_head;
-        if constexpr (F32) {
+        constexpr int N = F32 ? 4 : 8;
+        const T* p = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)(h * a.group + (live ? head : first_head)) * a.q_head;
+        const auto take = [&](int s, auto& x) {
+            const T* from = p + Keys<T, MX, D>::column(s, g);
+            if (a.q_wide) {
+                x = *reinterpret_cast<const vec<T, N>*>(from);
+            } else {
 #pragma unroll
-            for (int s = 0; s < D / 16; s++)
+                for (int i = 0; i < N; i++) x[i] = from[i];
+            }
+        };
 #pragma unroll
-                for (int i = 0; i < 4; i++) qf[s][i] = live ? p[Keys<T, MX, D>::column(s, g) + i] : 0.f;
-        } else {
+        for (int s = 0; s < D / (F32 ? 16 : 32); s++) {
+            if constexpr (F32) take(s, qf[s]);
+            else take(s, q[s]);
+        }
+        if (!live) {
 #pragma unroll
-            for (int s = 0; s < D / 32; s++)
+            for (auto& x : q) x = {};
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[s][i] = live ? p[Keys<T, MX, D>::column(s, g) + i] : (T)0.f;
+            for (auto& x : qf) x = {};
         }
     }
 
-    // page ids of this wave's steps, one tile of 16 keys a lane
-    const int steps = end > start ? (end - start + STEP - 1) / STEP : 0;
-    int pages = -1;
-    {
-        const int key = start + (wave + kWaves * (lane / TILES)) * STEP + lane % TILES * 16;
-        if (key < end) pages = a.table[b * a.table_row + (key >> a.page_shift)];
-        if ((uint32_t)pages >= (uint32_t)a.c.pages) pages = -1;
-    }
-    // A step's keys and values as they arrive: AHEAD steps are in flight, so that
-    // a wave has some 8 KB on the way whatever the type.
+    // Page ids of 64 of this wave's tiles of 16 keys, one a lane; the next 64 are
+    // fetched while these are used.
+    const int steps = (end - start + STEP - 1) / STEP;
+    const auto page_ids = [&](int window) {
+        const int tile = window * 64 + lane;
+        const int key = start + (wave + kWaves * (tile / TILES)) * STEP + tile % TILES * 16;
+        int id = -1;
+        if (key < end) id = a.table[b * a.table_row + (key >> a.page_shift)];
+        return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
+    };
+    int window = 0, ids = page_ids(0), next_ids = page_ids(1);
+    // A step's keys and values as they arrive, AHEAD steps in flight.
     struct Step {
         Keys<T, MX, D> k[TILES];
         Values<T, MX, D, KEYS> v;
@@ -293,9 +397,14 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
         int64_t row[TILES];
     } step[AHEAD];
     const auto find = [&](Step& x, int t) {  // page 0 stands in for a missing one
+        const int tile = t / kWaves * TILES;
+        if (tile / 64 != window) {
+            ids = next_ids;
+            next_ids = page_ids(++window + 1);
+        }
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            x.page[i] = __builtin_amdgcn_readlane(pages, t / kWaves * TILES + i);
+            x.page[i] = __builtin_amdgcn_readlane(ids, tile % 64 + i);
             x.row[i] = (((int64_t)max(x.page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
                        ((start + t * STEP + i * 16) & (a.c.page_size - 1));
         }
@@ -307,7 +416,6 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
 
     vec<float, 4> o[NT] = {};
     float m = -__builtin_inff(), from = 0.f, l = 0.f;
-    const float scale = a.scale * kLog2e;
 #pragma unroll
     for (int u = 0; u < AHEAD; u++)
         if (wave + u * kWaves < steps) {
@@ -427,7 +535,6 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
     l += __shfl_xor(l, 32);
 
     // the waves' parts, joined in two rounds through LDS, register by register
-    __shared__ float part[2][NT * 4 + 2][64];
 #pragma unroll
     for (int half = kWaves / 2; half; half /= 2) {
         if (wave >= half && wave < 2 * half) {
@@ -449,151 +556,204 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
         }
         __syncthreads();
     }
-    if (wave || !live) return;
-    const bool alone = n <= a.chunk;
-    if ((!alone || a.scores) && g == 0) a.sums[q_row * a.splits + split] = make_float2(m, l);
-    if (alone) {
-        const float x = l == 0.f ? 0.f : 1.f / l;
-        T* to = static_cast<T*>(a.out) + q_row * D;
+    if (wave == 0 && live) {
+        if (alone) {
+            if (a.scores && g == 0) a.sums[q_row] = make_float2(m, l);
+            const float x = l == 0.f ? 0.f : 1.f / l;
+            T* to = static_cast<T*>(a.out) + q_row * D;
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+            for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = (T)(l == 0.f ? 0.f : o[i][e] * x);
-    } else {
-        float* to = a.parts + (q_row * a.splits + split) * D;
+                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = (T)(l == 0.f ? 0.f : o[i][e] * x);
+        } else {
+            const int64_t row = (int64_t)(2 * blockIdx.x + opens) * kHeadTile + (lane & 15);
+            if (g == 0) a.part_sums[row] = make_float2(m, l);
+            float* to = a.parts + row * D;
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+            for (int i = 0; i < NT; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = o[i][e];
+                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = o[i][e];
+        }
+    }
+    unit += here;
+    off += here;
+    if (off == units * a.groups) {  // on to the next sequence that has tokens
+        off = 0;
+        do b++;
+        while (unit < stop && __builtin_amdgcn_readfirstlane(length_of(a, b)) == 0);
+    }
     }
 }
 
-// What is left when all parts are there.  The first blocks join the parts of a
-// query head each; the others add the weights of 1024 tokens of a kv head to
-// their mass, from the scores that the first launch left.
-constexpr int kMassKeys = 4 * kThreads;
+// What is left when all parts are there.  The first blocks join the parts of 32
+// columns of a query head each; the others add the weights of 1024 tokens of a
+// kv head to their mass, from the scores that the first launch left.
+constexpr int kJoinColumns = 32, kJoinLanes = kJoinColumns / 4, kJoinParts = kThreads / kJoinLanes;
+constexpr int kMassKeys = 4 * kThreads, kMassHeads = 8;
+
+// The rows of a query head's parts, in order: slot 2w + 1 of the workgroup that
+// opens it, then slots 2w.
+struct Parts {
+    int64_t first;
+    int count;
+    __device__ __forceinline__ Parts(const Attend& a, int b, int q_head) {
+        const int h = q_head / a.group, in = q_head - h * a.group;
+        const int2 span = a.spans[(int64_t)b * a.groups + h * a.head_tiles + in / kHeadTile];
+        first = (int64_t)2 * span.x * kHeadTile + in % kHeadTile;
+        count = span.y;
+    }
+    __device__ __forceinline__ int64_t row(int i) const { return first + (i ? 2 * i : 1) * kHeadTile; }
+};
 
 // The largest reference and the sum over a query head's parts, by one wave.
-__device__ __forceinline__ float2 total_of(const float2* sums, int parts, int lane) {
+__device__ __forceinline__ float2 total_of(const float2* sums, const Parts& parts, int lane) {
     float m = -__builtin_inff(), l = 0.f;
-    for (int i = lane; i < parts; i += 64) m = fmaxf(m, sums[i].x);
-    for (int x = 32; x; x /= 2) m = fmaxf(m, __shfl_xor(m, x));
-    for (int i = lane; i < parts; i += 64) l += sums[i].y * exp2_of(sums[i].x - or_zero(m));
+    for (int i = lane; i < parts.count; i += 64) {
+        const float2 x = sums[parts.row(i)];
+        const float top = fmaxf(m, x.x);
+        l = l * exp2_of(m - or_zero(top)) + x.y * exp2_of(x.x - or_zero(top));
+        m = top;
+    }
+    float top = m;
+#pragma unroll
+    for (int x = 32; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+    l *= exp2_of(m - or_zero(top));
+#pragma unroll
     for (int x = 32; x; x /= 2) l += __shfl_xor(l, x);
-    return make_float2(or_zero(m), l);
+    return make_float2(or_zero(top), l);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins) {
-    __shared__ float4 sum[kThreads];
-    __shared__ float2 total[kHeadTile * 16];
-    const int lane = threadIdx.x & 63, dim = a.c.head_dim;
-    if ((int)blockIdx.x < joins) {
-        const int64_t q_row = blockIdx.x;
-        const int n = length_of(a, (int)(q_row / a.q_heads));
-        if (n <= a.chunk) return;
-        const int parts = (n + a.chunk - 1) / a.chunk;
-        const float2* sums = a.sums + q_row * a.splits;
-        const float2 all = total_of(sums, parts, lane);
-        const int wide = dim / 4, rows = kThreads / wide;  // four columns a thread
-        const int r = threadIdx.x / wide, c = threadIdx.x % wide;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < rows)
-            for (int i = r; i < parts; i += rows) {
-                const float w = exp2_of(sums[i].x - all.x);
-                const float4 y = *reinterpret_cast<const float4*>(a.parts + (q_row * a.splits + i) * dim + 4 * c);
-                x.x += w * y.x, x.y += w * y.y, x.z += w * y.z, x.w += w * y.w;
-            }
-        sum[threadIdx.x] = x;
-        __syncthreads();
-        if (r == 0) {
-            for (int i = 1; i < rows; i++) {
-                const float4 y = sum[i * wide + c];
-                x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-            }
-            const float f = all.y == 0.f ? 0.f : 1.f / all.y;
-            T* to = static_cast<T*>(a.out) + q_row * dim + 4 * c;
-            const float o[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ void join(const Attend& a, int block) {
+    __shared__ float sum[kWaves][kJoinColumns];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, dim = a.c.head_dim;
+    const int q_row = block / (dim / kJoinColumns), first = block % (dim / kJoinColumns) * kJoinColumns;
+    const Parts parts(a, q_row / a.q_heads, q_row % a.q_heads);
+    if (parts.count <= 1) return;
+    const float* in = a.parts + first + threadIdx.x % kJoinLanes * 4;
+    // eight lanes take a part's columns, 32 parts at a time, four of them under way
+    vec<float, 4> x = {};
+    const float2 all = total_of(a.part_sums, parts, lane);
+    for (int i = threadIdx.x / kJoinLanes; i < parts.count; i += 4 * kJoinParts) {
+        vec<float, 4> y[4];
+        float w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) to[i] = (T)(all.y == 0.f ? 0.f : o[i] * f);
+        for (int u = 0; u < 4; u++) {
+            const int64_t row = parts.row(min(i + u * kJoinParts, parts.count - 1));
+            y[u] = *reinterpret_cast<const vec<float, 4>*>(in + row * dim);
+            w[u] = a.part_sums[row].x;
         }
-        return;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (i + u * kJoinParts < parts.count) x += exp2_of(w[u] - all.x) * y[u];
     }
+#pragma unroll
+    for (int d = kJoinLanes; d < 64; d *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], d);
+    if (lane < kJoinLanes)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[wave][lane * 4 + e] = x[e];
+    __syncthreads();
+    if (threadIdx.x < kJoinColumns) {
+        float o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) o += sum[w][threadIdx.x];
+        static_cast<T*>(a.out)[(int64_t)q_row * dim + first + threadIdx.x] = (T)(all.y == 0.f ? 0.f : o / all.y);
+    }
+}
+
+__device__ __forceinline__ void add_mass(const Attend& a, int block) {
+    __shared__ float2 total[kMassHeads];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int tiles = (a.bound + kMassKeys - 1) / kMassKeys;
-    const int tile = (blockIdx.x - joins) % tiles, bh = (blockIdx.x - joins) / tiles;
-    const int b = bh / a.c.kv_heads, h = bh % a.c.kv_heads;
+    const int tile = block % tiles, b = block / tiles / a.c.kv_heads, h = block / tiles % a.c.kv_heads;
     const int n = length_of(a, b);
     if (tile * kMassKeys >= n) return;
-    const int parts = (n + a.chunk - 1) / a.chunk;
     const int64_t first = (int64_t)b * a.q_heads + h * a.group;
-    const int key = tile * kMassKeys + 4 * threadIdx.x;
+    const int key = tile * kMassKeys + 4 * threadIdx.x, at = min(key, a.bound - 4);
+    const int page = a.table[b * a.table_row + (at >> a.page_shift)];
     vec<float, 4> w = {};
-    for (int base = 0; base < a.group; base += kHeadTile * 16) {
-        const int heads = min(a.group - base, kHeadTile * 16);
-        __syncthreads();
-        for (int i = threadIdx.x / 64; i < heads; i += kWaves) {
-            const float2 t = total_of(a.sums + (first + base + i) * a.splits, parts, lane);
+    for (int base = 0; base < a.group; base += kMassHeads) {
+        const int heads = min(a.group - base, kMassHeads);
+        vec<float, 4> s[kMassHeads];
+#pragma unroll
+        for (int i = 0; i < kMassHeads; i++)
+            if (i < heads) s[i] = *reinterpret_cast<const vec<float, 4>*>(a.scores + (first + base + i) * a.bound + at);
+        if (base) __syncthreads();
+        for (int i = wave; i < heads; i += kWaves) {
+            const Parts parts(a, b, h * a.group + base + i);
+            float2 t;
+            if (parts.count > 1) {
+                t = total_of(a.part_sums, parts, lane);
+            } else {
+                t = a.sums[first + base + i];
+                t.x = or_zero(t.x);
+            }
             if (lane == 0) total[i] = make_float2(t.x, t.y == 0.f ? 0.f : 1.f / t.y);
         }
         __syncthreads();
-        if (key < n)
-            for (int i = 0; i < heads; i++) {
-                const auto s = *reinterpret_cast<const vec<float, 4>*>(a.scores + (first + base + i) * a.bound + key);
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (total[i].y != 0.f) w[e] += exp2_of(s[e] - total[i].x) * total[i].y;
-            }
+        for (int i = 0; i < kMassHeads; i++)
+            if (i < heads && total[i].y != 0.f)
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] += exp2_of(s[i][e] - total[i].x) * total[i].y;
     }
-    if (key >= n) return;
-    const int page = a.table[b * a.table_row + (key >> a.page_shift)];
-    if (page < 0 || page >= a.c.pages) return;
-    float* mass = a.c.mass + ((int64_t)page * a.c.kv_heads + h) * a.c.page_size + (key & (a.c.page_size - 1));
+    if (key >= n || page < 0 || page >= a.c.pages) return;
+    float* mass = a.c.mass + (((int64_t)page * a.c.kv_heads + h) << a.page_shift) + (key & (a.c.page_size - 1));
     for (int e = 0; e < 4; e++)
         if (key + e < n) unsafeAtomicAdd(mass + e, w[e]);
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins) {
+    if ((int)blockIdx.x < joins) join<T>(a, blockIdx.x);
+    else add_mass(a, blockIdx.x - joins);
+}
+
 template <typename T, bool MX, int D>
-int launch(const Attend& a, hipStream_t stream) {
-    const int64_t groups = (int64_t)a.batch * a.c.kv_heads * a.head_tiles;
-    hipLaunchKernelGGL((attend_kernel<T, MX, D>), dim3((unsigned)(groups * a.splits)), dim3(kThreads),
-                       0, stream, a);
+int launch(const Attend& a, int workers, hipStream_t stream) {
+    hipLaunchKernelGGL((attend_kernel<T, MX, D>), dim3((unsigned)workers), dim3(kThreads), 0, stream, a);
     if (const int rc = (int)hipGetLastError()) return rc;
-    const int joins = a.splits > 1 ? a.batch * a.q_heads : 0;
+    const int64_t joins = a.bound > kUnit * kMinUnits ? (int64_t)a.batch * a.q_heads * (D / kJoinColumns) : 0;
     const int64_t tiles = a.scores ? (int64_t)((a.bound + kMassKeys - 1) / kMassKeys) * a.batch * a.c.kv_heads : 0;
     if (joins + tiles == 0) return 0;
-    hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)(joins + tiles)), dim3(kThreads), 0, stream, a, joins);
+    hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)(joins + tiles)), dim3(kThreads), 0, stream, a,
+                       (int)joins);
     return (int)hipGetLastError();
 }
 
 template <typename T, bool MX>
-int attend(const Attend& a, hipStream_t stream) {
+int attend(const Attend& a, int workers, hipStream_t stream) {
     switch (a.c.head_dim) {
-        case 64: return launch<T, MX, 64>(a, stream);
-        case 96: return launch<T, MX, 96>(a, stream);
-        case 128: return launch<T, MX, 128>(a, stream);
-        case 192: return launch<T, MX, 192>(a, stream);
-        default: return launch<T, MX, 256>(a, stream);
+        case 64: return launch<T, MX, 64>(a, workers, stream);
+        case 96: return launch<T, MX, 96>(a, workers, stream);
+        case 128: return launch<T, MX, 128>(a, workers, stream);
+        case 192: return launch<T, MX, 192>(a, workers, stream);
+        default: return launch<T, MX, 256>(a, workers, stream);
     }
 }
 
-// How a call is split: enough parts to give every CU several workgroups, none
-// shorter than a step of every wave.
-constexpr int kWorkgroups = 256 * 8, kMinChunk = 128, kBestChunk = 1024;
+// What a call needs of memory besides its arguments, and its workgroups: as many
+// as 256 CUs hold, but not more than there can be units.
 struct Plan {
-    int head_tiles, chunk, splits;
+    int64_t groups, units;  // of a sequence; of all, at most
+    int workers;
+    int64_t parts, part_sums, spans, scores, sums;  // bytes
+    int64_t bytes() const { return parts + part_sums + spans + scores + sums; }
 };
-Plan plan(const vramc_kv_cache& c, int q_heads, int table_width, int batch) {
+Plan plan(const vramc_kv_cache& c, int q_heads, int table_width, int batch, bool track) {
     Plan p;
-    p.head_tiles = (q_heads / c.kv_heads + kHeadTile - 1) / kHeadTile;
-    const int64_t bound = (int64_t)table_width * c.page_size;
-    const int64_t groups = (int64_t)batch * c.kv_heads * p.head_tiles;
-    int64_t chunk = bound * groups / kWorkgroups;
-    chunk = (chunk + kMinChunk - 1) / kMinChunk * kMinChunk;
-    if (chunk < kMinChunk) chunk = kMinChunk;
-    if (chunk > kBestChunk) chunk = kBestChunk;
-    p.chunk = (int)chunk;
-    p.splits = (int)((bound + chunk - 1) / chunk);
-    if (p.splits < 1) p.splits = 1;
+    const int64_t bound = (int64_t)table_width * c.page_size, rows = (int64_t)batch * q_heads;
+    p.groups = (int64_t)c.kv_heads * ((q_heads / c.kv_heads + kHeadTile - 1) / kHeadTile);
+    p.units = (bound + kUnit - 1) / kUnit * p.groups * batch;
+    const int resident = 256 * (c.head_dim <= 128 ? 3 : c.head_dim <= 192 ? 2 : 1);
+    p.workers = (int)(p.units < resident ? (p.units ? p.units : 1) : resident);
+    p.parts = (int64_t)p.workers * 2 * kHeadTile * c.head_dim * 4;
+    p.part_sums = (int64_t)p.workers * 2 * kHeadTile * 8;
+    p.spans = (p.groups * batch * 8 + 15) / 16 * 16;
+    p.scores = track ? rows * bound * 4 : 0;
+    p.sums = track ? rows * 8 : 0;
     return p;
 }
 
@@ -603,13 +763,11 @@ extern "C" int64_t vramc_kv_attend_workspace(const vramc_kv_cache* c, int q_head
                                              int batch, int track) {
     if (const int rc = check_cache(c)) return rc;
     if (q_heads <= 0 || q_heads % c->kv_heads || table_width < 0 || batch < 0) return RANS_EARG;
-    const int64_t bound = (int64_t)table_width * c->page_size;
-    if (bound > kMaxTokens || (int64_t)batch * q_heads > INT32_MAX / 2) return RANS_EARG;
-    const Plan p = plan(*c, q_heads, table_width, batch);
-    const int64_t rows = (int64_t)batch * q_heads;
-    if (rows * p.splits > INT32_MAX / 2) return RANS_EARG;  // a grid's workgroups
-    const int64_t parts = p.splits > 1 ? rows * p.splits * c->head_dim * 4 : 0;
-    return parts + (track ? rows * bound * 4 : 0) + (track || parts ? rows * p.splits * 8 : 0);
+    if ((int64_t)table_width * c->page_size > kMaxTokens || (int64_t)batch * q_heads > INT32_MAX / 16)
+        return RANS_EARG;
+    const Plan p = plan(*c, q_heads, table_width, batch, track);
+    if (p.units > INT32_MAX / 16) return RANS_EARG;  // shares and grids are counted in 32 bits
+    return p.bytes();
 }
 
 extern "C" int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q_seq,
@@ -621,25 +779,29 @@ extern "C" int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q
     if (need < 0) return (int)need;
     if (batch == 0) return 0;
     if (!q || !out || !lengths || (table_width && !table) || (track && !c->mass)) return RANS_EARG;
-    if (need && (!workspace || workspace_bytes < need)) return RANS_EWORKSPACE;
+    if (!workspace || workspace_bytes < need) return RANS_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return RANS_EARG;
-    const Plan p = plan(*c, q_heads, table_width, batch);
-    const int64_t rows = (int64_t)batch * q_heads;
-    Attend a{*c, q, q_seq, q_head, q_heads, q_heads / c->kv_heads, table, table_row, table_width,
-             lengths, batch, scale, out, p.chunk, p.splits, p.head_tiles,
-             __builtin_ctz(c->page_size), table_width * c->page_size, nullptr, nullptr, nullptr};
-    auto* work = static_cast<float*>(workspace);
-    if (p.splits > 1) {
-        a.parts = work;
-        work += rows * p.splits * c->head_dim;
+    const Plan p = plan(*c, q_heads, table_width, batch, track);
+    auto* work = static_cast<uint8_t*>(workspace);
+    const auto take = [&](int64_t bytes) {
+        auto* at = work;
+        work += bytes;
+        return static_cast<void*>(at);
+    };
+    const int64_t size = c->dtype == RANS_X_F32 ? 4 : 2;
+    const bool wide = ((uintptr_t)q | (uintptr_t)(q_seq * size) | (uintptr_t)(q_head * size)) % 16 == 0;
+    Attend a{*c, q, q_seq, q_head, wide, q_heads, q_heads / c->kv_heads, table, table_row, table_width,
+             lengths, batch, scale, out, (int)(p.groups / c->kv_heads), (int)p.groups,
+             __builtin_ctz(c->page_size), table_width * c->page_size, nullptr, nullptr, nullptr, nullptr, nullptr};
+    a.parts = static_cast<float*>(take(p.parts));
+    a.part_sums = static_cast<float2*>(take(p.part_sums));
+    a.spans = static_cast<int2*>(take(p.spans));
+    if (p.scores) {
+        a.scores = static_cast<float*>(take(p.scores));
+        a.sums = static_cast<float2*>(take(p.sums));
     }
-    if (track && table_width) {
-        a.scores = work;
-        work += rows * a.bound;
-    }
-    a.sums = reinterpret_cast<float2*>(work);
-    if (c->dtype == RANS_X_F32) return attend<float, false>(a, stream);
+    if (c->dtype == RANS_X_F32) return attend<float, false>(a, p.workers, stream);
     if (c->dtype == RANS_X_BF16)
-        return c->mx ? attend<__bf16, true>(a, stream) : attend<__bf16, false>(a, stream);
-    return c->mx ? attend<_Float16, true>(a, stream) : attend<_Float16, false>(a, stream);
+        return c->mx ? attend<__bf16, true>(a, p.workers, stream) : attend<__bf16, false>(a, p.workers, stream);
+    return c->mx ? attend<_Float16, true>(a, p.workers, stream) : attend<_Float16, false>(a, p.workers, stream);
 }
