@@ -39,7 +39,7 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kHeadTile = 16;     // query heads of a workgroup
 constexpr int kUnit = 128;        // keys that work is dealt in: a step of every wave
-constexpr int kMinUnits = 1;      // of a workgroup's share
+constexpr int kCus = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The reference is set this far below the largest score so far, and again when
@@ -83,10 +83,13 @@ __device__ __forceinline__ int length_of(const Attend& a, int b) {
 __device__ __forceinline__ int units_of(int n) { return (n + kUnit - 1) / kUnit; }
 
 // How units are dealt to workgroups: `rest` of them get one more than the others.
+// Beyond one for each CU, workgroups get two units at least: half as many parts
+// to join are worth more than a second workgroup's share of the latency (one
+// sequence of 32768 tokens: 15 us against 19).
 struct Shares {
     uint32_t workers, each, rest;
     __device__ __forceinline__ Shares(uint32_t units, uint32_t most) {
-        workers = min(most, (units + kMinUnits - 1) / kMinUnits);
+        workers = min(most, units <= kCus ? units : max((uint32_t)kCus, (units + 1) / 2));
         each = workers ? units / workers : 0;
         rest = units - each * workers;
     }
@@ -278,14 +281,19 @@ struct Values {
     }
 };
 
-// Waves of a SIMD that the registers are to allow.  Two cap them at 256, which
-// also keeps the sums in ordinary registers instead of accumulation registers,
-// from where every rescaling would have to copy them.
-template <typename T, int D>
-constexpr int kWavesOfSimd = D <= (sizeof(T) == 4 ? 96 : 128) ? 3 : D <= (sizeof(T) == 4 ? 128 : 192) ? 2 : 1;
+// Waves of a SIMD, and so workgroups of a CU, that the registers are to allow and
+// that the work is shared among.  Two cap the registers at 256, which also keeps
+// the sums in ordinary ones instead of accumulation registers, from where every
+// rescaling would have to copy them; three of 128 columns would spill (16
+// sequences of up to 32768 tokens: 290 us against 276; in 4 bits 103 against 91).
+// Narrow rows of 4 bits need three to have enough bytes under way (16 sequences
+// of 16384: 33.5 us against 36.2), the widest rows fill one wave's registers.
+constexpr int waves_of_simd(int size, bool mx, int dim) {
+    return mx && dim == 64 ? 3 : dim <= (size == 4 ? 128 : 192) ? 2 : 1;
+}
 
 template <typename T, bool MX, int D>
-__global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(Attend a) {
+__global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) attend_kernel(Attend a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int TILES = F32 ? 1 : 2;       // of 16 keys in a step
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
@@ -299,21 +307,25 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
 
     // this workgroup's share: each thread counts some sequences' units
     const int each = (a.batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
-    int mine = 0;
-    for (int i = b0; i < min(b0 + each, a.batch); i++) mine += units_of(length_of(a, i));
-    int sum = mine;
+    int mine = 0, before = 0, total = 0;
+    if (a.batch == 1) {  // nothing to count
+        total = units_of(length_of(a, 0));
+    } else {
+        for (int i = b0; i < min(b0 + each, a.batch); i++) mine += units_of(length_of(a, i));
+        int sum = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int x = __shfl_up(sum, d);
-        sum += lane >= d ? x : 0;
-    }
-    if (lane == 63) wave_units[wave] = sum;
-    __syncthreads();
-    int before = sum - mine, total = 0;
+        for (int d = 1; d < 64; d *= 2) {
+            const int x = __shfl_up(sum, d);
+            sum += lane >= d ? x : 0;
+        }
+        if (lane == 63) wave_units[wave] = sum;
+        __syncthreads();
+        before = sum - mine;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-        before += w < wave ? wave_units[w] : 0;
-        total += wave_units[w];
+        for (int w = 0; w < kWaves; w++) {
+            before += w < wave ? wave_units[w] : 0;
+            total += wave_units[w];
+        }
     }
     const Shares shares(__builtin_amdgcn_readfirstlane(total) * (uint32_t)a.groups, gridDim.x);
     for (int i = blockIdx.x; i < a.batch; i += gridDim.x)  // nothing to attend to
@@ -325,15 +337,19 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
     if (blockIdx.x >= shares.workers) return;
     uint32_t unit = shares.start(blockIdx.x);
     const uint32_t stop = shares.start(blockIdx.x + 1);
-    if (unit >= (uint32_t)before * a.groups && unit < (uint32_t)(before + mine) * a.groups) {
-        uint32_t off = unit - (uint32_t)before * a.groups;
-        int i = b0;
-        for (uint32_t x; off >= (x = (uint32_t)units_of(length_of(a, i)) * a.groups); i++) off -= x;
-        place[0] = i;
-        place[1] = (int)off;
+    int b = 0, off = (int)unit;
+    if (a.batch > 1) {
+        if (unit >= (uint32_t)before * a.groups && unit < (uint32_t)(before + mine) * a.groups) {
+            uint32_t in = unit - (uint32_t)before * a.groups;
+            int i = b0;
+            for (uint32_t x; in >= (x = (uint32_t)units_of(length_of(a, i)) * a.groups); i++) in -= x;
+            place[0] = i;
+            place[1] = (int)in;
+        }
+        __syncthreads();
+        b = __builtin_amdgcn_readfirstlane(place[0]);
+        off = __builtin_amdgcn_readfirstlane(place[1]);
     }
-    __syncthreads();
-    int b = __builtin_amdgcn_readfirstlane(place[0]), off = __builtin_amdgcn_readfirstlane(place[1]);
     const float scale = a.scale * kLog2e;
 
     while (unit < stop) {
@@ -536,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
 
     // the waves' parts, joined in two rounds through LDS, register by register
 #pragma unroll
-    for (int half = kWaves / 2; half; half /= 2) {
+    for (int half = steps > 1 ? kWaves / 2 : 0; half; half /= 2) {
         if (wave >= half && wave < 2 * half) {
             float(&to)[NT * 4 + 2][64] = part[wave - half];
 #pragma unroll
@@ -585,11 +601,16 @@ __global__ void __launch_bounds__(kThreads, (kWavesOfSimd<T, D>)) attend_kernel(
     }
 }
 
-// What is left when all parts are there.  The first blocks join the parts of 32
-// columns of a query head each; the others add the weights of 1024 tokens of a
-// kv head to their mass, from the scores that the first launch left.
+// What is left when all parts are there.  The first blocks join the parts; the
+// others add the weights of 1024 tokens of a kv head to their mass, from the
+// scores that the first launch left.  Where the workgroups make some eight parts
+// of a group or fewer, a thread joins four columns of a query head; where more, a
+// block joins 32 columns, 32 parts at a time: with 256 parts (one sequence of
+// 32768 tokens) that takes 5 us in place of 12, but 3072 blocks for 3 parts of
+// each of 768 heads take 12 us in place of 5.
+constexpr int kFewParts = 8;
 constexpr int kJoinColumns = 32, kJoinLanes = kJoinColumns / 4, kJoinParts = kThreads / kJoinLanes;
-constexpr int kMassKeys = 4 * kThreads, kMassHeads = 8;
+constexpr int kMassKeys = 4 * kThreads, kMassHeads = kThreads / 16;
 
 // The rows of a query head's parts, in order: slot 2w + 1 of the workgroup that
 // opens it, then slots 2w.
@@ -605,10 +626,11 @@ struct Parts {
     __device__ __forceinline__ int64_t row(int i) const { return first + (i ? 2 * i : 1) * kHeadTile; }
 };
 
-// The largest reference and the sum over a query head's parts, by one wave.
+// The largest reference and the sum over a query head's parts, by LANES lanes.
+template <int LANES>
 __device__ __forceinline__ float2 total_of(const float2* sums, const Parts& parts, int lane) {
     float m = -__builtin_inff(), l = 0.f;
-    for (int i = lane; i < parts.count; i += 64) {
+    for (int i = lane; i < parts.count; i += LANES) {
         const float2 x = sums[parts.row(i)];
         const float top = fmaxf(m, x.x);
         l = l * exp2_of(m - or_zero(top)) + x.y * exp2_of(x.x - or_zero(top));
@@ -616,11 +638,45 @@ __device__ __forceinline__ float2 total_of(const float2* sums, const Parts& part
     }
     float top = m;
 #pragma unroll
-    for (int x = 32; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
+    for (int x = LANES / 2; x; x /= 2) top = fmaxf(top, __shfl_xor(top, x));
     l *= exp2_of(m - or_zero(top));
 #pragma unroll
-    for (int x = 32; x; x /= 2) l += __shfl_xor(l, x);
+    for (int x = LANES / 2; x; x /= 2) l += __shfl_xor(l, x);
     return make_float2(or_zero(top), l);
+}
+
+template <typename T>
+__device__ __forceinline__ void join_few(const Attend& a, int block) {
+    const int dim = a.c.head_dim;
+    const int64_t at = 4 * ((int64_t)block * kThreads + threadIdx.x), q_row = at / dim;
+    if (q_row >= (int64_t)a.batch * a.q_heads) return;
+    const Parts parts(a, (int)(q_row / a.q_heads), (int)(q_row % a.q_heads));
+    if (parts.count <= 1) return;
+    const float* in = a.parts + (at - q_row * dim);
+    vec<float, 4> x = {};
+    float m = -__builtin_inff(), l = 0.f;
+    for (int i = 0; i < parts.count; i += 4) {
+        vec<float, 4> y[4];
+        float2 ml[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int64_t row = parts.row(min(i + u, parts.count - 1));
+            y[u] = *reinterpret_cast<const vec<float, 4>*>(in + row * dim);
+            ml[u] = a.part_sums[row];
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (i + u < parts.count) {
+                const float top = fmaxf(m, ml[u].x);
+                const float keep = exp2_of(m - or_zero(top)), w = exp2_of(ml[u].x - or_zero(top));
+                x = x * keep + y[u] * w;
+                l = l * keep + ml[u].y * w;
+                m = top;
+            }
+    }
+    T* to = static_cast<T*>(a.out) + at;
+#pragma unroll
+    for (int e = 0; e < 4; e++) to[e] = (T)(l == 0.f ? 0.f : x[e] / l);
 }
 
 template <typename T>
@@ -633,7 +689,7 @@ __device__ __forceinline__ void join(const Attend& a, int block) {
     const float* in = a.parts + first + threadIdx.x % kJoinLanes * 4;
     // eight lanes take a part's columns, 32 parts at a time, four of them under way
     vec<float, 4> x = {};
-    const float2 all = total_of(a.part_sums, parts, lane);
+    const float2 all = total_of<64>(a.part_sums, parts, lane);
     for (int i = threadIdx.x / kJoinLanes; i < parts.count; i += 4 * kJoinParts) {
         vec<float, 4> y[4];
         float w[4];
@@ -665,7 +721,6 @@ __device__ __forceinline__ void join(const Attend& a, int block) {
 
 __device__ __forceinline__ void add_mass(const Attend& a, int block) {
     __shared__ float2 total[kMassHeads];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int tiles = (a.bound + kMassKeys - 1) / kMassKeys;
     const int tile = block % tiles, b = block / tiles / a.c.kv_heads, h = block / tiles % a.c.kv_heads;
     const int n = length_of(a, b);
@@ -681,16 +736,13 @@ __device__ __forceinline__ void add_mass(const Attend& a, int block) {
         for (int i = 0; i < kMassHeads; i++)
             if (i < heads) s[i] = *reinterpret_cast<const vec<float, 4>*>(a.scores + (first + base + i) * a.bound + at);
         if (base) __syncthreads();
-        for (int i = wave; i < heads; i += kWaves) {
+        // the totals of 16 heads at once, 16 lanes each
+        const int i = threadIdx.x / 16;
+        if (i < heads) {
             const Parts parts(a, b, h * a.group + base + i);
-            float2 t;
-            if (parts.count > 1) {
-                t = total_of(a.part_sums, parts, lane);
-            } else {
-                t = a.sums[first + base + i];
-                t.x = or_zero(t.x);
-            }
-            if (lane == 0) total[i] = make_float2(t.x, t.y == 0.f ? 0.f : 1.f / t.y);
+            const float2 t = parts.count > 1 ? total_of<16>(a.part_sums, parts, threadIdx.x % 16)
+                                             : a.sums[first + base + i];
+            if (threadIdx.x % 16 == 0) total[i] = make_float2(or_zero(t.x), t.y == 0.f ? 0.f : 1.f / t.y);
         }
         __syncthreads();
 #pragma unroll
@@ -706,20 +758,25 @@ __device__ __forceinline__ void add_mass(const Attend& a, int block) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins) {
-    if ((int)blockIdx.x < joins) join<T>(a, blockIdx.x);
-    else add_mass(a, blockIdx.x - joins);
+__global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins, bool few) {
+    if ((int)blockIdx.x >= joins) add_mass(a, blockIdx.x - joins);
+    else if (few) join_few<T>(a, blockIdx.x);
+    else join<T>(a, blockIdx.x);
 }
 
 template <typename T, bool MX, int D>
 int launch(const Attend& a, int workers, hipStream_t stream) {
     hipLaunchKernelGGL((attend_kernel<T, MX, D>), dim3((unsigned)workers), dim3(kThreads), 0, stream, a);
     if (const int rc = (int)hipGetLastError()) return rc;
-    const int64_t joins = a.bound > kUnit * kMinUnits ? (int64_t)a.batch * a.q_heads * (D / kJoinColumns) : 0;
+    const bool few = workers <= (int64_t)a.batch * a.groups * kFewParts;
+    const int64_t rows = (int64_t)a.batch * a.q_heads;
+    const int64_t joins = a.bound <= kUnit ? 0
+                          : few                        ? (rows * (D / 4) + kThreads - 1) / kThreads
+                                                       : rows * (D / kJoinColumns);
     const int64_t tiles = a.scores ? (int64_t)((a.bound + kMassKeys - 1) / kMassKeys) * a.batch * a.c.kv_heads : 0;
     if (joins + tiles == 0) return 0;
     hipLaunchKernelGGL((finish_kernel<T>), dim3((unsigned)(joins + tiles)), dim3(kThreads), 0, stream, a,
-                       (int)joins);
+                       (int)joins, few);
     return (int)hipGetLastError();
 }
 
@@ -735,7 +792,7 @@ int attend(const Attend& a, int workers, hipStream_t stream) {
 }
 
 // What a call needs of memory besides its arguments, and its workgroups: as many
-// as 256 CUs hold, but not more than there can be units.
+// as the CUs hold, but not more than there can be units.
 struct Plan {
     int64_t groups, units;  // of a sequence; of all, at most
     int workers;
@@ -747,7 +804,7 @@ Plan plan(const vramc_kv_cache& c, int q_heads, int table_width, int batch, bool
     const int64_t bound = (int64_t)table_width * c.page_size, rows = (int64_t)batch * q_heads;
     p.groups = (int64_t)c.kv_heads * ((q_heads / c.kv_heads + kHeadTile - 1) / kHeadTile);
     p.units = (bound + kUnit - 1) / kUnit * p.groups * batch;
-    const int resident = 256 * (c.head_dim <= 128 ? 3 : c.head_dim <= 192 ? 2 : 1);
+    const int resident = kCus * waves_of_simd(c.dtype == RANS_X_F32 ? 4 : 2, c.mx, c.head_dim);
     p.workers = (int)(p.units < resident ? (p.units ? p.units : 1) : resident);
     p.parts = (int64_t)p.workers * 2 * kHeadTile * c.head_dim * 4;
     p.part_sums = (int64_t)p.workers * 2 * kHeadTile * 8;

@@ -143,24 +143,31 @@ class PagedCache:
         return cls(k, v, dtype, *scales, *more, lib=lib)
 
     # ------------------------------------------------------------- arguments
+    # The checks run on every token step: messages are made only for a failure.
     def _stream(self):
-        _check(rans._device() == self._index,
-               f"the cache is on {self.device}, the current device is another")
+        if rans._device() != self._index:
+            raise ValueError(f"the cache is on {self.device}, the current device is another")
         return rans._stream()
 
-    def _ints(self, name, t, dtype, dim):
-        _check(t.dtype is dtype and t.dim() == dim and t.get_device() == self._index
-               and (t.shape[-1] <= 1 or t.stride(-1) == 1),
-               f"{name} must be {dtype}, {dim}-dimensional, on {self.device}, its last "
-               f"dimension dense; got {t.dtype} {tuple(t.shape)} on {t.device}")
+    def _ints(self, name, t, dtype, shape):
+        """Checks integers of a shape (None for any size) whose last dimension
+        is dense."""
+        got = t.shape
+        if (t.dtype is not dtype or t.get_device() != self._index or len(got) != len(shape)
+                or (got[0] != shape[0] and shape[0] is not None)
+                or (got[-1] > 1 and t.stride(-1) != 1)):
+            want = tuple("n" if n is None else n for n in shape)
+            raise ValueError(f"{name} must be {want} of {dtype} on {self.device}, its last dimension "
+                             f"dense; got {tuple(got)} of {t.dtype} on {t.device}, strides {t.stride()}")
 
     def _rows(self, name, t, heads):
         """Checks rows x heads x head_dim values; a last dimension that is not
         dense is copied."""
-        _check(t.dim() == 3 and t.shape[2] == self.head_dim and t.dtype is self.dtype
-               and t.get_device() == self._index and (heads is None or t.shape[1] == heads),
-               f"{name} must be (n, {heads or 'heads'}, {self.head_dim}) of {self.dtype} on "
-               f"{self.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+        got = t.shape
+        if (len(got) != 3 or got[2] != self.head_dim or t.dtype is not self.dtype
+                or t.get_device() != self._index or (heads is not None and got[1] != heads)):
+            raise ValueError(f"{name} must be (n, {heads or 'heads'}, {self.head_dim}) of {self.dtype} "
+                             f"on {self.device}, got {tuple(got)} of {t.dtype} on {t.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient; the cache has none: detach it or use "
                              "torch.no_grad()")
@@ -183,13 +190,14 @@ class PagedCache:
         cache, whose mass starts at 0."""
         k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
         n = k.shape[0]
-        self._ints("slots", slots, torch.int64, 1)
-        _check(v.shape[0] == n and slots.shape[0] == n, "k, v and slots must have as many tokens")
+        if v.shape[0] != n:
+            raise ValueError(f"{n} keys and {v.shape[0]} values")
+        self._ints("slots", slots, torch.int64, (n,))
         at = None
         if self.mass is not None:
-            _check(positions is not None, "a tracked cache needs the tokens' positions")
-            self._ints("positions", positions, torch.int32, 1)
-            _check(positions.shape[0] == n, "positions must have as many tokens as k")
+            if positions is None:
+                raise ValueError("a tracked cache needs the tokens' positions")
+            self._ints("positions", positions, torch.int32, (n,))
             at = positions.data_ptr()
         rc = self.lib.vramc_kv_append(self._ref, k.data_ptr(), k.stride(0), k.stride(1),
                                       v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), at,
@@ -199,11 +207,11 @@ class PagedCache:
     def read(self, slots):
         """The keys and values in slots (int64), (tokens, kv_heads, head_dim)
         of the cache's dtype; zeros for a slot outside the cache."""
-        self._ints("slots", slots, torch.int64, 1)
-        shape = (slots.shape[0], self.kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
-        rc = self.lib.vramc_kv_read(self._ref, slots.data_ptr(), slots.shape[0], k.data_ptr(),
-                                    v.data_ptr(), self._stream())
+        self._ints("slots", slots, torch.int64, (None,))
+        n, stream = slots.shape[0], self._stream()
+        k = torch.empty((n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        v = torch.empty_like(k)
+        rc = self.lib.vramc_kv_read(self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), stream)
         assert rc == 0, f"HIP error {rc}"
         return k, v
 
@@ -216,25 +224,26 @@ class PagedCache:
         summed over the query heads of its kv head, is added to mass; by default
         where the cache has it."""
         q = self._rows("q", q, None)
-        batch, heads = q.shape[:2]
-        _check(heads > 0 and heads % self.kv_heads == 0,
-               f"{heads} query heads are no multiple of {self.kv_heads} kv heads")
-        self._ints("table", table, torch.int32, 2)
-        self._ints("lengths", lengths, torch.int32, 1)
-        _check(table.shape[0] == batch and lengths.shape[0] == batch,
-               "q, table and lengths must have as many sequences")
-        track = self.mass is not None if track is None else bool(track)
-        _check(not track or self.mass is not None, "the cache was made without track")
+        batch, heads, _ = q.shape
+        if heads <= 0 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.kv_heads} kv heads")
+        self._ints("table", table, torch.int32, (batch, None))
+        self._ints("lengths", lengths, torch.int32, (batch,))
+        if track is None:
+            track = self.mass is not None
+        elif track and self.mass is None:
+            raise ValueError("the cache was made without track")
         stream, width = self._stream(), table.shape[1]
         out = torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
         need = self.lib.vramc_kv_attend_workspace(self._ref, heads, width, batch, track)
-        _check(need >= 0, f"{batch} sequences of {heads} heads over {width} pages: too many ({need})")
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        if need < 0:
+            raise ValueError(f"{batch} sequences of {heads} heads over {width} pages: too many ({need})")
+        work = torch.empty(need, dtype=torch.uint8, device=self.device)
         rc = self.lib.vramc_kv_attend(
             self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, table.data_ptr(),
             table.stride(0), width, lengths.data_ptr(), batch,
             self.head_dim ** -0.5 if scale is None else scale, track, out.data_ptr(),
-            None if work is None else work.data_ptr(), need, stream)
+            work.data_ptr(), need, stream)
         assert rc == 0, f"HIP error {rc}"
         return out
 
@@ -248,30 +257,31 @@ class PagedCache:
         one sequence alone; the pages beyond the new lengths are free.  into: a
         table of other pages, which all kept tokens are copied to in order,
         while the sequences' own pages stay as they are."""
-        _check(self.mass is not None, "the cache was made without track")
-        self._ints("table", table, torch.int32, 2)
-        self._ints("lengths", lengths, torch.int32, 1)
-        self._ints("seen", seen, torch.int32, 1)
+        if self.mass is None:
+            raise ValueError("the cache was made without track")
+        self._ints("table", table, torch.int32, (None, None))
         batch, width = table.shape
-        _check(lengths.shape[0] == batch and seen.shape[0] == batch,
-               "table, lengths and seen must have as many sequences")
-        budget, recent = int(budget), int(recent)
-        _check(0 < budget < 2 ** 31, f"budget {budget}: a positive number of tokens")
-        _check(0 <= recent <= budget, f"recent {recent}: 0 to the budget")
+        self._ints("lengths", lengths, torch.int32, (batch,))
+        self._ints("seen", seen, torch.int32, (batch,))
+        if not 0 < budget < 2 ** 31:
+            raise ValueError(f"budget {budget}: a positive number of tokens")
+        if not 0 <= recent <= budget:
+            raise ValueError(f"recent {recent}: 0 to the budget")
+        other, row, wide = None, 0, 0
         if into is not None:
-            self._ints("into", into, torch.int32, 2)
-            _check(into.shape[0] == batch, "into must have as many sequences as table")
-            _check(into.shape[1] * self.page_size >= min(budget, width * self.page_size),
-                   f"into has no room for {budget} tokens")
+            self._ints("into", into, torch.int32, (batch, None))
+            other, row, wide = into.data_ptr(), into.stride(0), into.shape[1]
+            if wide * self.page_size < min(budget, width * self.page_size):
+                raise ValueError(f"into has no room for {budget} tokens")
         stream = self._stream()
         need = self.lib.vramc_kv_evict_workspace(self._ref, width, batch, budget, into is not None)
-        _check(need >= 0, f"{batch} sequences over {width} pages: too many ({need})")
+        if need < 0:
+            raise ValueError(f"{batch} sequences over {width} pages: too many ({need})")
         work = torch.empty(need, dtype=torch.uint8, device=self.device)
         out = torch.empty(batch, dtype=torch.int32, device=self.device)
         rc = self.lib.vramc_kv_evict(
             self._ref, table.data_ptr(), table.stride(0), width, lengths.data_ptr(),
-            seen.data_ptr(), batch, budget, recent, None if into is None else into.data_ptr(),
-            0 if into is None else into.stride(0), 0 if into is None else into.shape[1],
-            out.data_ptr(), work.data_ptr(), need, stream)
+            seen.data_ptr(), batch, budget, recent, other, row, wide, out.data_ptr(),
+            work.data_ptr(), need, stream)
         assert rc == 0, f"HIP error {rc}"
         return out
