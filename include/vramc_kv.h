@@ -41,7 +41,7 @@ typedef struct vramc_kv_cache {
     uint8_t *k_scale, *v_scale; /* mx only */
     float* mass;          /* [pages][kv_heads][page_size] accumulated weight, or NULL */
     int32_t* position;    /* [pages][kv_heads][page_size] token positions, or NULL
-                             (present where mass is) */
+                             (present where mass is); both 16-byte aligned */
 } vramc_kv_cache;
 
 /* Writes `tokens` keys and values into their slots: k[t*k_token + h*k_head + d]

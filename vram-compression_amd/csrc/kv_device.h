@@ -54,7 +54,8 @@ inline int check_cache(const vramc_kv_cache* c) {
         return RANS_EUNSUPPORTED;
     if (c->mx && c->dtype == RANS_X_F32) return RANS_EUNSUPPORTED;
     if (c->mx && (!c->k_scale || !c->v_scale)) return RANS_EARG;
-    if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 || (!c->mass != !c->position)) return RANS_EARG;
+    if (((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)c->mass | (uintptr_t)c->position) % 16) return RANS_EARG;
+    if (!c->mass != !c->position) return RANS_EARG;
     return 0;
 }
 

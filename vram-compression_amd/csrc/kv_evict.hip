@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kSelect = 1024;          // threads that select
 constexpr int kWaves = kSelect / 64;
-constexpr int kBatch = 16;             // keys that a lane loads at once
 constexpr int kKeys = 32;              // keys of a lane
 constexpr int kPiece = kSelect * kKeys;
 constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
@@ -195,40 +194,40 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             first = piece * kPiece + wave * 64 * each;
             limit = min(n, first + 64 * each);
             // the wave's pages: at most 2048 tokens, 16 or more to a page
-            const int page0 = first >> e.page_shift, pages = (max(limit, 1) - 1) >> e.page_shift;
+            const int page0 = first >> e.page_shift, last = (max(limit, 1) - 1) >> e.page_shift;
             int page[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                page[u] = page0 + 64 * u + lane <= pages ? row[page0 + 64 * u + lane] : -1;
+                page[u] = page0 + 64 * u + lane <= last ? row[page0 + 64 * u + lane] : -1;
                 if ((uint32_t)page[u] >= (uint32_t)e.c.pages) page[u] = -1;
             }
-            for (int i = 0; i < each; i += kBatch) {
-                if (first + 64 * i >= limit) {  // nothing there
-                    for (int u = i; u < each; u++) keys[64 * u] = 0;
-                    break;
-                }
-                float m[kBatch];
-                int p[kBatch];
-                bool there[kBatch];
+            // four neighbouring tokens a lane, 256 a wave, all loads before the first use
+            vec<uint32_t, 4>* to = reinterpret_cast<vec<uint32_t, 4>*>(piece_keys + wave * 64 * each) + lane;
+            vec<float, 4> m[kKeys / 4];
+            vec<int, 4> p[kKeys / 4];
+            uint32_t there = 0;
 #pragma unroll
-                for (int u = 0; u < kBatch; u++) {
-                    const int j = min(first + 64 * (i + u) + lane, limit - 1);
+            for (int u = 0; u < kKeys / 4; u++)
+                if (4 * u < each && first + 256 * u < limit) {
+                    const int j = min(first + 256 * u + 4 * lane, limit - 1) & ~3;
                     const int k = (j >> e.page_shift) - page0;
                     const int x = __shfl(page[0], k & 63), y = __shfl(page[1], k & 63);
                     const int in = k < 64 ? x : y;
-                    there[u] = in >= 0;
+                    there |= (uint32_t)(in >= 0) << u;
                     const int64_t at = ((((int64_t)max(in, 0) * e.c.kv_heads + h) << e.page_shift) +
                                         (j & (e.c.page_size - 1)));
-                    m[u] = e.c.mass[at];
-                    p[u] = e.c.position[at];
+                    m[u] = *reinterpret_cast<const vec<float, 4>*>(e.c.mass + at);
+                    p[u] = *reinterpret_cast<const vec<int, 4>*>(e.c.position + at);
                 }
 #pragma unroll
-                for (int u = 0; u < kBatch; u++)
-                    if (i + u < each)
-                        keys[64 * (i + u)] = first + 64 * (i + u) + lane < limit
-                                                 ? rank_of(m[u], p[u], there[u], recent)
-                                                 : 0;
-            }
+            for (int u = 0; u < kKeys / 4; u++)
+                if (4 * u < each) {
+                    vec<uint32_t, 4> r = {};
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (first + 256 * u + 4 * lane + i < limit) r[i] = rank_of(m[u][i], p[u][i], there >> u & 1, recent);
+                    to[64 * u] = r;
+                }
         };
         const auto over_keys = [&](auto f) {  // f(i, key): the wave's tokens 64 * i..
             for (int i = 0; i < each; i += 4) {
@@ -303,12 +302,15 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                         if (room <= ones) above |= 1u << bit;
                         else room -= ones;
                     }
-                    if (lane == 0) found[0] = (int)above, found[1] = room;
+                    int ties = 0;
+#pragma unroll
+                    for (int u = 0; u < kFew / 64; u++) ties += __popcll(__ballot(left[u] == above));
+                    if (lane == 0) found[0] = (int)above, found[1] = room, found[2] = ties;
                 }
                 __syncthreads();
                 above = (uint32_t)found[0];
                 room = found[1];
-                in_bin = -1;  // equal keys, as many as there may be
+                in_bin = found[2];
                 break;
             }
             bits = shift == 21 ? 11 : 10;

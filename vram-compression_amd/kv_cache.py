@@ -108,7 +108,7 @@ class PagedCache:
                    and t.is_contiguous(),
                    f"{name} must be a contiguous {dt} tensor {shape} on {k.device}, got "
                    f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        _check(k.data_ptr() % 16 == 0 and v.data_ptr() % 16 == 0, "k and v must be 16-byte aligned")
+            _check(t.data_ptr() % 16 == 0 or name.endswith("scale"), f"{name} must be 16-byte aligned")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.mass, self.position, self.dtype, self.device = mass, position, dtype, k.device
         self._index = k.get_device()
