@@ -62,8 +62,8 @@ __device__ __forceinline__ uint32_t rank_of(float m, int position, bool there, i
 }
 
 // Copies the tokens of list entries first .. first + kRows - 1, below count, of
-// a kv head, by one wave: 16 bytes a lane, four loads of keys and four of
-// values before the first store.
+// a kv head, by one wave: 16 bytes a lane, two loads of keys and two of values
+// before the first store (59 us in place of 62 with four, 4096 of 32768 tokens).
 __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, int count, int64_t* from_at,
                           int64_t* to_at) {
     const int lane = threadIdx.x & 63, b = group / e.c.kv_heads, h = group % e.c.kv_heads;
@@ -90,7 +90,7 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
     const int wide = e.c.mx ? e.c.head_dim / 32 : e.c.head_dim * (e.c.dtype == RANS_X_F32 ? 4 : 2) / 16;
     auto* k = static_cast<vec<uint32_t, 4>*>(e.c.k);
     auto* v = static_cast<vec<uint32_t, 4>*>(e.c.v);
-    constexpr int U = 4;
+    constexpr int U = 2;
     for (int at = lane; at < n * wide; at += 64 * U) {
         vec<uint32_t, 4> x[U], y[U];
         int64_t to[U];

@@ -46,6 +46,8 @@ class KvCacheDesc(ctypes.Structure):
 def bind(lib):
     """Sets the argument types of the cache's entry points on a handle of
     librans_hip.so and returns it; raises AttributeError if one is missing."""
+    if getattr(lib, "_kv_bound", False):
+        return lib
     P, I32, I64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
     D = ctypes.POINTER(KvCacheDesc)
     sig = {
@@ -61,6 +63,7 @@ def bind(lib):
         f = getattr(lib, name)
         f.argtypes = args
         f.restype = res
+    lib._kv_bound = True
     return lib
 
 
@@ -104,15 +107,16 @@ class PagedCache:
         if mass is not None:
             want += [("mass", mass, torch.float32, lead), ("position", position, torch.int32, lead)]
         for name, t, dt, shape in want:
-            _check(t.is_cuda and t.device == k.device and t.dtype is dt and tuple(t.shape) == shape
-                   and t.is_contiguous(),
-                   f"{name} must be a contiguous {dt} tensor {shape} on {k.device}, got "
-                   f"{t.dtype} {tuple(t.shape)} on {t.device}")
-            _check(t.data_ptr() % 16 == 0 or name.endswith("scale"), f"{name} must be 16-byte aligned")
+            if not (t.is_cuda and t.device == k.device and t.dtype is dt and t.shape == shape
+                    and t.is_contiguous()):
+                raise ValueError(f"{name} must be a contiguous {dt} tensor {shape} on {k.device}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+            if t.data_ptr() % 16 and not name.endswith("scale"):
+                raise ValueError(f"{name} must be 16-byte aligned")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.mass, self.position, self.dtype, self.device = mass, position, dtype, k.device
         self._index = k.get_device()
-        self.lib = bind(lib or rans.build())
+        self.lib = bind(lib or rans._host_lib())
         ptr = {n: t.data_ptr() for n, t, _, _ in want}
         self._desc = KvCacheDesc(pages=self.pages, kv_heads=self.kv_heads,
                                  page_size=self.page_size, head_dim=self.head_dim,
