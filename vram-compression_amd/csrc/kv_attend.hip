@@ -284,12 +284,14 @@ struct Values {
 // Waves of a SIMD, and so workgroups of a CU, that the registers are to allow and
 // that the work is shared among.  Two cap the registers at 256, which also keeps
 // the sums in ordinary ones instead of accumulation registers, from where every
-// rescaling would have to copy them; three of 128 columns would spill (16
-// sequences of up to 32768 tokens: 290 us against 276; in 4 bits 103 against 91).
-// Narrow rows of 4 bits need three to have enough bytes under way (16 sequences
-// of 16384: 33.5 us against 36.2), the widest rows fill one wave's registers.
+// rescaling would have to copy them; with three, 128 columns spill (16 sequences
+// of up to 32768 tokens: 290 us against 276).  Rows of 4 bits are short and need
+// the third for the bytes under way (the same sequences: 90 us against 91; of
+// 16384 tokens and 64 columns 33 against 37); the widest rows fill one wave's
+// registers.
 constexpr int waves_of_simd(int size, bool mx, int dim) {
-    return mx && dim == 64 ? 3 : dim <= (size == 4 ? 128 : 192) ? 2 : 1;
+    if (mx) return dim <= 128 ? 3 : 2;
+    return dim <= (size == 4 ? 128 : 192) ? 2 : 1;
 }
 
 template <typename T, bool MX, int D>
@@ -298,7 +300,6 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
     constexpr int TILES = F32 ? 1 : 2;       // of 16 keys in a step
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
     constexpr int NT = D / 16;               // tiles of the output
-    constexpr int AHEAD = !MX ? 1 : 2;
     using C = Deal<D>;
     __shared__ int wave_units[kWaves], place[2];
     __shared__ float part[2][NT * 4 + 2][64];
@@ -405,14 +406,14 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
         return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
     };
     int window = 0, ids = page_ids(0), next_ids = page_ids(1);
-    // A step's keys and values as they arrive, AHEAD steps in flight.
-    struct Step {
-        Keys<T, MX, D> k[TILES];
-        Values<T, MX, D, KEYS> v;
-        int page[TILES];
-        int64_t row[TILES];
-    } step[AHEAD];
-    const auto find = [&](Step& x, int t) {  // page 0 stands in for a missing one
+    // The step at hand.  As soon as its keys are multiplied the next step's take
+    // their registers, and so with the values, so that some of both is always
+    // under way.
+    Keys<T, MX, D> k[TILES];
+    Values<T, MX, D, KEYS> v;
+    int page[TILES];
+    int64_t row[TILES];
+    const auto find = [&](int t) {  // page 0 stands in for a missing one
         const int tile = t / kWaves * TILES;
         if (tile / 64 != window) {
             ids = next_ids;
@@ -420,32 +421,30 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
         }
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            x.page[i] = __builtin_amdgcn_readlane(ids, tile % 64 + i);
-            x.row[i] = (((int64_t)max(x.page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
+            page[i] = __builtin_amdgcn_readlane(ids, tile % 64 + i);
+            row[i] = (((int64_t)max(page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
                        ((start + t * STEP + i * 16) & (a.c.page_size - 1));
         }
     };
-    const auto load_keys = [&](Step& x) {
+    const auto load_keys = [&] {
 #pragma unroll
-        for (int i = 0; i < TILES; i++) x.k[i].load(a.c, x.row[i], lane);
+        for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
     };
 
     vec<float, 4> o[NT] = {};
     float m = -__builtin_inff(), from = 0.f, l = 0.f;
-#pragma unroll
-    for (int u = 0; u < AHEAD; u++)
-        if (wave + u * kWaves < steps) {
-            find(step[u], wave + u * kWaves);
-            load_keys(step[u]);
-            step[u].v.load(a.c, step[u].row, lane);
-        }
-    const auto compute = [&](Step& x, int t) {
+    if (wave < steps) {
+        find(wave);
+        load_keys();
+        v.load(a.c, row, lane);
+    }
+    for (int t = wave; t < steps; t += kWaves) {
         const int key0 = start + t * STEP;
         bool whole = key0 + STEP <= end;
         bool there[TILES];
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
-            there[i] = x.page[i] >= 0;
+            there[i] = page[i] >= 0;
             whole &= there[i];
         }
         vec<float, 4> s[TILES] = {};
@@ -456,17 +455,17 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                 for (int c = 0; c < D / 16; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x.k[i].x[c].w[e]),
+                        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
                                                                     qf[c][e], s[i], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) s[i] = mma(x.k[i].operand(c, g), q[c], s[i]);
+                for (int c = 0; c < D / 32; c++) s[i] = mma(k[i].operand(c, g), q[c], s[i]);
             }
         }
-        const int next = t + AHEAD * kWaves;
-        if (next < steps) {
-            find(x, next);
-            load_keys(x);
+        const bool more = t + kWaves < steps;
+        if (more) {
+            find(t + kWaves);
+            load_keys();
         }
 #pragma unroll
         for (int i = 0; i < TILES; i++)
@@ -479,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                 for (int e = 0; e < 4; e++) {
                     const bool gone = !there[i] || key0 + 16 * i + 4 * g + e >= end;
                     if (gone) s[i][e] = -__builtin_inff();
-                    x.v.clear(4 * i + e, gone);
+                    v.clear(4 * i + e, gone);
                 }
         }
         if (a.scores && live) {
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
             for (int j = 0; j < KEYS; j++)
 #pragma unroll
                 for (int i = 0; i < NT; i++)
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v.value(i, j), p[j], o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[j], o[i], 0, 0, 0);
         } else {
             vec<T, 2> hi2[4], lo2[4];
 #pragma unroll
@@ -531,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                 vec<uint32_t, 4> even, odd;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t y = x.v.pair(i, 2 * j), z = x.v.pair(i, 2 * j + 1);
+                    const uint32_t y = v.pair(i, 2 * j), z = v.pair(i, 2 * j + 1);
                     even[j] = __builtin_amdgcn_perm(z, y, 0x05040100);
                     odd[j] = __builtin_amdgcn_perm(z, y, 0x07060302);
                 }
@@ -540,12 +539,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                 o[2 * i + 1] = mma(f, lo, mma(f, hi, o[2 * i + 1]));
             }
         }
-        if (next < steps) x.v.load(a.c, x.row, lane);
-    };
-    for (int t = wave; t < steps; t += AHEAD * kWaves) {
-#pragma unroll
-        for (int u = 0; u < AHEAD; u++)
-            if (t + u * kWaves < steps) compute(step[u], t + u * kWaves);
+        if (more) v.load(a.c, row, lane);
     }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
