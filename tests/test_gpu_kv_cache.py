@@ -259,7 +259,8 @@ STORES = [("bf16", False), ("f16", False), ("f32", False), ("bf16", True), ("f16
 @pytest.mark.parametrize("dtype,mx", STORES)
 @pytest.mark.parametrize("dim,page,heads,group", [(64, 16, 2, 7), (96, 32, 3, 1), (128, 64, 2, 6),
                                                   (192, 128, 1, 5), (256, 16, 1, 16),
-                                                  (128, 256, 1, 40), (64, 64, 5, 17)])
+                                                  (128, 256, 1, 40), (64, 64, 5, 17),
+                                                  (192, 32, 1, 24), (256, 16, 2, 20), (96, 128, 1, 33)])
 def test_attend(kv, dtype, mx, dim, page, heads, group):
     """Every storage, width and page size: lengths of none, one, just around
     tiles and pages, and some hundreds."""

@@ -5,7 +5,8 @@
 // and multiplies:
 //
 //  - The query heads of a kv head are the 16 columns of the matrix cores'
-//    tiles, so keys and values are read once for up to 16 of them.  Scores are
+//    tiles, so keys and values are read once for up to 16 of them (32 where two
+//    tiles fit the registers).  Scores are
 //    made transposed, S^T = K Q^T (16 keys x 16 heads): a lane then holds, for
 //    one head, the scores of keys 4g..4g+3 of each tile (g = lane / 16), and
 //    that is just how the second product O^T = V^T P^T wants its right operand
@@ -37,7 +38,6 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
-constexpr int kHeadTile = 16;     // query heads of a workgroup
 constexpr int kUnit = 128;        // keys that work is dealt in: a step of every wave
 constexpr int kCus = 256;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -64,13 +64,14 @@ struct Attend {
     int batch;
     float scale;
     void* out;
+    int tile;                // query heads that are taken at once, 16 or 32
     int head_tiles, groups;  // tiles of a kv head's queries; tiles of all kv heads
     int page_shift;
     int bound;               // tokens that a row of the table has room for
     // Workgroup w leaves the part that starts a group in slot 2w + 1 and one
     // that goes on from the workgroup before it in 2w.
-    float* parts;            // [slots][16][dim]
-    float2* part_sums;       // [slots][16]: reference (log2) and sum
+    float* parts;            // [slots][tile][dim]
+    float2* part_sums;       // [slots][tile]: reference (log2) and sum
     int2* spans;             // [batch][groups]: first workgroup of a group, number of parts
     float* scores;           // [batch * q_heads][bound], log2, where weights are tracked
     float2* sums;            // [batch * q_heads], of groups in one part, where they are
@@ -281,6 +282,16 @@ struct Values {
     }
 };
 
+// Tiles of query heads that a wave takes at once: two where a kv head has more
+// than 16 and the registers hold their queries and sums beside the keys, so that
+// up to 32 heads read the cache once (16 sequences of up to 16384 tokens, 32
+// heads of 128 columns: 37 us against 42; 24 of 64 in f32 54 against 72).  4-bit
+// pages are cheap to read and dear to convert with fewer waves at it: one tile
+// (24 heads of 128 columns 35 us against 41).
+constexpr int pair_of(int size, bool mx, int dim, int group) {
+    return group > 16 && !mx && size * dim <= (size == 4 ? 512 : 384) ? 2 : 1;
+}
+
 // Waves of a SIMD, and so workgroups of a CU, that the registers are to allow and
 // that the work is shared among.  Two cap the registers at 256, which also keeps
 // the sums in ordinary ones instead of accumulation registers, from where every
@@ -289,13 +300,14 @@ struct Values {
 // the third for the bytes under way (the same sequences: 90 us against 91; of
 // 16384 tokens and 64 columns 33 against 37); the widest rows fill one wave's
 // registers.
-constexpr int waves_of_simd(int size, bool mx, int dim) {
+constexpr int waves_of_simd(int size, bool mx, int dim, int pair) {
+    if (pair == 2) return size * dim <= 256 ? 2 : 1;
     if (mx) return dim <= 128 ? 3 : 2;
     return dim <= (size == 4 ? 128 : 192) ? 2 : 1;
 }
 
-template <typename T, bool MX, int D>
-__global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) attend_kernel(Attend a) {
+template <typename T, bool MX, int D, int PAIR>
+__global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR)) attend_kernel(Attend a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int TILES = F32 ? 1 : 2;       // of 16 keys in a step
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
@@ -357,22 +369,24 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
     const int n = __builtin_amdgcn_readfirstlane(length_of(a, b)), units = units_of(n);
     const int group = off / units, first_unit = off - group * units;
     const int here = min((uint32_t)(units - first_unit), stop - unit);
-    const int h = group / a.head_tiles, first_head = group % a.head_tiles * kHeadTile;
+    const int h = group / a.head_tiles, first_head = group % a.head_tiles * a.tile;
     const int start = first_unit * kUnit, end = min(n, (first_unit + here) * kUnit);
     const bool opens = first_unit == 0, alone = here == units;
     if (opens && threadIdx.x == 0)
         a.spans[(int64_t)b * a.groups + group] =
             make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + units - 1) - blockIdx.x + 1);
-    const int head = first_head + (lane & 15);
-    const bool live = head < a.group;
-    const int64_t q_row = (int64_t)b * a.q_heads + h * a.group + head;
+    const auto head_of = [&](int r) { return first_head + 16 * r + (lane & 15); };
+    const auto live = [&](int r) { return head_of(r) < a.group; };
+    const auto q_row = [&](int r) { return (int64_t)b * a.q_heads + h * a.group + head_of(r); };
 
     // the queries, in the keys' order of columns; heads beyond the group are zero
-    Half8<T> q[F32 ? 1 : D / 32];
-    vec<float, 4> qf[F32 ? D / 16 : 1];
-    {
+    Half8<T> q[PAIR][F32 ? 1 : D / 32];
+    vec<float, 4> qf[PAIR][F32 ? D / 16 : 1];
+#pragma unroll
+    for (int r = 0; r < PAIR; r++) {
         constexpr int N = F32 ? 4 : 8;
-        const T* p = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)(h * a.group + (live ? head : first_head)) * a.q_head;
+        const T* p = static_cast<const T*>(a.q) + b * a.q_seq +
+                     (int64_t)(h * a.group + (live(r) ? head_of(r) : first_head)) * a.q_head;
         const auto take = [&](int s, auto& x) {
             const T* from = p + Keys<T, MX, D>::column(s, g);
             if (a.q_wide) {
@@ -384,14 +398,14 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
         };
 #pragma unroll
         for (int s = 0; s < D / (F32 ? 16 : 32); s++) {
-            if constexpr (F32) take(s, qf[s]);
-            else take(s, q[s]);
+            if constexpr (F32) take(s, qf[r][s]);
+            else take(s, q[r][s]);
         }
-        if (!live) {
+        if (!live(r)) {
 #pragma unroll
-            for (auto& x : q) x = {};
+            for (auto& x : q[r]) x = {};
 #pragma unroll
-            for (auto& x : qf) x = {};
+            for (auto& x : qf[r]) x = {};
         }
     }
 
@@ -431,8 +445,10 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
         for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
     };
 
-    vec<float, 4> o[NT] = {};
-    float m = -__builtin_inff(), from = 0.f, l = 0.f;
+    vec<float, 4> o[PAIR][NT] = {};
+    float m[PAIR], from[PAIR] = {}, l[PAIR] = {};
+#pragma unroll
+    for (int r = 0; r < PAIR; r++) m[r] = -__builtin_inff();
     if (wave < steps) {
         find(wave);
         load_keys();
@@ -447,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
             there[i] = page[i] >= 0;
             whole &= there[i];
         }
-        vec<float, 4> s[TILES] = {};
+        vec<float, 4> s[PAIR][TILES] = {};
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
             if constexpr (F32) {
@@ -455,11 +471,17 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                 for (int c = 0; c < D / 16; c++)
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
-                                                                    qf[c][e], s[i], 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < PAIR; r++)
+                            s[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
+                                                                           qf[r][c][e], s[r][i], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 32; c++) s[i] = mma(k[i].operand(c, g), q[c], s[i]);
+                for (int c = 0; c < D / 32; c++) {
+                    const auto x = k[i].operand(c, g);
+#pragma unroll
+                    for (int r = 0; r < PAIR; r++) s[r][i] = mma(x, q[r][c], s[r][i]);
+                }
             }
         }
         const bool more = t + kWaves < steps;
@@ -467,64 +489,75 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
             find(t + kWaves);
             load_keys();
         }
-#pragma unroll
-        for (int i = 0; i < TILES; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[i][e] *= scale;
         if (!whole) {
 #pragma unroll
+            for (int j = 0; j < KEYS; j++) v.clear(j, !there[j >> 2] || key0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end);
+        }
+        float p[PAIR][KEYS];
+#pragma unroll
+        for (int r = 0; r < PAIR; r++) {
+#pragma unroll
             for (int i = 0; i < TILES; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool gone = !there[i] || key0 + 16 * i + 4 * g + e >= end;
-                    if (gone) s[i][e] = -__builtin_inff();
-                    v.clear(4 * i + e, gone);
-                }
-        }
-        if (a.scores && live) {
+                for (int e = 0; e < 4; e++) s[r][i][e] *= scale;
+            if (!whole) {
 #pragma unroll
-            for (int i = 0; i < TILES; i++)
-                if (key0 + 16 * i < a.bound)
-                    *reinterpret_cast<vec<float, 4>*>(a.scores + q_row * a.bound + key0 + 16 * i + 4 * g) = s[i];
-        }
-        float top = -__builtin_inff();
+                for (int i = 0; i < TILES; i++)
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) top = fmaxf(top, s[i][e]);
-        if (__builtin_expect(__any(top > m + kSlack<T>), 0)) {
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            if (top > m + kSlack<T>) {
-                from = or_zero(top - kBelow<T>);
-                const float keep = exp2_of(m - from);
-                l *= keep;
-#pragma unroll
-                for (int i = 0; i < NT; i++) o[i] *= keep;
-                m = top - kBelow<T>;
+                    for (int e = 0; e < 4; e++)
+                        if (!there[i] || key0 + 16 * i + 4 * g + e >= end) s[r][i][e] = -__builtin_inff();
             }
-        }
-        float p[KEYS];
+            if (a.scores && live(r)) {
 #pragma unroll
-        for (int j = 0; j < KEYS; j++) {
-            p[j] = exp2_of(s[j >> 2][j & 3] - from);
-            l += p[j];
+                for (int i = 0; i < TILES; i++)
+                    if (key0 + 16 * i < a.bound)
+                        *reinterpret_cast<vec<float, 4>*>(a.scores + q_row(r) * a.bound + key0 + 16 * i + 4 * g) = s[r][i];
+            }
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top = fmaxf(top, s[r][i][e]);
+            if (__builtin_expect(__any(top > m[r] + kSlack<T>), 0)) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (top > m[r] + kSlack<T>) {
+                    from[r] = or_zero(top - kBelow<T>);
+                    const float keep = exp2_of(m[r] - from[r]);
+                    l[r] *= keep;
+#pragma unroll
+                    for (int i = 0; i < NT; i++) o[r][i] *= keep;
+                    m[r] = top - kBelow<T>;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < KEYS; j++) {
+                p[r][j] = exp2_of(s[r][j >> 2][j & 3] - from[r]);
+                l[r] += p[r][j];
+            }
         }
         if constexpr (F32) {
 #pragma unroll
             for (int j = 0; j < KEYS; j++)
 #pragma unroll
                 for (int i = 0; i < NT; i++)
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[j], o[i], 0, 0, 0);
-        } else {
-            vec<T, 2> hi2[4], lo2[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const vec<float, 2> w = {p[2 * j], p[2 * j + 1]};
-                hi2[j] = __builtin_convertvector(w, vec<T, 2>);
-                lo2[j] = __builtin_convertvector(w - __builtin_convertvector(hi2[j], vec<float, 2>), vec<T, 2>);
+                    for (int r = 0; r < PAIR; r++)
+                        o[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[r][j], o[r][i], 0, 0, 0);
+        } else {
+            Half8<T> hi[PAIR], lo[PAIR];
+#pragma unroll
+            for (int r = 0; r < PAIR; r++) {
+                vec<T, 2> hi2[4], lo2[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const vec<float, 2> w = {p[r][2 * j], p[r][2 * j + 1]};
+                    hi2[j] = __builtin_convertvector(w, vec<T, 2>);
+                    lo2[j] = __builtin_convertvector(w - __builtin_convertvector(hi2[j], vec<float, 2>), vec<T, 2>);
+                }
+                hi[r] = __builtin_bit_cast(Half8<T>, hi2);
+                lo[r] = __builtin_bit_cast(Half8<T>, lo2);
             }
-            const auto hi = __builtin_bit_cast(Half8<T>, hi2), lo = __builtin_bit_cast(Half8<T>, lo2);
 #pragma unroll
             for (int i = 0; i < NT / 2; i++) {
                 vec<uint32_t, 4> even, odd;
@@ -535,54 +568,64 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D)) att
                     odd[j] = __builtin_amdgcn_perm(z, y, 0x07060302);
                 }
                 const auto e = __builtin_bit_cast(Half8<T>, even), f = __builtin_bit_cast(Half8<T>, odd);
-                o[2 * i] = mma(e, lo, mma(e, hi, o[2 * i]));
-                o[2 * i + 1] = mma(f, lo, mma(f, hi, o[2 * i + 1]));
+#pragma unroll
+                for (int r = 0; r < PAIR; r++) {
+                    o[r][2 * i] = mma(e, lo[r], mma(e, hi[r], o[r][2 * i]));
+                    o[r][2 * i + 1] = mma(f, lo[r], mma(f, hi[r], o[r][2 * i + 1]));
+                }
             }
         }
         if (more) v.load(a.c, row, lane);
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+#pragma unroll
+    for (int r = 0; r < PAIR; r++) {
+        l[r] += __shfl_xor(l[r], 16);
+        l[r] += __shfl_xor(l[r], 32);
+    }
 
     // the waves' parts, joined in two rounds through LDS, register by register
-#pragma unroll
     for (int half = steps > 1 ? kWaves / 2 : 0; half; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
-            float(&to)[NT * 4 + 2][64] = part[wave - half];
 #pragma unroll
-            for (int i = 0; i < NT * 4; i++) to[i][lane] = o[i / 4][i % 4];
-            to[NT * 4][lane] = m;
-            to[NT * 4 + 1][lane] = l;
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float(&in)[NT * 4 + 2][64] = part[wave];
-            const float other = in[NT * 4][lane], both = fmaxf(m, other);
-            const float x = exp2_of(m - or_zero(both)), y = exp2_of(other - or_zero(both));
-            l = l * x + in[NT * 4 + 1][lane] * y;
+        for (int r = 0; r < PAIR; r++) {
+            if (wave >= half && wave < 2 * half) {
+                float(&to)[NT * 4 + 2][64] = part[wave - half];
 #pragma unroll
-            for (int i = 0; i < NT * 4; i++) o[i / 4][i % 4] = o[i / 4][i % 4] * x + in[i][lane] * y;
-            m = both;
+                for (int i = 0; i < NT * 4; i++) to[i][lane] = o[r][i / 4][i % 4];
+                to[NT * 4][lane] = m[r];
+                to[NT * 4 + 1][lane] = l[r];
+            }
+            __syncthreads();
+            if (wave < half) {
+                const float(&in)[NT * 4 + 2][64] = part[wave];
+                const float other = in[NT * 4][lane], both = fmaxf(m[r], other);
+                const float x = exp2_of(m[r] - or_zero(both)), y = exp2_of(other - or_zero(both));
+                l[r] = l[r] * x + in[NT * 4 + 1][lane] * y;
+#pragma unroll
+                for (int i = 0; i < NT * 4; i++) o[r][i / 4][i % 4] = o[r][i / 4][i % 4] * x + in[i][lane] * y;
+                m[r] = both;
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
-    if (wave == 0 && live) {
+#pragma unroll
+    for (int r = 0; r < PAIR; r++) {
+        if (wave || !live(r)) continue;
         if (alone) {
-            if (a.scores && g == 0) a.sums[q_row] = make_float2(m, l);
-            const float x = l == 0.f ? 0.f : 1.f / l;
-            T* to = static_cast<T*>(a.out) + q_row * D;
+            if (a.scores && g == 0) a.sums[q_row(r)] = make_float2(m[r], l[r]);
+            const float x = l[r] == 0.f ? 0.f : 1.f / l[r];
+            T* to = static_cast<T*>(a.out) + q_row(r) * D;
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = (T)(l == 0.f ? 0.f : o[i][e] * x);
+                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = (T)(l[r] == 0.f ? 0.f : o[r][i][e] * x);
         } else {
-            const int64_t row = (int64_t)(2 * blockIdx.x + opens) * kHeadTile + (lane & 15);
-            if (g == 0) a.part_sums[row] = make_float2(m, l);
-            float* to = a.parts + row * D;
+            const int64_t at = (int64_t)(2 * blockIdx.x + opens) * a.tile + 16 * r + (lane & 15);
+            if (g == 0) a.part_sums[at] = make_float2(m[r], l[r]);
+            float* to = a.parts + at * D;
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = o[i][e];
+                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = o[r][i][e];
         }
     }
     unit += here;
@@ -610,14 +653,15 @@ constexpr int kMassKeys = 4 * kThreads, kMassHeads = kThreads / 16;
 // opens it, then slots 2w.
 struct Parts {
     int64_t first;
-    int count;
+    int count, tile;
     __device__ __forceinline__ Parts(const Attend& a, int b, int q_head) {
         const int h = q_head / a.group, in = q_head - h * a.group;
-        const int2 span = a.spans[(int64_t)b * a.groups + h * a.head_tiles + in / kHeadTile];
-        first = (int64_t)2 * span.x * kHeadTile + in % kHeadTile;
+        const int2 span = a.spans[(int64_t)b * a.groups + h * a.head_tiles + in / a.tile];
+        tile = a.tile;
+        first = (int64_t)2 * span.x * tile + in % tile;
         count = span.y;
     }
-    __device__ __forceinline__ int64_t row(int i) const { return first + (i ? 2 * i : 1) * kHeadTile; }
+    __device__ __forceinline__ int64_t row(int i) const { return first + (i ? 2 * i : 1) * tile; }
 };
 
 // The largest reference and the sum over a query head's parts, by LANES lanes.
@@ -760,7 +804,11 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(Attend a, int joins, b
 
 template <typename T, bool MX, int D>
 int launch(const Attend& a, int workers, hipStream_t stream) {
-    hipLaunchKernelGGL((attend_kernel<T, MX, D>), dim3((unsigned)workers), dim3(kThreads), 0, stream, a);
+    const dim3 grid((unsigned)workers), block(kThreads);
+    if constexpr (pair_of(sizeof(T), MX, D, 17) == 2) {
+        if (a.tile == 32) hipLaunchKernelGGL((attend_kernel<T, MX, D, 2>), grid, block, 0, stream, a);
+    }
+    if (a.tile == 16) hipLaunchKernelGGL((attend_kernel<T, MX, D, 1>), grid, block, 0, stream, a);
     if (const int rc = (int)hipGetLastError()) return rc;
     const bool few = workers <= (int64_t)a.batch * a.groups * kFewParts;
     const int64_t rows = (int64_t)a.batch * a.q_heads;
@@ -789,19 +837,22 @@ int attend(const Attend& a, int workers, hipStream_t stream) {
 // as the CUs hold, but not more than there can be units.
 struct Plan {
     int64_t groups, units;  // of a sequence; of all, at most
-    int workers;
+    int workers, tile;
     int64_t parts, part_sums, spans, scores, sums;  // bytes
     int64_t bytes() const { return parts + part_sums + spans + scores + sums; }
 };
 Plan plan(const vramc_kv_cache& c, int q_heads, int table_width, int batch, bool track) {
     Plan p;
     const int64_t bound = (int64_t)table_width * c.page_size, rows = (int64_t)batch * q_heads;
-    p.groups = (int64_t)c.kv_heads * ((q_heads / c.kv_heads + kHeadTile - 1) / kHeadTile);
+    const int size = c.dtype == RANS_X_F32 ? 4 : 2, group = q_heads / c.kv_heads;
+    const int pair = pair_of(size, c.mx, c.head_dim, group);
+    p.tile = 16 * pair;
+    p.groups = (int64_t)c.kv_heads * ((group + p.tile - 1) / p.tile);
     p.units = (bound + kUnit - 1) / kUnit * p.groups * batch;
-    const int resident = kCus * waves_of_simd(c.dtype == RANS_X_F32 ? 4 : 2, c.mx, c.head_dim);
+    const int resident = kCus * waves_of_simd(size, c.mx, c.head_dim, pair);
     p.workers = (int)(p.units < resident ? (p.units ? p.units : 1) : resident);
-    p.parts = (int64_t)p.workers * 2 * kHeadTile * c.head_dim * 4;
-    p.part_sums = (int64_t)p.workers * 2 * kHeadTile * 8;
+    p.parts = (int64_t)p.workers * 2 * p.tile * c.head_dim * 4;
+    p.part_sums = (int64_t)p.workers * 2 * p.tile * 8;
     p.spans = (p.groups * batch * 8 + 15) / 16 * 16;
     p.scores = track ? rows * bound * 4 : 0;
     p.sums = track ? rows * 8 : 0;
@@ -842,7 +893,7 @@ extern "C" int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q
     const int64_t size = c->dtype == RANS_X_F32 ? 4 : 2;
     const bool wide = ((uintptr_t)q | (uintptr_t)(q_seq * size) | (uintptr_t)(q_head * size)) % 16 == 0;
     Attend a{*c, q, q_seq, q_head, wide, q_heads, q_heads / c->kv_heads, table, table_row, table_width,
-             lengths, batch, scale, out, (int)(p.groups / c->kv_heads), (int)p.groups,
+             lengths, batch, scale, out, p.tile, (int)(p.groups / c->kv_heads), (int)p.groups,
              __builtin_ctz(c->page_size), table_width * c->page_size, nullptr, nullptr, nullptr, nullptr, nullptr};
     a.parts = static_cast<float*>(take(p.parts));
     a.part_sums = static_cast<float2*>(take(p.part_sums));
