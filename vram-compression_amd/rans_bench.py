@@ -3,6 +3,7 @@
   python vram-compression_amd/rans_bench.py bench   # timing sweep, JSON report
   python vram-compression_amd/rans_bench.py configs # the benchmark configurations
   python vram-compression_amd/rans_bench.py chain [grouped|separate|both] [LAYERS] [BATCH]
+  python vram-compression_amd/rans_bench.py tokens [LAYERS] [BATCH] [BUDGET] [STEPS]
   python vram-compression_amd/rans_bench.py profile [ROWS COLS BITS DIST ESC R C N FETCH]
 
 Mirror of kernel/bench.py of snuri00/vram-compression (same function names
@@ -716,6 +717,96 @@ def chain(bits=3.25, layers=28, seed=0, iters=3, grouped=False, batch=1):
                 effective_GBps=nweights * 2 / t_rans / 1e3, speedup_vs_bf16=t_bf16 / t_rans)
 
 
+class AttentionLayer(torch.nn.Module):
+    """A Qwen2.5-1.5B-shaped attention layer (random init, no rotary positions)
+    whose projections are rANS-coded and whose past is a PagedCache."""
+
+    def __init__(self, cache, hidden=1536, heads=12, bits=3.25):
+        super().__init__()
+        import rans_linear
+        wide = cache.kv_heads * cache.head_dim
+        shape = dict(q_proj=heads * cache.head_dim, k_proj=wide, v_proj=wide)
+        for name, rows in shape.items():
+            setattr(self, name, torch.nn.Linear(hidden, rows, bias=False))
+        self.o_proj = torch.nn.Linear(heads * cache.head_dim, hidden, bias=False)
+        rans_linear.replace_linears(self, bits, tune=False)
+        self.cache, self.heads = cache, heads
+
+    def forward(self, h, table, lengths, slots, positions):
+        """One new token of each sequence: h (sequences, hidden) in the cache's
+        dtype; lengths counts the new tokens, slots and positions are theirs."""
+        c, n = self.cache, h.shape[0]
+        x = torch.nn.functional.rms_norm(h, h.shape[-1:])
+        q, k, v = (p(x).view(n, -1, c.head_dim) for p in (self.q_proj, self.k_proj, self.v_proj))
+        c.append(k, v, slots, positions)
+        return h + self.o_proj(c.attend(q, table, lengths).view(n, -1))
+
+
+class AttentionStack:
+    """Layers whose caches hold the same sequences, each in pages of its own
+    table row, and what a serving loop keeps of them: step() takes one token of
+    every sequence through all layers and, where `slack` tokens have gathered
+    beyond the budget, drops as many from every layer by their weight."""
+
+    def __init__(self, layers=2, batch=4, budget=2048, slack=64, recent=256, page=64,
+                 dtype=torch.bfloat16, mx=True, track=True, bits=3.25, seed=0):
+        import kv_cache
+        torch.manual_seed(seed)
+        width = -(-(budget + slack) // page)
+        self.budget, self.slack, self.recent, self.batch = budget, slack, recent, batch
+        self.table = torch.arange(batch * width, dtype=torch.int32, device="cuda").view(batch, width)
+        self.rows = torch.arange(batch, device="cuda")
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
+        self.seen = torch.zeros(batch, dtype=torch.int32, device="cuda")
+        self.held = 0  # tokens of every sequence, as the host knows them
+        self.layers = [AttentionLayer(kv_cache.PagedCache.allocate(batch * width, 2, 128, page, dtype, mx, track),
+                                      bits=bits) for _ in range(layers)]
+
+    @torch.no_grad()
+    def step(self, h):
+        slots = self.layers[0].cache.slots(self.table, self.rows, self.lengths)
+        positions = self.seen.clone()
+        self.lengths += 1
+        self.seen += 1
+        self.held += 1
+        for layer in self.layers:
+            h = layer(h, self.table, self.lengths, slots, positions)
+        if self.held == self.budget + self.slack:
+            for layer in self.layers:
+                left = layer.cache.evict(self.table, self.lengths, self.seen, self.budget, self.recent)
+            self.lengths, self.held = left, self.budget
+        return h
+
+
+def tokens(layers=2, batch=4, budget=2048, steps=256):
+    """Tokens through Qwen2.5-1.5B-shaped attention layers whose weights are
+    rANS-coded and whose caches are 4-bit pages held at a budget: the caches are
+    filled to the budget, then `steps` tokens of `batch` sequences are timed.
+    Prints one JSON line."""
+    stack = AttentionStack(layers, batch, budget, recent=min(256, budget // 2))
+    h = torch.randn(batch, 1536, device="cuda").bfloat16()
+    for _ in range(budget + stack.slack):
+        stack.step(h)
+    torch.cuda.synchronize()
+    t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    t0.record()
+    for _ in range(steps):
+        out = stack.step(h)
+    t1.record()
+    t1.synchronize()
+    cache = stack.layers[0].cache
+    r = dict(config="Qwen2.5-1.5B-shaped attention layers, rANS weights, 4-bit cache at a budget",
+             layers=layers, batch=batch, budget=budget, steps=steps,
+             us_per_step_and_layer=t0.elapsed_time(t1) / steps / layers * 1e3,
+             cache_bits_per_value=8 * (cache.k.numel() + cache.k_scale.numel()) / (2 * cache.k.numel()),
+             cache_MB_per_layer=cache.nbytes / 1e6,
+             bf16_MB_per_layer_of_all_tokens=batch * 2 * 2 * 128 * 2 * int(stack.seen[0]) / 1e6,
+             finite=bool(torch.isfinite(out).all()))
+    print(json.dumps({k: (round(v, 4) if isinstance(v, float) else v) for k, v in r.items()}),
+          flush=True)
+    return r
+
+
 def configs():
     """The benchmark configurations beyond the headline shape: MLP shapes at
     2.25 bits with 0.1% escapes, q_proj at 4.25 bits, the headline shape at
@@ -814,6 +905,8 @@ if __name__ == "__main__":
     elif sys.argv[1] == "profile":
         types = (int, int, float, str, float, int, int, int, str)
         profile(*(t(v) for t, v in zip(types, sys.argv[2:])))
+    elif sys.argv[1] == "tokens":
+        tokens(*(int(v) for v in sys.argv[2:6]))
     elif sys.argv[1] == "chain":  # chain [grouped|separate|both] [layers] [batch]
         mode = sys.argv[2] if len(sys.argv) > 2 else "both"
         layers = int(sys.argv[3]) if len(sys.argv) > 3 else 28
