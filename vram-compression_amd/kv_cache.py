@@ -226,7 +226,8 @@ class PagedCache:
         q_heads, head_dim); a sequence without tokens gets zeros.  scale:
         head_dim**-0.5 unless given.  track: whether every token's weight,
         summed over the query heads of its kv head, is added to mass; by default
-        where the cache has it."""
+        where the cache has it.  The table's width bounds the lengths: one cut
+        to the pages in use (table[:, :n]) spares what longer ones would need."""
         q = self._rows("q", q, None)
         batch, heads, _ = q.shape
         if heads <= 0 or heads % self.kv_heads:
@@ -238,7 +239,8 @@ class PagedCache:
         elif track and self.mass is None:
             raise ValueError("the cache was made without track")
         stream, width = self._stream(), table.shape[1]
-        out = torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        out = torch.empty_like(q) if q.is_contiguous() else \
+            torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
         need = self.lib.vramc_kv_attend_workspace(self._ref, heads, width, batch, track)
         if need < 0:
             raise ValueError(f"{batch} sequences of {heads} heads over {width} pages: too many ({need})")
