@@ -325,12 +325,7 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
         total = units_of(length_of(a, 0));
     } else {
         for (int i = b0; i < min(b0 + each, a.batch); i++) mine += units_of(length_of(a, i));
-        int sum = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int x = __shfl_up(sum, d);
-            sum += lane >= d ? x : 0;
-        }
+        const int sum = wave_scan(mine);
         if (lane == 63) wave_units[wave] = sum;
         __syncthreads();
         before = sum - mine;

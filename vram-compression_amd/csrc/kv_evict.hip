@@ -21,7 +21,7 @@ constexpr int kWaves = kSelect / 64;
 constexpr int kKeys = 32;              // keys of a lane
 constexpr int kPiece = kSelect * kKeys;
 constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
-constexpr int kFew = 256;              // keys that a search by bits takes over
+constexpr int kFew = 128;              // keys that are compared with each other
 constexpr int kMove = 256;             // threads that move
 constexpr int kRows = 16;              // tokens that a wave moves at once
 // With at most this many moves a kv head (known from the table's width and the
@@ -130,12 +130,7 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
 // below this one; the workgroup's whole sum in *all.
 __device__ __forceinline__ uint32_t before_of(uint32_t x, uint32_t* waves, uint32_t* all) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    uint32_t sum = x;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t y = __shfl_up(sum, d);
-        sum += lane >= d ? y : 0;
-    }
+    const uint32_t sum = wave_scan((int)x);
     __syncthreads();
     if (lane == 63) waves[wave] = sum;
     __syncthreads();
@@ -168,7 +163,8 @@ __device__ __forceinline__ uint64_t lowest_set(uint64_t x, int n) {
 __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
     extern __shared__ uint32_t piece_keys[];
     __shared__ int hist[kBins], found[4];
-    __shared__ uint32_t waves[kWaves], few[kFew];
+    __shared__ uint32_t waves[kWaves];
+    __shared__ __attribute__((aligned(16))) uint32_t few[kFew];
     __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -244,6 +240,7 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
         __syncthreads();
         if (pieces == 1) load(0);
+        if (threadIdx.x < kFew) few[threadIdx.x] = 0;  // below every key
         if (threadIdx.x == 0) found[3] = 0;
         for (int shift = 21, bits = 11;; shift = shift == 21 ? 10 : 0) {
             for (int piece = 0; piece < pieces; piece++) {
@@ -262,16 +259,13 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             // the bin that holds the room-th largest: a sum from the top over
             // the threads, two bins each
             const int low = hist[2 * threadIdx.x], high = hist[2 * threadIdx.x + 1];
-            int sum = low + high;
-            for (int d = 1; d < 64; d *= 2) {
-                const int x = __shfl_down(sum, d);
-                sum += lane + d < 64 ? x : 0;
-            }
-            if (lane == 0) waves[wave] = sum;
+            const int sum = wave_scan(low + high);
+            if (lane == 63) waves[wave] = sum;
             __syncthreads();
             hist[2 * threadIdx.x] = hist[2 * threadIdx.x + 1] = 0;
-            int over = sum - low - high;  // in the bins above these two
-            for (int w = wave + 1; w < kWaves; w++) over += waves[w];
+            int over = -sum;  // in the bins above these two
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) over += w >= wave ? waves[w] : 0;
             if (over < room && room <= over + low + high) {
                 const bool upper = room <= over + high;
                 found[0] = 2 * threadIdx.x + upper;
@@ -284,28 +278,35 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             in_bin = found[2];
             if (room == in_bin || shift == 0) break;  // all that share these digits are kept
             if (in_bin <= kFew && pieces == 1) {
-                // few are left: one wave looks at all of them, bit by bit
+                // few are left: a thread each counts those above it
                 over_keys([&](int, uint32_t r) {
-                    if (r && (r ^ above) >> shift == 0) few[atomicAdd(&found[3], 1)] = r;
+                    const bool one = r && (r ^ above) >> shift == 0;
+                    const uint64_t ones = __ballot(one);
+                    if (!ones) return;
+                    int at = 0;
+                    if (lane == 0) at = atomicAdd(&found[3], (int)__popcll(ones));
+                    at = __builtin_amdgcn_readfirstlane(at);
+                    if (one) few[at + __popcll(ones & low_bits(lane))] = r;
                 });
                 __syncthreads();
-                if (wave == 0) {
-                    uint32_t left[kFew / 64];
+                if ((int)threadIdx.x < in_bin) {
+                    const uint32_t mine = few[threadIdx.x];
+                    int more = 0, as_much = 0;
+                    for (int i = 0; i < in_bin; i += 32) {
+                        vec<uint32_t, 4> r[8];
 #pragma unroll
-                    for (int u = 0; u < kFew / 64; u++) left[u] = 64 * u + lane < in_bin ? few[64 * u + lane] : 0;
-                    for (int bit = shift - 1; bit >= 0; bit--) {
-                        const uint32_t next = above >> bit | 1;
-                        int ones = 0;
+                        for (int u = 0; u < 8; u++) r[u] = *reinterpret_cast<const vec<uint32_t, 4>*>(few + i + 4 * u);
 #pragma unroll
-                        for (int u = 0; u < kFew / 64; u++)
-                            if (64 * u < in_bin) ones += __popcll(__ballot(left[u] >> bit == next));
-                        if (room <= ones) above |= 1u << bit;
-                        else room -= ones;
+                        for (int u = 0; u < 32; u++) {
+                            more += r[u / 4][u % 4] > mine;
+                            as_much += r[u / 4][u % 4] >= mine;
+                        }
                     }
-                    int ties = 0;
-#pragma unroll
-                    for (int u = 0; u < kFew / 64; u++) ties += __popcll(__ballot(left[u] == above));
-                    if (lane == 0) found[0] = (int)above, found[1] = room, found[2] = ties;
+                    if (more < room && room <= as_much) {  // the same values, if several
+                        found[0] = (int)mine;
+                        found[1] = room - more;
+                        found[2] = as_much - more;
+                    }
                 }
                 __syncthreads();
                 above = (uint32_t)found[0];
