@@ -66,7 +66,10 @@ int vramc_kv_read(const vramc_kv_cache* c, const int64_t* slots, int64_t tokens,
  *   out[b,h] = sum_j p_j v[j], p = softmax_j(scale * q[b,h] . k[j])
  * over tokens j < lengths[b], token j at place j % page_size of page
  * table[b*table_row + j/page_size], kv head h / (q_heads/kv_heads).  Sums and
- * softmax are in f32, out ([batch][q_heads][head_dim]) is rounded once.  Tokens
+ * softmax are in f32, out ([batch][q_heads][head_dim]) is rounded once.  A value
+ * that is not finite, or so large that 256 times its column's sum of magnitudes
+ * leaves f32, makes its column of its sequences' outputs NaN or infinite; a
+ * token of weight 0 counts there too.  Tokens
  * whose table entry is no page of the cache are left out; a sequence without
  * tokens gets zeros.  lengths beyond table_width * page_size are cut to it.
  * With track, mass[token] of each kv head increases by the sum of p over the

@@ -134,3 +134,32 @@ def test_fails_loudly_without_gpu(kv):
         kv.PagedCache.allocate(4, 2, 128)
     with pytest.raises(RuntimeError):
         kv.PagedCache(torch.zeros(4, 2, 64, 128), torch.zeros(4, 2, 64, 128), torch.float32)
+
+
+def test_refuses_what_no_grid_holds(kv, lib):
+    """A launch has fewer than 2^32 threads: what would need more is an argument
+    refused, not a failed launch."""
+    c = ctypes.byref(desc(kv))
+    assert lib.vramc_kv_append(c, P, 256, 128, P, 256, 128, P, P, 1 << 28, None) == EARG
+    assert lib.vramc_kv_read(c, P, 1 << 28, P, P, None) == EARG
+    for heads, width, batch in ((2, 1, (1 << 21) + 1), (4, 1 << 17, 1 << 13)):
+        assert lib.vramc_kv_attend_workspace(c, heads, width, batch, 1) == EARG
+    assert lib.vramc_kv_attend_workspace(c, 2, 1, 1 << 21, 0) > 0
+    assert lib.vramc_kv_evict_workspace(c, 1 << 24, 1, 1 << 30, 1) == EARG
+    assert lib.vramc_kv_evict_workspace(c, 1 << 23, 1, 1 << 29, 1) > 0
+
+
+def test_slots_of_padding(kv):
+    """Indexes without a page have no slot: negative ones, those beyond the
+    table, those of a table without pages."""
+    import types
+
+    import torch
+    cache = types.SimpleNamespace(page_size=16)
+    table = torch.tensor([[3, -1, 5], [0, 2, 7]], dtype=torch.int32)
+    sequence = torch.tensor([0, 0, 0, 0, 0, 1, 1, 1, 1], dtype=torch.int32)
+    index = torch.tensor([0, 15, 16, 47, 48, -1, -16, -17, 20], dtype=torch.int32)
+    got = kv.PagedCache.slots(cache, table, sequence, index)
+    assert got.dtype is torch.int64
+    assert got.tolist() == [48, 63, -1, 95, -1, -1, -1, -1, 36]
+    assert kv.PagedCache.slots(cache, table[:, :0], sequence, index).tolist() == [-1] * 9

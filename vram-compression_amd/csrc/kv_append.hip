@@ -171,7 +171,7 @@ struct Shape {
 Shape shape_of(const vramc_kv_cache& c, int64_t tokens) {
     const int per_row = c.head_dim / kPer, rows = kThreads / per_row;
     const int64_t n = (tokens + rows - 1) / rows * c.kv_heads;
-    return {dim3(n > INT32_MAX ? 0 : (unsigned)n), dim3((unsigned)per_row, (unsigned)rows)};
+    return {dim3(n > kMaxThreads / kThreads ? 0 : (unsigned)n), dim3((unsigned)per_row, (unsigned)rows)};
 }
 
 template <typename T, bool MX>

@@ -828,6 +828,10 @@ int attend(const Attend& a, int workers, hipStream_t stream) {
     }
 }
 
+// Query rows and units of a call: a grid of both launches' blocks for either
+// stays below 2^32 threads, and shares and row lengths are counted in 32 bits.
+constexpr int64_t kMaxRows = 1 << 22, kMaxUnits = 1 << 26;
+
 // What a call needs of memory besides its arguments, and its workgroups: as many
 // as the CUs hold, but not more than there can be units.
 struct Plan {
@@ -860,10 +864,10 @@ extern "C" int64_t vramc_kv_attend_workspace(const vramc_kv_cache* c, int q_head
                                              int batch, int track) {
     if (const int rc = check_cache(c)) return rc;
     if (q_heads <= 0 || q_heads % c->kv_heads || table_width < 0 || batch < 0) return RANS_EARG;
-    if ((int64_t)table_width * c->page_size > kMaxTokens || (int64_t)batch * q_heads > INT32_MAX / 16)
+    if ((int64_t)table_width * c->page_size > kMaxTokens || (int64_t)batch * q_heads > kMaxRows)
         return RANS_EARG;
     const Plan p = plan(*c, q_heads, table_width, batch, track);
-    if (p.units > INT32_MAX / 16) return RANS_EARG;  // shares and grids are counted in 32 bits
+    if (p.units > kMaxUnits) return RANS_EARG;
     return p.bytes();
 }
 

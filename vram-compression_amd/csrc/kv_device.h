@@ -15,7 +15,8 @@
 namespace {
 
 constexpr int kMxBlock = 32;  // values to a scale byte
-constexpr int64_t kMaxTokens = 1 << 30;  // that a row of the table has room for
+constexpr int64_t kMaxTokens = 1 << 29;  // that a row of the table has room for
+constexpr int64_t kMaxThreads = UINT32_MAX;  // of a launch
 
 template <typename T, int N>
 using vec = T __attribute__((ext_vector_type(N)));

@@ -86,7 +86,10 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
             e.c.position[to] = p;
         }
     }
+    // the wave's own writes to LDS before its reads of them by other lanes
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     const int wide = e.c.mx ? e.c.head_dim / 32 : e.c.head_dim * (e.c.dtype == RANS_X_F32 ? 4 : 2) / 16;
     auto* k = static_cast<vec<uint32_t, 4>*>(e.c.k);
     auto* v = static_cast<vec<uint32_t, 4>*>(e.c.v);
@@ -381,11 +384,10 @@ __global__ void __launch_bounds__(kMove) move_kernel(Evict e) {
     if (first < count) move_rows(e, group, first, count, rows[wave][0], rows[wave][1]);
 }
 
-// Lets the selecting workgroup have more LDS than 64 KB, once a process.
+// Lets the selecting workgroup have more LDS than 64 KB on the current device.
 int allow_lds() {
-    static const hipError_t rc = hipFuncSetAttribute(reinterpret_cast<const void*>(select_kernel),
-                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kPiece * 4);
-    return (int)rc;
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(select_kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, kPiece * 4);
 }
 
 // Tokens of a kv head that one call can move.
@@ -427,7 +429,8 @@ extern "C" int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int
     const bool here = most <= kMovesHere;
     const int64_t keys = e.bound < kPiece ? e.bound : kPiece;
     const size_t lds = (size_t)((keys + 4 * kSelect - 1) / (4 * kSelect) * (4 * kSelect) * 4);
-    if (const int rc = allow_lds()) return rc;
+    if (lds > 32768)  // with what the kernel has besides, up to 64 KB need no leave
+        if (const int rc = allow_lds()) return rc;
     hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), lds, stream, e, here);
     if (const int rc = (int)hipGetLastError()) return rc;
     if (here) return 0;

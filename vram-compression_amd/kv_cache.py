@@ -179,11 +179,15 @@ class PagedCache:
 
     def slots(self, table, sequence, index):
         """The slots (int64) of tokens `index` of sequences `sequence` (rows of
-        table), -1 where the table has no page for them."""
-        page = index.long() // self.page_size
-        known = page < table.shape[1]
-        page = table[sequence.long(), page.clamp(max=max(0, table.shape[1] - 1))].long()
-        slot = page * self.page_size + index.long() % self.page_size
+        table), -1 where the table has no page for them (a negative index, as of
+        padding, among them)."""
+        index, width = index.long(), table.shape[1]
+        if width == 0:
+            return torch.full_like(index, -1)
+        page = torch.div(index, self.page_size, rounding_mode="floor")
+        known = (page >= 0) & (page < width)
+        page = table[sequence.long(), page.clamp(0, width - 1)].long()
+        slot = page * self.page_size + index % self.page_size
         return torch.where(known & (page >= 0), slot, -1)
 
     # ------------------------------------------------------------ operations
