@@ -3,15 +3,22 @@
 // A kv head of a sequence ranks its tokens by a 32-bit key that sorts as the
 // order of eviction does.  One workgroup reads the keys of up to 32768 tokens
 // into LDS once, finds the budget-th largest by radix selection (11, 11 and 10
-// bits, histograms in LDS too), and keeps every token above it and of those
-// equal to it as many as there is room for, lowest index first.  A wave goes
-// over neighbouring tokens, so that ranks within it are counts of ballot bits,
-// and the order of indices costs one exchange between the waves.  Longer
-// sequences go through in pieces of 32768 tokens, read again for every step.
+// bits, histograms in LDS too; the first digit is counted while the keys come
+// in), and keeps every token above it and of those equal to it as many as there
+// is room for, lowest index first.  A wave goes over neighbouring tokens, so
+// that ranks within it are counts of ballot bits, and the order of indices
+// costs one exchange between the waves.  Longer sequences go through in pieces
+// of 32768 tokens, read again for every step.
 //
 // What moves is then two ordered lists of places, all different, and moving a
 // copy of rows.  In place a kept token moves only if it lies beyond the budget:
 // a decode step's eviction moves one token, not the cache.
+//
+// Selection is bound by the latency of its steps (reads, digits, lists) on one
+// workgroup a head, moving by HBM: 8 heads of 4 sequences of 32768 tokens cut to
+// 4096 take 22 us and then 134 MB, read and written, 30 us (4.4 TB/s); 2 heads of
+// 64 sequences of 2049 cut to 2048 8.9 us in one launch, where two take 12.1.  One
+// sequence of 131072 tokens, in pieces, takes 134 us in all.
 #include "kv_device.h"
 
 namespace {
@@ -21,7 +28,6 @@ constexpr int kWaves = kSelect / 64;
 constexpr int kKeys = 32;              // keys of a lane
 constexpr int kPiece = kSelect * kKeys;
 constexpr int kBins = 2 * kSelect;     // of a digit of 11 bits
-constexpr int kFew = 128;              // keys that are compared with each other
 constexpr int kMove = 256;             // threads that move
 constexpr int kRows = 16;              // tokens that a wave moves at once
 // With at most this many moves a kv head (known from the table's width and the
@@ -63,7 +69,9 @@ __device__ __forceinline__ uint32_t rank_of(float m, int position, bool there, i
 
 // Copies the tokens of list entries first .. first + kRows - 1, below count, of
 // a kv head, by one wave: 16 bytes a lane, two loads of keys and two of values
-// before the first store (59 us in place of 62 with four, 4096 of 32768 tokens).
+// before the first store (16 sequences of 16384 tokens in 4 bits cut to 2048: 37.4
+// us, with four 39.5), the stores past the caches (4 sequences of 32768 in bf16 cut
+// to 4096: 52.7 us against 57.1; the former 37.4 against 40.1).
 __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, int count, int64_t* from_at,
                           int64_t* to_at) {
     const int lane = threadIdx.x & 63, b = group / e.c.kv_heads, h = group % e.c.kv_heads;
@@ -111,8 +119,8 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (to[u] >= 0) {
-                k[to[u]] = x[u];
-                v[to[u]] = y[u];
+                __builtin_nontemporal_store(x[u], k + to[u]);
+                __builtin_nontemporal_store(y[u], v + to[u]);
             }
     }
     if (e.c.mx) {
@@ -165,9 +173,8 @@ __device__ __forceinline__ uint64_t lowest_set(uint64_t x, int n) {
 
 __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
     extern __shared__ uint32_t piece_keys[];
-    __shared__ int hist[kBins], found[4];
+    __shared__ int hist[kBins], found[3];
     __shared__ uint32_t waves[kWaves];
-    __shared__ __attribute__((aligned(16))) uint32_t few[kFew];
     __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -189,7 +196,7 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         const int each = pieces > 1 ? kKeys : (n + 4 * kSelect - 1) / (4 * kSelect) * 4;
         int first, limit;  // the wave's tokens in the piece at hand, and its keys
         uint32_t* keys = piece_keys + wave * 64 * each + lane;
-        const auto load = [&](int piece) {
+        const auto load = [&](int piece, bool count) {
             first = piece * kPiece + wave * 64 * each;
             limit = min(n, first + 64 * each);
             // the wave's pages: at most 2048 tokens, 16 or more to a page
@@ -224,7 +231,10 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                     vec<uint32_t, 4> r = {};
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (first + 256 * u + 4 * lane + i < limit) r[i] = rank_of(m[u][i], p[u][i], there >> u & 1, recent);
+                        if (first + 256 * u + 4 * lane + i < limit) {
+                            r[i] = rank_of(m[u][i], p[u][i], there >> u & 1, recent);
+                            if (count) atomicAdd(&hist[r[i] >> 21], 1);
+                        }
                     to[64 * u] = r;
                 }
         };
@@ -242,17 +252,11 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         int in_bin = 0;      // and how many do
         hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
         __syncthreads();
-        if (pieces == 1) load(0);
-        if (threadIdx.x < kFew) few[threadIdx.x] = 0;  // below every key
-        if (threadIdx.x == 0) found[3] = 0;
+        if (pieces == 1) load(0, true);  // the first digit is counted on the way
         for (int shift = 21, bits = 11;; shift = shift == 21 ? 10 : 0) {
             for (int piece = 0; piece < pieces; piece++) {
-                if (pieces > 1) load(piece);
-                if (shift == 21)
-                    over_keys([&](int, uint32_t r) {
-                        if (r) atomicAdd(&hist[r >> 21], 1);
-                    });
-                else
+                if (pieces > 1) load(piece, shift == 21);
+                if (shift < 21)
                     over_keys([&](int, uint32_t r) {
                         if (r && (r ^ above) >> (shift + bits) == 0)
                             atomicAdd(&hist[r >> shift & ((1 << bits) - 1)], 1);
@@ -280,43 +284,6 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             room = found[1];
             in_bin = found[2];
             if (room == in_bin || shift == 0) break;  // all that share these digits are kept
-            if (in_bin <= kFew && pieces == 1) {
-                // few are left: a thread each counts those above it
-                over_keys([&](int, uint32_t r) {
-                    const bool one = r && (r ^ above) >> shift == 0;
-                    const uint64_t ones = __ballot(one);
-                    if (!ones) return;
-                    int at = 0;
-                    if (lane == 0) at = atomicAdd(&found[3], (int)__popcll(ones));
-                    at = __builtin_amdgcn_readfirstlane(at);
-                    if (one) few[at + __popcll(ones & low_bits(lane))] = r;
-                });
-                __syncthreads();
-                if ((int)threadIdx.x < in_bin) {
-                    const uint32_t mine = few[threadIdx.x];
-                    int more = 0, as_much = 0;
-                    for (int i = 0; i < in_bin; i += 32) {
-                        vec<uint32_t, 4> r[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++) r[u] = *reinterpret_cast<const vec<uint32_t, 4>*>(few + i + 4 * u);
-#pragma unroll
-                        for (int u = 0; u < 32; u++) {
-                            more += r[u / 4][u % 4] > mine;
-                            as_much += r[u / 4][u % 4] >= mine;
-                        }
-                    }
-                    if (more < room && room <= as_much) {  // the same values, if several
-                        found[0] = (int)mine;
-                        found[1] = room - more;
-                        found[2] = as_much - more;
-                    }
-                }
-                __syncthreads();
-                above = (uint32_t)found[0];
-                room = found[1];
-                in_bin = found[2];
-                break;
-            }
             bits = shift == 21 ? 11 : 10;
         }
         // Kept: what exceeds `above`, which has the digits found and zeros behind
@@ -327,7 +294,7 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         // Lane i of a wave decides about its i-th 64 tokens, all bits at once.
         uint32_t ties = 0, lists[2] = {0, 0};  // of the pieces so far
         for (int piece = 0; piece < pieces; piece++) {
-            if (pieces > 1) load(piece);
+            if (pieces > 1) load(piece, false);
             uint64_t more = 0, same = 0;
             over_keys([&](int i, uint32_t r) {
                 const uint64_t x = __ballot(r > above), y = __ballot(r == above);
