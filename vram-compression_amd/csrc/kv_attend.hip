@@ -32,6 +32,12 @@
 // the lengths, which only the GPU knows, decide how many workgroups a sequence
 // gets.  A share that ends inside a sequence leaves a part; a second launch joins
 // the parts, and adds the weights to the tokens' mass where that is tracked.
+//
+// Measured: 16 sequences of up to 32768 tokens, 40 query heads over 8 of 128
+// columns: 271 us in bf16 (1.61 GB, 5.9 TB/s; VALU 10% busy, matrix cores 6%), 87
+// us from 4 bits (0.43 GB, 4.9 TB/s; 50% and 21%), and 5 us to join.  Short calls
+// are latency: one sequence of 32768 tokens over 2 heads 11.6 and 3.9 us, of 5
+// tokens 4.9 and 2.2.
 #include "kv_device.h"
 
 namespace {
@@ -85,8 +91,9 @@ __device__ __forceinline__ int units_of(int n) { return (n + kUnit - 1) / kUnit;
 
 // How units are dealt to workgroups: `rest` of them get one more than the others.
 // Beyond one for each CU, workgroups get two units at least: half as many parts
-// to join are worth more than a second workgroup's share of the latency (one
-// sequence of 32768 tokens: 15 us against 19).
+// to join are worth more than a second workgroup's share of the latency (three
+// sequences of 1777 tokens in f32: 15.2 us against 15.8; four of up to 4096 in 4
+// bits 14.8 against 15.1).
 struct Shares {
     uint32_t workers, each, rest;
     __device__ __forceinline__ Shares(uint32_t units, uint32_t most) {
@@ -285,7 +292,7 @@ struct Values {
 // Tiles of query heads that a wave takes at once: two where a kv head has more
 // than 16 and the registers hold their queries and sums beside the keys, so that
 // up to 32 heads read the cache once (16 sequences of up to 16384 tokens, 32
-// heads of 128 columns: 37 us against 42; 24 of 64 in f32 54 against 72).  4-bit
+// heads of 128 columns: 36 us against 42; 24 of 64 in f32 54 against 71).  4-bit
 // pages are cheap to read and dear to convert with fewer waves at it: one tile
 // (24 heads of 128 columns 35 us against 41).
 constexpr int pair_of(int size, bool mx, int dim, int group) {
@@ -296,10 +303,10 @@ constexpr int pair_of(int size, bool mx, int dim, int group) {
 // that the work is shared among.  Two cap the registers at 256, which also keeps
 // the sums in ordinary ones instead of accumulation registers, from where every
 // rescaling would have to copy them; with three, 128 columns spill (16 sequences
-// of up to 32768 tokens: 290 us against 276).  Rows of 4 bits are short and need
-// the third for the bytes under way (the same sequences: 90 us against 91; of
-// 16384 tokens and 64 columns 33 against 37); the widest rows fill one wave's
-// registers.
+// of up to 32768 tokens: 286 us against 276).  Rows of 4 bits are short and need
+// the third for the bytes under way (the same sequences: 93 us against 94; of
+// 16384 tokens 34 against 38 with 64 columns, 54 against 62 with 96); the widest
+// rows fill one wave's registers.
 constexpr int waves_of_simd(int size, bool mx, int dim, int pair) {
     if (pair == 2) return size * dim <= 256 ? 2 : 1;
     if (mx) return dim <= 128 ? 3 : 2;
@@ -637,9 +644,9 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
 // others add the weights of 1024 tokens of a kv head to their mass, from the
 // scores that the first launch left.  Where the workgroups make some eight parts
 // of a group or fewer, a thread joins four columns of a query head; where more, a
-// block joins 32 columns, 32 parts at a time: with 256 parts (one sequence of
-// 32768 tokens) that takes 5 us in place of 12, but 3072 blocks for 3 parts of
-// each of 768 heads take 12 us in place of 5.
+// block joins 32 columns, 32 parts at a time: one sequence of 131072 tokens takes
+// 30 us in place of 80, three of 1777 in f32 15.1 in place of 17.1, but 64 of 2049
+// (two parts of each of 768 heads) 33.7 us in place of 28.7.
 constexpr int kFewParts = 8;
 constexpr int kJoinColumns = 32, kJoinLanes = kJoinColumns / 4, kJoinParts = kThreads / kJoinLanes;
 constexpr int kMassKeys = 4 * kThreads, kMassHeads = kThreads / 16;
