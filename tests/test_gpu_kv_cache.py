@@ -282,6 +282,22 @@ def test_attend_one_long_sequence(kv, dtype, mx, length):
 
 
 @pytest.mark.parametrize("dtype,mx", STORES)
+@pytest.mark.parametrize("heads,group,top", [(8, 2, 60), (4, 3, 420), (2, 1, 900), (3, 18, 300)])
+def test_attend_many_sequences(kv, dtype, mx, heads, group, top):
+    """More groups than workgroups and fewer, so that a workgroup's share is
+    several groups, ends inside of one or where one starts; every fifth sequence
+    is empty.  The same call gives the same bits."""
+    rng = np.random.default_rng(top)
+    lengths = [0 if i % 5 == 3 else int(rng.integers(1, top)) for i in range(230)]
+    pages = sum(-(-n // 32) for n in lengths)
+    c = make(kv, dtype, mx, 64, 32, heads, pages, seed=top)
+    table, n = tables(lengths, 32, pages, seed=top)
+    q = torch.randn(len(lengths), heads * group, 64, device="cuda").to(DTYPES[dtype])
+    got = check_attend(kv, c, dtype, q, table, n)
+    assert torch.equal(c.attend(q, table, n), got)
+
+
+@pytest.mark.parametrize("dtype,mx", STORES)
 def test_attend_what_is_masked_can_be_anything(kv, dtype, mx):
     """Behind a sequence's last token lie NaN and infinities; table entries
     that are no page of the cache leave their tokens out; lengths beyond the

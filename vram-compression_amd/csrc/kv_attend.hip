@@ -89,15 +89,28 @@ __device__ __forceinline__ int length_of(const Attend& a, int b) {
 
 __device__ __forceinline__ int units_of(int n) { return (n + kUnit - 1) / kUnit; }
 
+// Units that starting a group is worth: its queries, page ids and first keys come
+// one after the other, and its waves' parts are joined.  A group's units then lie
+// behind as many empty ones, and a share of many short groups has fewer units than
+// one of a long group (8 kv heads of 128 columns: 256 sequences of up to 200 tokens
+// 48.2 -> 42.1 us, 64 of up to 1000 in 4 bits 22.7 -> 20.8).
+constexpr int kOpen = 2;
+
 // How units are dealt to workgroups: `rest` of them get one more than the others.
 // Beyond one for each CU, workgroups get two units at least: half as many parts
 // to join are worth more than a second workgroup's share of the latency (three
 // sequences of 1777 tokens in f32: 15.2 us against 15.8; four of up to 4096 in 4
 // bits 14.8 against 15.1).
 struct Shares {
-    uint32_t workers, each, rest;
-    __device__ __forceinline__ Shares(uint32_t units, uint32_t most) {
+    uint32_t workers, open, each, rest;
+    // units of all groups, and how many groups have any
+    __device__ __forceinline__ Shares(uint32_t units, uint32_t groups, uint32_t most) {
         workers = min(most, units <= kCus ? units : max((uint32_t)kCus, (units + 1) / 2));
+        // Not where hardly any share has more than one group, and not where both
+        // shares and groups are of few units, which are best cut evenly (64 sequences
+        // of up to 200 tokens 16.0 us against 18.8).
+        open = 4 * groups >= workers && units >= min(2 * groups, 3 * workers) ? kOpen : 0;
+        units += open * groups;
         each = workers ? units / workers : 0;
         rest = units - each * workers;
     }
@@ -320,29 +333,43 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
     constexpr int STEP = 16 * TILES, KEYS = 4 * TILES;
     constexpr int NT = D / 16;               // tiles of the output
     using C = Deal<D>;
-    __shared__ int wave_units[kWaves], place[2];
-    __shared__ float part[2][NT * 4 + 2][64];
+    __shared__ int wave_units[kWaves], wave_some[kWaves], place[2];
+    constexpr int JOIN = NT > 12 ? NT / 2 : NT;  // tiles that are joined at once, in 64 KB
+    __shared__ float part[kWaves][4][JOIN][64], part_of[kWaves][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4;
 
     // this workgroup's share: each thread counts some sequences' units
     const int each = (a.batch + kThreads - 1) / kThreads, b0 = threadIdx.x * each;
-    int mine = 0, before = 0, total = 0;
+    int mine = 0, some = 0, units_before = 0, some_before = 0, all_units = 0, all_some = 0;
     if (a.batch == 1) {  // nothing to count
-        total = units_of(length_of(a, 0));
+        all_units = units_of(length_of(a, 0));
+        all_some = all_units > 0;
     } else {
-        for (int i = b0; i < min(b0 + each, a.batch); i++) mine += units_of(length_of(a, i));
-        const int sum = wave_scan(mine);
-        if (lane == 63) wave_units[wave] = sum;
+        for (int i = b0; i < min(b0 + each, a.batch); i++) {
+            const int units = units_of(length_of(a, i));
+            mine += units;
+            some += units > 0;
+        }
+        const int sum = wave_scan(mine), have = wave_scan(some);
+        if (lane == 63) {
+            wave_units[wave] = sum;
+            wave_some[wave] = have;
+        }
         __syncthreads();
-        before = sum - mine;
+        units_before = sum - mine;
+        some_before = have - some;
 #pragma unroll
         for (int w = 0; w < kWaves; w++) {
-            before += w < wave ? wave_units[w] : 0;
-            total += wave_units[w];
+            units_before += w < wave ? wave_units[w] : 0;
+            some_before += w < wave ? wave_some[w] : 0;
+            all_units += wave_units[w];
+            all_some += wave_some[w];
         }
     }
-    const Shares shares(__builtin_amdgcn_readfirstlane(total) * (uint32_t)a.groups, gridDim.x);
+    const Shares shares(__builtin_amdgcn_readfirstlane(all_units) * (uint32_t)a.groups,
+                        __builtin_amdgcn_readfirstlane(all_some) * (uint32_t)a.groups, gridDim.x);
+    const int open = shares.open;
     for (int i = blockIdx.x; i < a.batch; i += gridDim.x)  // nothing to attend to
         if (length_of(a, i) == 0) {
             T* to = static_cast<T*>(a.out) + (int64_t)i * a.q_heads * D;
@@ -354,10 +381,16 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
     const uint32_t stop = shares.start(blockIdx.x + 1);
     int b = 0, off = (int)unit;
     if (a.batch > 1) {
-        if (unit >= (uint32_t)before * a.groups && unit < (uint32_t)(before + mine) * a.groups) {
-            uint32_t in = unit - (uint32_t)before * a.groups;
+        const uint32_t before = (uint32_t)(units_before + open * some_before) * a.groups;
+        if (unit >= before && unit - before < (uint32_t)(mine + open * some) * a.groups) {
+            uint32_t in = unit - before;
             int i = b0;
-            for (uint32_t x; in >= (x = (uint32_t)units_of(length_of(a, i)) * a.groups); i++) in -= x;
+            for (;; i++) {
+                const int units = units_of(length_of(a, i));
+                const uint32_t x = units ? (uint32_t)(units + open) * a.groups : 0;
+                if (in < x) break;
+                in -= x;
+            }
             place[0] = i;
             place[1] = (int)in;
         }
@@ -366,22 +399,38 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
         off = __builtin_amdgcn_readfirstlane(place[1]);
     }
     const float scale = a.scale * kLog2e;
+    int n = __builtin_amdgcn_readfirstlane(length_of(a, b));
 
     while (unit < stop) {
-    const int n = __builtin_amdgcn_readfirstlane(length_of(a, b)), units = units_of(n);
-    const int group = off / units, first_unit = off - group * units;
-    const int here = min((uint32_t)(units - first_unit), stop - unit);
+    const int units = units_of(n);
+    const int group = off / (units + open), in = off - group * (units + open);
+    const int dealt = min((uint32_t)(units + open - in), stop - unit);
+    const int first_unit = max(in - open, 0), here = in + dealt - open - first_unit;
+    if (here > 0) {
     const int h = group / a.head_tiles, first_head = group % a.head_tiles * a.tile;
     const int start = first_unit * kUnit, end = min(n, (first_unit + here) * kUnit);
-    const bool opens = first_unit == 0, alone = here == units;
+    const bool opens = in <= open, alone = here == units;
     if (opens && threadIdx.x == 0)
         a.spans[(int64_t)b * a.groups + group] =
-            make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + units - 1) - blockIdx.x + 1);
+            make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + (units + open - in) - 1) - blockIdx.x + 1);
     const auto head_of = [&](int r) { return first_head + 16 * r + (lane & 15); };
     const auto live = [&](int r) { return head_of(r) < a.group; };
     const auto q_row = [&](int r) { return (int64_t)b * a.q_heads + h * a.group + head_of(r); };
 
-    // the queries, in the keys' order of columns; heads beyond the group are zero
+    // Page ids of 64 of this wave's tiles of 16 keys, one a lane; the next 64 are
+    // fetched while these are used.
+    const int steps = (end - start + STEP - 1) / STEP;
+    const auto page_ids = [&](int window) {
+        const int tile = window * 64 + lane;
+        const int key = start + (wave + kWaves * (tile / TILES)) * STEP + tile % TILES * 16;
+        int id = -1;
+        if (key < end) id = a.table[b * a.table_row + (key >> a.page_shift)];
+        return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
+    };
+    int window = 0, ids = page_ids(0), next_ids = page_ids(1);
+
+    // the queries, in the keys' order of columns; columns of the tiles beyond the
+    // group repeat its first head, and are not written anywhere
     Half8<T> q[PAIR][F32 ? 1 : D / 32];
     vec<float, 4> qf[PAIR][F32 ? D / 16 : 1];
 #pragma unroll
@@ -403,25 +452,8 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
             if constexpr (F32) take(s, qf[r][s]);
             else take(s, q[r][s]);
         }
-        if (!live(r)) {
-#pragma unroll
-            for (auto& x : q[r]) x = {};
-#pragma unroll
-            for (auto& x : qf[r]) x = {};
-        }
     }
 
-    // Page ids of 64 of this wave's tiles of 16 keys, one a lane; the next 64 are
-    // fetched while these are used.
-    const int steps = (end - start + STEP - 1) / STEP;
-    const auto page_ids = [&](int window) {
-        const int tile = window * 64 + lane;
-        const int key = start + (wave + kWaves * (tile / TILES)) * STEP + tile % TILES * 16;
-        int id = -1;
-        if (key < end) id = a.table[b * a.table_row + (key >> a.page_shift)];
-        return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
-    };
-    int window = 0, ids = page_ids(0), next_ids = page_ids(1);
     // The step at hand.  As soon as its keys are multiplied the next step's take
     // their registers, and so with the values, so that some of both is always
     // under way.
@@ -585,57 +617,61 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
         l[r] += __shfl_xor(l[r], 32);
     }
 
-    // the waves' parts, joined in two rounds through LDS, register by register
-    for (int half = steps > 1 ? kWaves / 2 : 0; half; half /= 2) {
-#pragma unroll
-        for (int r = 0; r < PAIR; r++) {
-            if (wave >= half && wave < 2 * half) {
-                float(&to)[NT * 4 + 2][64] = part[wave - half];
-#pragma unroll
-                for (int i = 0; i < NT * 4; i++) to[i][lane] = o[r][i / 4][i % 4];
-                to[NT * 4][lane] = m[r];
-                to[NT * 4 + 1][lane] = l[r];
-            }
-            __syncthreads();
-            if (wave < half) {
-                const float(&in)[NT * 4 + 2][64] = part[wave];
-                const float other = in[NT * 4][lane], both = fmaxf(m[r], other);
-                const float x = exp2_of(m[r] - or_zero(both)), y = exp2_of(other - or_zero(both));
-                l[r] = l[r] * x + in[NT * 4 + 1][lane] * y;
-#pragma unroll
-                for (int i = 0; i < NT * 4; i++) o[r][i / 4][i % 4] = o[r][i / 4][i % 4] * x + in[i][lane] * y;
-                m[r] = both;
-            }
-            __syncthreads();
-        }
-    }
+    // The waves' parts, joined through LDS: wave w takes register w of every tile,
+    // neighbouring columns of a lane, and writes them.  (In two rounds of halves,
+    // one wave writing all: 256 sequences of up to 200 tokens in 4 bits 30 us
+    // against 26, 16 of up to 32768 276 against 274.)
 #pragma unroll
     for (int r = 0; r < PAIR; r++) {
-        if (wave || !live(r)) continue;
+        float top = -__builtin_inff(), sum = 0.f, w[kWaves], x[NT] = {};
+#pragma unroll
+        for (int c = 0; c < NT; c += JOIN) {
+            __syncthreads();  // what was there has been read
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int i = 0; i < JOIN; i++) part[wave][e][i][lane] = o[r][c + i][e];
+            if (c == 0) {
+                part_of[wave][0][lane] = m[r];
+                part_of[wave][1][lane] = l[r];
+            }
+            __syncthreads();
+            if (c == 0) {
+#pragma unroll
+                for (int u = 0; u < kWaves; u++) top = fmaxf(top, w[u] = part_of[u][0][lane]);
+#pragma unroll
+                for (int u = 0; u < kWaves; u++) {
+                    w[u] = exp2_of(w[u] - or_zero(top));
+                    sum += part_of[u][1][lane] * w[u];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < JOIN; i++)
+#pragma unroll
+                for (int u = 0; u < kWaves; u++) x[c + i] += part[u][wave][i][lane] * w[u];
+        }
+        if (!live(r)) continue;
+        const int column = 4 * g + wave;
         if (alone) {
-            if (a.scores && g == 0) a.sums[q_row(r)] = make_float2(m[r], l[r]);
-            const float x = l[r] == 0.f ? 0.f : 1.f / l[r];
+            if (a.scores && wave == 0 && g == 0) a.sums[q_row(r)] = make_float2(top, sum);
+            const float unit_sum = sum == 0.f ? 0.f : 1.f / sum;
             T* to = static_cast<T*>(a.out) + q_row(r) * D;
 #pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = (T)(l[r] == 0.f ? 0.f : o[r][i][e] * x);
+            for (int i = 0; i < NT; i++) to[C::column(i, column)] = (T)(sum == 0.f ? 0.f : x[i] * unit_sum);
         } else {
             const int64_t at = (int64_t)(2 * blockIdx.x + opens) * a.tile + 16 * r + (lane & 15);
-            if (g == 0) a.part_sums[at] = make_float2(m[r], l[r]);
+            if (wave == 0 && g == 0) a.part_sums[at] = make_float2(top, sum);
             float* to = a.parts + at * D;
 #pragma unroll
-            for (int i = 0; i < NT; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) to[C::column(i, 4 * g + e)] = o[r][i][e];
+            for (int i = 0; i < NT; i++) to[C::column(i, column)] = x[i];
         }
     }
-    unit += here;
-    off += here;
-    if (off == units * a.groups) {  // on to the next sequence that has tokens
+    }
+    unit += dealt;
+    off += dealt;
+    if (off == (units + open) * a.groups) {  // on to the next sequence that has tokens
         off = 0;
-        do b++;
-        while (unit < stop && __builtin_amdgcn_readfirstlane(length_of(a, b)) == 0);
+        while (unit < stop && (n = __builtin_amdgcn_readfirstlane(length_of(a, ++b))) == 0) {}
     }
     }
 }
