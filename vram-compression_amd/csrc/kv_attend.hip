@@ -827,10 +827,22 @@ __device__ __forceinline__ void add_mass(const Attend& a, int block) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] += exp2_of(s[i][e] - total[i].x) * total[i].y;
     }
-    if (key >= n || page < 0 || page >= a.c.pages) return;
-    float* mass = a.c.mass + (((int64_t)page * a.c.kv_heads + h) << a.page_shift) + (key & (a.c.page_size - 1));
-    for (int e = 0; e < 4; e++)
-        if (key + e < n) unsafeAtomicAdd(mass + e, w[e]);
+    // By neighbouring lanes to neighbouring tokens: as each lane's four, the additions
+    // of 16 sequences of up to 32768 tokens, 40 heads, took 25 us longer (393 against
+    // 368 us in all).
+    __shared__ __attribute__((aligned(16))) float sum[kMassKeys];
+    __shared__ int64_t places[kThreads];
+    const bool there = key < n && page >= 0 && page < a.c.pages;
+    *reinterpret_cast<vec<float, 4>*>(sum + 4 * threadIdx.x) = w;
+    places[threadIdx.x] =
+        there ? (((int64_t)page * a.c.kv_heads + h) << a.page_shift) + (key & (a.c.page_size - 1)) : -1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int i = e * kThreads + threadIdx.x;
+        const int64_t to = places[i / 4];
+        if (to >= 0 && tile * kMassKeys + i < n) unsafeAtomicAdd(a.c.mass + to + i % 4, sum[i]);
+    }
 }
 
 template <typename T>
