@@ -12,7 +12,8 @@
 //    that is just how the second product O^T = V^T P^T wants its right operand
 //    if its inner index runs over the keys in the order (tile, g, 0..3).  So
 //    weights never leave the lane that made them, softmax needs a lane's own
-//    values and two exchanges for the maximum, and no LDS is touched.
+//    values and two exchanges for the maximum, and no LDS is touched before the
+//    waves' sums are joined.
 //  - V^T wants eight keys of one column in a lane.  A lane loads neighbouring
 //    columns of eight keys (a row of the cache by 16 lanes, all of a page's
 //    bytes by a few instructions) and transposes pairs with byte permutes;
@@ -34,10 +35,10 @@
 // the parts, and adds the weights to the tokens' mass where that is tracked.
 //
 // Measured: 16 sequences of up to 32768 tokens, 40 query heads over 8 of 128
-// columns: 271 us in bf16 (1.61 GB, 5.9 TB/s; VALU 10% busy, matrix cores 6%), 87
-// us from 4 bits (0.43 GB, 4.9 TB/s; 50% and 21%), and 5 us to join.  Short calls
-// are latency: one sequence of 32768 tokens over 2 heads 11.6 and 3.9 us, of 5
-// tokens 4.9 and 2.2.
+// columns: 269 us in bf16 (1.61 GB, 6.0 TB/s; VALU 9% busy, matrix cores 6%), 85
+// us from 4 bits (0.43 GB, 5.0 TB/s; 52% and 22%), and 5 us to join.  Short calls
+// are latency: one sequence of 32768 tokens over 2 heads 10.9 and 4.0 us, of 5
+// tokens 5.5 and 1.9.
 #include "kv_device.h"
 
 namespace {
