@@ -403,277 +403,276 @@ __global__ void __launch_bounds__(kThreads, waves_of_simd(sizeof(T), MX, D, PAIR
     int n = __builtin_amdgcn_readfirstlane(length_of(a, b));
 
     while (unit < stop) {
-    const int units = units_of(n);
-    const int group = off / (units + open), in = off - group * (units + open);
-    const int dealt = min((uint32_t)(units + open - in), stop - unit);
-    const int first_unit = max(in - open, 0), here = in + dealt - open - first_unit;
-    if (here > 0) {
-    const int h = group / a.head_tiles, first_head = group % a.head_tiles * a.tile;
-    const int start = first_unit * kUnit, end = min(n, (first_unit + here) * kUnit);
-    const bool opens = in <= open, alone = here == units;
-    if (opens && threadIdx.x == 0)
-        a.spans[(int64_t)b * a.groups + group] =
-            make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + (units + open - in) - 1) - blockIdx.x + 1);
-    const auto head_of = [&](int r) { return first_head + 16 * r + (lane & 15); };
-    const auto live = [&](int r) { return head_of(r) < a.group; };
-    const auto q_row = [&](int r) { return (int64_t)b * a.q_heads + h * a.group + head_of(r); };
+        const int units = units_of(n), cost = units + open;
+        const int group = off / cost, in = off - group * cost;
+        const int dealt = min((uint32_t)(cost - in), stop - unit);
+        const int first_unit = max(in - open, 0), here = in + dealt - open - first_unit;
+        if (here <= 0) break;  // the share ends in a group's empty units
+        const int h = group / a.head_tiles, first_head = group % a.head_tiles * a.tile;
+        const int start = first_unit * kUnit, end = min(n, (first_unit + here) * kUnit);
+        const bool opens = in <= open, alone = here == units;
+        if (opens && threadIdx.x == 0)
+            a.spans[(int64_t)b * a.groups + group] =
+                make_int2(blockIdx.x, alone ? 1 : shares.worker_of(unit + (cost - in) - 1) - blockIdx.x + 1);
+        const auto head_of = [&](int r) { return first_head + 16 * r + (lane & 15); };
+        const auto live = [&](int r) { return head_of(r) < a.group; };
+        const auto q_row = [&](int r) { return (int64_t)b * a.q_heads + h * a.group + head_of(r); };
 
-    // Page ids of 64 of this wave's tiles of 16 keys, one a lane; the next 64 are
-    // fetched while these are used.
-    const int steps = (end - start + STEP - 1) / STEP;
-    const auto page_ids = [&](int window) {
-        const int tile = window * 64 + lane;
-        const int key = start + (wave + kWaves * (tile / TILES)) * STEP + tile % TILES * 16;
-        int id = -1;
-        if (key < end) id = a.table[b * a.table_row + (key >> a.page_shift)];
-        return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
-    };
-    int window = 0, ids = page_ids(0), next_ids = page_ids(1);
-
-    // the queries, in the keys' order of columns; columns of the tiles beyond the
-    // group repeat its first head, and are not written anywhere
-    Half8<T> q[PAIR][F32 ? 1 : D / 32];
-    vec<float, 4> qf[PAIR][F32 ? D / 16 : 1];
-#pragma unroll
-    for (int r = 0; r < PAIR; r++) {
-        constexpr int N = F32 ? 4 : 8;
-        const T* p = static_cast<const T*>(a.q) + b * a.q_seq +
-                     (int64_t)(h * a.group + (live(r) ? head_of(r) : first_head)) * a.q_head;
-        const auto take = [&](int s, auto& x) {
-            const T* from = p + Keys<T, MX, D>::column(s, g);
-            if (a.q_wide) {
-                x = *reinterpret_cast<const vec<T, N>*>(from);
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; i++) x[i] = from[i];
-            }
+        // Page ids of 64 of this wave's tiles of 16 keys, one a lane; the next 64 are
+        // fetched while these are used.
+        const int steps = (end - start + STEP - 1) / STEP;
+        const auto page_ids = [&](int window) {
+            const int tile = window * 64 + lane;
+            const int key = start + (wave + kWaves * (tile / TILES)) * STEP + tile % TILES * 16;
+            int id = -1;
+            if (key < end) id = a.table[b * a.table_row + (key >> a.page_shift)];
+            return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
         };
-#pragma unroll
-        for (int s = 0; s < D / (F32 ? 16 : 32); s++) {
-            if constexpr (F32) take(s, qf[r][s]);
-            else take(s, q[r][s]);
-        }
-    }
+        int window = 0, ids = page_ids(0), next_ids = page_ids(1);
 
-    // The step at hand.  As soon as its keys are multiplied the next step's take
-    // their registers, and so with the values, so that some of both is always
-    // under way.
-    Keys<T, MX, D> k[TILES];
-    Values<T, MX, D, KEYS> v;
-    int page[TILES];
-    int64_t row[TILES];
-    const auto find = [&](int t) {  // page 0 stands in for a missing one
-        const int tile = t / kWaves * TILES;
-        if (tile / 64 != window) {
-            ids = next_ids;
-            next_ids = page_ids(++window + 1);
-        }
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            page[i] = __builtin_amdgcn_readlane(ids, tile % 64 + i);
-            row[i] = (((int64_t)max(page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
-                       ((start + t * STEP + i * 16) & (a.c.page_size - 1));
-        }
-    };
-    const auto load_keys = [&] {
-#pragma unroll
-        for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
-    };
-
-    vec<float, 4> o[PAIR][NT] = {};
-    float m[PAIR], from[PAIR] = {}, l[PAIR] = {};
-#pragma unroll
-    for (int r = 0; r < PAIR; r++) m[r] = -__builtin_inff();
-    if (wave < steps) {
-        find(wave);
-        load_keys();
-        v.load(a.c, row, lane);
-    }
-    for (int t = wave; t < steps; t += kWaves) {
-        const int key0 = start + t * STEP;
-        bool whole = key0 + STEP <= end;
-        bool there[TILES];
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            there[i] = page[i] >= 0;
-            whole &= there[i];
-        }
-        vec<float, 4> s[PAIR][TILES] = {};
-#pragma unroll
-        for (int i = 0; i < TILES; i++) {
-            if constexpr (F32) {
-#pragma unroll
-                for (int c = 0; c < D / 16; c++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-#pragma unroll
-                        for (int r = 0; r < PAIR; r++)
-                            s[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
-                                                                           qf[r][c][e], s[r][i], 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int c = 0; c < D / 32; c++) {
-                    const auto x = k[i].operand(c, g);
-#pragma unroll
-                    for (int r = 0; r < PAIR; r++) s[r][i] = mma(x, q[r][c], s[r][i]);
-                }
-            }
-        }
-        const bool more = t + kWaves < steps;
-        if (more) {
-            find(t + kWaves);
-            load_keys();
-        }
-        if (!whole) {
-#pragma unroll
-            for (int j = 0; j < KEYS; j++) v.clear(j, !there[j >> 2] || key0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end);
-        }
-        float p[PAIR][KEYS];
+        // the queries, in the keys' order of columns; columns of the tiles beyond the
+        // group repeat its first head, and are not written anywhere
+        Half8<T> q[PAIR][F32 ? 1 : D / 32];
+        vec<float, 4> qf[PAIR][F32 ? D / 16 : 1];
 #pragma unroll
         for (int r = 0; r < PAIR; r++) {
+            constexpr int N = F32 ? 4 : 8;
+            const T* p = static_cast<const T*>(a.q) + b * a.q_seq +
+                         (int64_t)(h * a.group + (live(r) ? head_of(r) : first_head)) * a.q_head;
+            const auto take = [&](int s, auto& x) {
+                const T* from = p + Keys<T, MX, D>::column(s, g);
+                if (a.q_wide) {
+                    x = *reinterpret_cast<const vec<T, N>*>(from);
+                } else {
 #pragma unroll
-            for (int i = 0; i < TILES; i++)
+                    for (int i = 0; i < N; i++) x[i] = from[i];
+                }
+            };
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[r][i][e] *= scale;
+            for (int s = 0; s < D / (F32 ? 16 : 32); s++) {
+                if constexpr (F32) take(s, qf[r][s]);
+                else take(s, q[r][s]);
+            }
+        }
+
+        // The step at hand.  As soon as its keys are multiplied the next step's take
+        // their registers, and so with the values, so that some of both is always
+        // under way.
+        Keys<T, MX, D> k[TILES];
+        Values<T, MX, D, KEYS> v;
+        int page[TILES];
+        int64_t row[TILES];
+        const auto find = [&](int t) {  // page 0 stands in for a missing one
+            const int tile = t / kWaves * TILES;
+            if (tile / 64 != window) {
+                ids = next_ids;
+                next_ids = page_ids(++window + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                page[i] = __builtin_amdgcn_readlane(ids, tile % 64 + i);
+                row[i] = (((int64_t)max(page[i], 0) * a.c.kv_heads + h) << a.page_shift) +
+                           ((start + t * STEP + i * 16) & (a.c.page_size - 1));
+            }
+        };
+        const auto load_keys = [&] {
+#pragma unroll
+            for (int i = 0; i < TILES; i++) k[i].load(a.c, row[i], lane);
+        };
+
+        vec<float, 4> o[PAIR][NT] = {};
+        float m[PAIR], from[PAIR] = {}, l[PAIR] = {};
+#pragma unroll
+        for (int r = 0; r < PAIR; r++) m[r] = -__builtin_inff();
+        if (wave < steps) {
+            find(wave);
+            load_keys();
+            v.load(a.c, row, lane);
+        }
+        for (int t = wave; t < steps; t += kWaves) {
+            const int key0 = start + t * STEP;
+            bool whole = key0 + STEP <= end;
+            bool there[TILES];
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                there[i] = page[i] >= 0;
+                whole &= there[i];
+            }
+            vec<float, 4> s[PAIR][TILES] = {};
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int c = 0; c < D / 16; c++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+#pragma unroll
+                            for (int r = 0; r < PAIR; r++)
+                                s[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i].x[c].w[e]),
+                                                                               qf[r][c][e], s[r][i], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        const auto x = k[i].operand(c, g);
+#pragma unroll
+                        for (int r = 0; r < PAIR; r++) s[r][i] = mma(x, q[r][c], s[r][i]);
+                    }
+                }
+            }
+            const bool more = t + kWaves < steps;
+            if (more) {
+                find(t + kWaves);
+                load_keys();
+            }
             if (!whole) {
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (!there[i] || key0 + 16 * i + 4 * g + e >= end) s[r][i][e] = -__builtin_inff();
+                for (int j = 0; j < KEYS; j++) v.clear(j, !there[j >> 2] || key0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end);
             }
-            if (a.scores && live(r)) {
-#pragma unroll
-                for (int i = 0; i < TILES; i++)
-                    if (key0 + 16 * i < a.bound)
-                        *reinterpret_cast<vec<float, 4>*>(a.scores + q_row(r) * a.bound + key0 + 16 * i + 4 * g) = s[r][i];
-            }
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < TILES; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) top = fmaxf(top, s[r][i][e]);
-            if (__builtin_expect(__any(top > m[r] + kSlack<T>), 0)) {
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                if (top > m[r] + kSlack<T>) {
-                    from[r] = or_zero(top - kBelow<T>);
-                    const float keep = exp2_of(m[r] - from[r]);
-                    l[r] *= keep;
-#pragma unroll
-                    for (int i = 0; i < NT; i++) o[r][i] *= keep;
-                    m[r] = top - kBelow<T>;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < KEYS; j++) {
-                p[r][j] = exp2_of(s[r][j >> 2][j & 3] - from[r]);
-                l[r] += p[r][j];
-            }
-        }
-        if constexpr (F32) {
-#pragma unroll
-            for (int j = 0; j < KEYS; j++)
-#pragma unroll
-                for (int i = 0; i < NT; i++)
-#pragma unroll
-                    for (int r = 0; r < PAIR; r++)
-                        o[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[r][j], o[r][i], 0, 0, 0);
-        } else {
-            Half8<T> hi[PAIR], lo[PAIR];
+            float p[PAIR][KEYS];
 #pragma unroll
             for (int r = 0; r < PAIR; r++) {
-                vec<T, 2> hi2[4], lo2[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const vec<float, 2> w = {p[r][2 * j], p[r][2 * j + 1]};
-                    hi2[j] = __builtin_convertvector(w, vec<T, 2>);
-                    lo2[j] = __builtin_convertvector(w - __builtin_convertvector(hi2[j], vec<float, 2>), vec<T, 2>);
+                for (int i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[r][i][e] *= scale;
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < TILES; i++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (!there[i] || key0 + 16 * i + 4 * g + e >= end) s[r][i][e] = -__builtin_inff();
                 }
-                hi[r] = __builtin_bit_cast(Half8<T>, hi2);
-                lo[r] = __builtin_bit_cast(Half8<T>, lo2);
+                if (a.scores && live(r)) {
+#pragma unroll
+                    for (int i = 0; i < TILES; i++)
+                        if (key0 + 16 * i < a.bound)
+                            *reinterpret_cast<vec<float, 4>*>(a.scores + q_row(r) * a.bound + key0 + 16 * i + 4 * g) = s[r][i];
+                }
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = fmaxf(top, s[r][i][e]);
+                if (__builtin_expect(__any(top > m[r] + kSlack<T>), 0)) {
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    if (top > m[r] + kSlack<T>) {
+                        from[r] = or_zero(top - kBelow<T>);
+                        const float keep = exp2_of(m[r] - from[r]);
+                        l[r] *= keep;
+#pragma unroll
+                        for (int i = 0; i < NT; i++) o[r][i] *= keep;
+                        m[r] = top - kBelow<T>;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < KEYS; j++) {
+                    p[r][j] = exp2_of(s[r][j >> 2][j & 3] - from[r]);
+                    l[r] += p[r][j];
+                }
             }
+            if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < NT / 2; i++) {
-                vec<uint32_t, 4> even, odd;
+                for (int j = 0; j < KEYS; j++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t y = v.pair(i, 2 * j), z = v.pair(i, 2 * j + 1);
-                    even[j] = __builtin_amdgcn_perm(z, y, 0x05040100);
-                    odd[j] = __builtin_amdgcn_perm(z, y, 0x07060302);
-                }
-                const auto e = __builtin_bit_cast(Half8<T>, even), f = __builtin_bit_cast(Half8<T>, odd);
+                    for (int i = 0; i < NT; i++)
+#pragma unroll
+                        for (int r = 0; r < PAIR; r++)
+                            o[r][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.value(i, j), p[r][j], o[r][i], 0, 0, 0);
+            } else {
+                Half8<T> hi[PAIR], lo[PAIR];
 #pragma unroll
                 for (int r = 0; r < PAIR; r++) {
-                    o[r][2 * i] = mma(e, lo[r], mma(e, hi[r], o[r][2 * i]));
-                    o[r][2 * i + 1] = mma(f, lo[r], mma(f, hi[r], o[r][2 * i + 1]));
+                    vec<T, 2> hi2[4], lo2[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const vec<float, 2> w = {p[r][2 * j], p[r][2 * j + 1]};
+                        hi2[j] = __builtin_convertvector(w, vec<T, 2>);
+                        lo2[j] = __builtin_convertvector(w - __builtin_convertvector(hi2[j], vec<float, 2>), vec<T, 2>);
+                    }
+                    hi[r] = __builtin_bit_cast(Half8<T>, hi2);
+                    lo[r] = __builtin_bit_cast(Half8<T>, lo2);
+                }
+#pragma unroll
+                for (int i = 0; i < NT / 2; i++) {
+                    vec<uint32_t, 4> even, odd;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t y = v.pair(i, 2 * j), z = v.pair(i, 2 * j + 1);
+                        even[j] = __builtin_amdgcn_perm(z, y, 0x05040100);
+                        odd[j] = __builtin_amdgcn_perm(z, y, 0x07060302);
+                    }
+                    const auto e = __builtin_bit_cast(Half8<T>, even), f = __builtin_bit_cast(Half8<T>, odd);
+#pragma unroll
+                    for (int r = 0; r < PAIR; r++) {
+                        o[r][2 * i] = mma(e, lo[r], mma(e, hi[r], o[r][2 * i]));
+                        o[r][2 * i + 1] = mma(f, lo[r], mma(f, hi[r], o[r][2 * i + 1]));
+                    }
                 }
             }
+            if (more) v.load(a.c, row, lane);
         }
-        if (more) v.load(a.c, row, lane);
-    }
 #pragma unroll
-    for (int r = 0; r < PAIR; r++) {
-        l[r] += __shfl_xor(l[r], 16);
-        l[r] += __shfl_xor(l[r], 32);
-    }
+        for (int r = 0; r < PAIR; r++) {
+            l[r] += __shfl_xor(l[r], 16);
+            l[r] += __shfl_xor(l[r], 32);
+        }
 
-    // The waves' parts, joined through LDS: wave w takes register w of every tile,
-    // neighbouring columns of a lane, and writes them.  (In two rounds of halves,
-    // one wave writing all: 256 sequences of up to 200 tokens in 4 bits 30 us
-    // against 26, 16 of up to 32768 276 against 274.)
+        // The waves' parts, joined through LDS: wave w takes register w of every tile,
+        // neighbouring columns of a lane, and writes them.  (In two rounds of halves,
+        // one wave writing all: 256 sequences of up to 200 tokens in 4 bits 30 us
+        // against 26, 16 of up to 32768 276 against 274.)
 #pragma unroll
-    for (int r = 0; r < PAIR; r++) {
-        float top = -__builtin_inff(), sum = 0.f, w[kWaves], x[NT] = {};
+        for (int r = 0; r < PAIR; r++) {
+            float top = -__builtin_inff(), sum = 0.f, w[kWaves], x[NT] = {};
 #pragma unroll
-        for (int c = 0; c < NT; c += JOIN) {
-            __syncthreads();  // what was there has been read
+            for (int c = 0; c < NT; c += JOIN) {
+                __syncthreads();  // what was there has been read
 #pragma unroll
-            for (int e = 0; e < 4; e++)
+                for (int e = 0; e < 4; e++)
 #pragma unroll
-                for (int i = 0; i < JOIN; i++) part[wave][e][i][lane] = o[r][c + i][e];
-            if (c == 0) {
-                part_of[wave][0][lane] = m[r];
-                part_of[wave][1][lane] = l[r];
-            }
-            __syncthreads();
-            if (c == 0) {
-#pragma unroll
-                for (int u = 0; u < kWaves; u++) top = fmaxf(top, w[u] = part_of[u][0][lane]);
-#pragma unroll
-                for (int u = 0; u < kWaves; u++) {
-                    w[u] = exp2_of(w[u] - or_zero(top));
-                    sum += part_of[u][1][lane] * w[u];
+                    for (int i = 0; i < JOIN; i++) part[wave][e][i][lane] = o[r][c + i][e];
+                if (c == 0) {
+                    part_of[wave][0][lane] = m[r];
+                    part_of[wave][1][lane] = l[r];
                 }
+                __syncthreads();
+                if (c == 0) {
+#pragma unroll
+                    for (int u = 0; u < kWaves; u++) top = fmaxf(top, w[u] = part_of[u][0][lane]);
+#pragma unroll
+                    for (int u = 0; u < kWaves; u++) {
+                        w[u] = exp2_of(w[u] - or_zero(top));
+                        sum += part_of[u][1][lane] * w[u];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < JOIN; i++)
+#pragma unroll
+                    for (int u = 0; u < kWaves; u++) x[c + i] += part[u][wave][i][lane] * w[u];
             }
+            if (!live(r)) continue;
+            const int column = 4 * g + wave;
+            if (alone) {
+                if (a.scores && wave == 0 && g == 0) a.sums[q_row(r)] = make_float2(top, sum);
+                const float unit_sum = sum == 0.f ? 0.f : 1.f / sum;
+                T* to = static_cast<T*>(a.out) + q_row(r) * D;
 #pragma unroll
-            for (int i = 0; i < JOIN; i++)
+                for (int i = 0; i < NT; i++) to[C::column(i, column)] = (T)(sum == 0.f ? 0.f : x[i] * unit_sum);
+            } else {
+                const int64_t at = (int64_t)(2 * blockIdx.x + opens) * a.tile + 16 * r + (lane & 15);
+                if (wave == 0 && g == 0) a.part_sums[at] = make_float2(top, sum);
+                float* to = a.parts + at * D;
 #pragma unroll
-                for (int u = 0; u < kWaves; u++) x[c + i] += part[u][wave][i][lane] * w[u];
+                for (int i = 0; i < NT; i++) to[C::column(i, column)] = x[i];
+            }
         }
-        if (!live(r)) continue;
-        const int column = 4 * g + wave;
-        if (alone) {
-            if (a.scores && wave == 0 && g == 0) a.sums[q_row(r)] = make_float2(top, sum);
-            const float unit_sum = sum == 0.f ? 0.f : 1.f / sum;
-            T* to = static_cast<T*>(a.out) + q_row(r) * D;
-#pragma unroll
-            for (int i = 0; i < NT; i++) to[C::column(i, column)] = (T)(sum == 0.f ? 0.f : x[i] * unit_sum);
-        } else {
-            const int64_t at = (int64_t)(2 * blockIdx.x + opens) * a.tile + 16 * r + (lane & 15);
-            if (wave == 0 && g == 0) a.part_sums[at] = make_float2(top, sum);
-            float* to = a.parts + at * D;
-#pragma unroll
-            for (int i = 0; i < NT; i++) to[C::column(i, column)] = x[i];
+        unit += dealt;
+        off += dealt;
+        if (off == cost * a.groups) {  // on to the next sequence that has tokens
+            off = 0;
+            while (unit < stop && (n = __builtin_amdgcn_readfirstlane(length_of(a, ++b))) == 0) {}
         }
-    }
-    }
-    unit += dealt;
-    off += dealt;
-    if (off == (units + open) * a.groups) {  // on to the next sequence that has tokens
-        off = 0;
-        while (unit < stop && (n = __builtin_amdgcn_readfirstlane(length_of(a, ++b))) == 0) {}
-    }
     }
 }
 
