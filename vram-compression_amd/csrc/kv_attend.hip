@@ -35,8 +35,8 @@
 // the parts, and adds the weights to the tokens' mass where that is tracked.
 //
 // Measured: 16 sequences of up to 32768 tokens, 40 query heads over 8 of 128
-// columns: 269 us in bf16 (1.61 GB, 6.0 TB/s; VALU 9% busy, matrix cores 6%), 85
-// us from 4 bits (0.43 GB, 5.0 TB/s; 52% and 22%), and 5 us to join.  Short calls
+// columns: 269 us in bf16 (1.61 GB, 6.0 TB/s; VALU 10% busy, matrix cores 6%), 85
+// us from 4 bits (0.43 GB, 5.0 TB/s; 51% and 21%), and 5 us to join.  Short calls
 // are latency: one sequence of 32768 tokens over 2 heads 10.9 and 4.0 us, of 5
 // tokens 5.5 and 1.9.
 #include "kv_device.h"
