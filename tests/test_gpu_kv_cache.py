@@ -363,6 +363,23 @@ def test_attend_scores_that_are_not_finite(kv, dtype):
     assert np.isnan(got[2]).all() and np.isnan(got[3]).all()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_attend_values_that_are_not_finite(kv, dtype):
+    """They spoil their own column, for the heads and the sequence that read
+    them, and nothing else."""
+    c = make(kv, dtype, False, 64, 16, 2, 12, seed=6)
+    table, n = tables([70, 100], 16, 12, seed=6)
+    q = torch.randn(2, 6, 64, device="cuda").to(DTYPES[dtype])
+    want = c.attend(q, table, n)
+    c.v[table[0, 2], 0, 5, 17] = math.inf
+    c.v[table[1, 6], 1, 3, 40] = math.nan
+    got = c.attend(q, table, n)
+    spoiled = torch.zeros_like(got, dtype=torch.bool)
+    spoiled[0, :3, 17] = spoiled[1, 3:, 40] = True
+    assert not torch.isfinite(got[spoiled]).any()
+    assert torch.equal(got[~spoiled], want[~spoiled])
+
+
 @pytest.mark.parametrize("dtype,mx", STORES)
 def test_attend_scores_far_apart(kv, dtype, mx):
     """Scores in the thousands: the running maximum carries, the largest token
