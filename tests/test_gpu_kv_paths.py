@@ -1,0 +1,44 @@
+"""Paths of the key-value cache's kernels that only certain sizes reach, each
+against a plain implementation in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv(rans):
+    import kv_cache
+    return kv_cache
+
+
+@pytest.mark.parametrize("length", [32768, 32769, 65537, 140000])
+@pytest.mark.parametrize("budget_of", [lambda n: n - 3, lambda n: n // 2, lambda n: 700])
+def test_evict_in_pieces(kv, length, budget_of):
+    """Keys that are held at once and keys that go through in pieces, every
+    digit of them: masses differ in their last bits only, or are one of few."""
+    budget, page = budget_of(length), 128
+    pages = -(-length // page)
+    for seed, few in ((0, False), (1, True)):
+        g = torch.Generator(device="cuda").manual_seed(length + seed)
+        c = kv.PagedCache.allocate(pages, 2, 64, page, torch.float16, mx=True, track=True)
+        c.k.copy_(torch.randint(0, 256, c.k.shape, device="cuda", generator=g))
+        bits = torch.randint(0, 4 if few else 5000, c.mass.shape, device="cuda", generator=g)
+        c.mass.copy_((bits + 0x3f800000).int().view(torch.float32))
+        c.position.copy_(torch.arange(pages * page, device="cuda").view(pages, 1, page).expand_as(c.mass))
+        table = torch.randperm(pages, device="cuda", generator=g).int()[None]
+        n = torch.tensor([length], dtype=torch.int32, device="cuda")
+        mass, position, k = (getattr(c, w)[table[0].long()].transpose(0, 1).flatten(1, 2).cpu().numpy()
+                             for w in ("mass", "position", "k"))
+        assert c.evict(table, n, n, budget, 100).tolist() == [budget]
+        got = [getattr(c, w)[table[0].long()].transpose(0, 1).flatten(1, 2).cpu().numpy()
+               for w in ("mass", "position", "k")]
+        for h in range(2):
+            recent = position[h, :length] >= length - 100
+            order = np.lexsort((np.arange(length), -mass[h, :length].astype(np.float64), ~recent))
+            kept = np.sort(order[:budget])
+            at = np.arange(budget)
+            at[np.setdiff1d(at, kept)] = kept[kept >= budget]
+            for x, y in zip((mass, position, k), got):
+                assert np.array_equal(y[h, :budget], x[h][at])

@@ -67,6 +67,14 @@ __device__ __forceinline__ uint32_t rank_of(float m, int position, bool there, i
     return !there ? 1 : position >= recent ? 0xffffffffu : sorted;
 }
 
+// What a wave's lanes wrote to or read from LDS before, for its other lanes that
+// read or write there next.
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Copies the tokens of list entries first .. first + kRows - 1, below count, of
 // a kv head, by one wave: 16 bytes a lane, two loads of keys and two of values
 // before the first store (16 sequences of 16384 tokens in 4 bits cut to 2048: 37.4
@@ -94,10 +102,7 @@ __device__ __forceinline__ void move_rows(const Evict& e, int group, int first, 
             e.c.position[to] = p;
         }
     }
-    // the wave's own writes to LDS before its reads of them by other lanes
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_order();
     const int wide = e.c.mx ? e.c.head_dim / 32 : e.c.head_dim * (e.c.dtype == RANS_X_F32 ? 4 : 2) / 16;
     auto* k = static_cast<vec<uint32_t, 4>*>(e.c.k);
     auto* v = static_cast<vec<uint32_t, 4>*>(e.c.v);
@@ -225,6 +230,7 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                     m[u] = *reinterpret_cast<const vec<float, 4>*>(e.c.mass + at);
                     p[u] = *reinterpret_cast<const vec<int, 4>*>(e.c.position + at);
                 }
+            wave_order();  // other lanes have read the last piece's keys
 #pragma unroll
             for (int u = 0; u < kKeys / 4; u++)
                 if (4 * u < each) {
@@ -237,6 +243,7 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                         }
                     to[64 * u] = r;
                 }
+            wave_order();
         };
         const auto over_keys = [&](auto f) {  // f(i, key): the wave's tokens 64 * i..
             for (int i = 0; i < each; i += 4) {
