@@ -92,8 +92,9 @@ int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q_seq, int64
  * other sequences share must not be passed.  Otherwise all kept tokens of
  * every sequence are copied, in order, to the pages into[b*into_row + i/
  * page_size], which must be none of the sequences' own.  Keys, values, mass
- * and position move together.  new_lengths[b] = min(lengths[b], budget).
- * workspace as above. */
+ * and position move together.  new_lengths[b] = min(lengths[b], budget); it must
+ * share no memory with lengths, seen, table or into (RANS_EARG).  workspace as
+ * above. */
 int64_t vramc_kv_evict_workspace(const vramc_kv_cache* c, int table_width, int batch, int budget,
                                  int into);
 int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int64_t table_row,

@@ -372,6 +372,20 @@ int64_t most_moves(const vramc_kv_cache& c, int table_width, int budget, bool in
     return budget < over ? budget : over;
 }
 
+// Whether n integers at a share memory with rows of `wide` at b, `step` apart.
+bool overlap(const int32_t* a, int64_t n, const int32_t* b, int64_t step, int64_t wide, int64_t rows) {
+    const auto meets = [&](int64_t from, int64_t to) {  // integers of b
+        return (uintptr_t)a < (uintptr_t)(b + to) && (uintptr_t)(b + from) < (uintptr_t)(a + n);
+    };
+    const int64_t last = step * (rows - 1);
+    bool any = wide > 0 && meets(last < 0 ? last : 0, (last > 0 ? last : 0) + wide);
+    if (any && rows > 1) {  // or only with what lies between the rows
+        any = false;
+        for (int64_t r = 0; r < rows && !any; r++) any = meets(r * step, r * step + wide);
+    }
+    return any;
+}
+
 }  // namespace
 
 extern "C" int64_t vramc_kv_evict_workspace(const vramc_kv_cache* c, int table_width, int batch,
@@ -395,6 +409,12 @@ extern "C" int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int
     const int64_t most = most_moves(*c, table_width, budget, into != nullptr);
     if (into && (int64_t)into_width * c->page_size < most) return RANS_EARG;
     if (!workspace || workspace_bytes < need) return RANS_EWORKSPACE;
+    // Workgroups read all of these while others write the new lengths.
+    if ((uintptr_t)workspace % 16 || overlap(new_lengths, batch, lengths, 0, batch, 1) ||
+        overlap(new_lengths, batch, seen, 0, batch, 1) ||
+        overlap(new_lengths, batch, table, table_row, table_width, batch) ||
+        (into && overlap(new_lengths, batch, into, into_row, into_width, batch)))
+        return RANS_EARG;
     const int64_t heads = (int64_t)batch * c->kv_heads;
     auto* count = static_cast<int32_t*>(workspace);
     Evict e{*c, __builtin_ctz(c->page_size), table, table_row, table_width * c->page_size, lengths,
