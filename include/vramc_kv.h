@@ -86,15 +86,18 @@ int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q_seq, int64
 /* Cuts every sequence longer than `budget` to that many tokens, each kv head
  * by itself: kept first are the tokens with position >= seen[b] - recent, then
  * those of the largest mass (NaN counts as -infinity), ties to the lower
- * index; tokens whose table entry is no page of the cache go first.  With into
- * = NULL the kept tokens stay where they are and those at index >= budget, in
- * order, move into the places that became free below it, in order: pages that
- * other sequences share must not be passed.  Otherwise all kept tokens of
- * every sequence are copied, in order, to the pages into[b*into_row + i/
- * page_size], which must be none of the sequences' own.  Keys, values, mass
- * and position move together.  new_lengths[b] = min(lengths[b], budget); it must
- * share no memory with lengths, seen, table or into (RANS_EARG).  workspace as
- * above. */
+ * index.  Tokens whose table entry is no page of the cache are never kept, and
+ * places whose entry is none are never filled: where some of the first
+ * min(lengths[b], budget) places are such, as many fewer tokens are kept.  With
+ * into = NULL the kept tokens stay where they are and those at index >= budget,
+ * in order, move into the places that became free below it, in order: pages
+ * that other sequences share must not be passed.  Otherwise the kept tokens of
+ * every sequence, also of one within the budget, are copied, in order, to the
+ * places of the pages into[b*into_row + i/page_size], which must be none of the
+ * sequences' own.  Keys, values, mass and position move together.
+ * new_lengths[b] = min(lengths[b], budget), or with into, where there are fewer
+ * tokens than places, the place behind the last that is filled; it must share no
+ * memory with lengths, seen, table or into (RANS_EARG).  workspace as above. */
 int64_t vramc_kv_evict_workspace(const vramc_kv_cache* c, int table_width, int batch, int budget,
                                  int into);
 int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int64_t table_row,

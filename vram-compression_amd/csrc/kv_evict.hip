@@ -57,6 +57,15 @@ __device__ __forceinline__ int64_t place(const Evict& e, const int32_t* row, int
     return ((((int64_t)page * e.c.kv_heads + h) << e.page_shift) + (j & (e.c.page_size - 1)));
 }
 
+// The i-th index of a row that has a page; there are more than i.
+__device__ __forceinline__ int nth_place(const Evict& e, const int32_t* row, int i) {
+    for (int k = 0;; k++) {
+        if ((uint32_t)row[k] >= (uint32_t)e.c.pages) continue;
+        if (i < e.c.page_size) return (k << e.page_shift) + i;
+        i -= e.c.page_size;
+    }
+}
+
 // Sorts as the order in which tokens are kept: 1 for a token that is nowhere,
 // the mass's bits made monotonic (NaN as -infinity), all ones for a recent one.
 // 0 stands behind a sequence's last token and is never among the kept.
@@ -177,25 +186,58 @@ __device__ __forceinline__ uint64_t lowest_set(uint64_t x, int n) {
 }
 
 __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_here) {
-    extern __shared__ uint32_t piece_keys[];
+    extern __shared__ __attribute__((aligned(16))) uint32_t piece_keys[];
     __shared__ int hist[kBins], found[3];
+    __shared__ int absent, gaps;  // tokens, and places of the other pages, that have no page
     __shared__ uint32_t waves[kWaves];
     __shared__ int64_t rows[kWaves][2][kRows];
     const int b = blockIdx.x / e.c.kv_heads, h = blockIdx.x % e.c.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = min(max(e.lengths[b], 0), e.bound);
     const int32_t* row = e.table + b * e.table_row;
+    const int32_t* other = e.into ? e.into + b * e.into_row : nullptr;
     const int recent = (int)max((int64_t)e.seen[b] - e.recent, (int64_t)INT32_MIN);
-    if (h == 0 && threadIdx.x == 0) e.new_lengths[b] = min(n, e.budget);
+    const int keep = min(n, e.budget);
+    if (h == 0 && threadIdx.x == 0) e.new_lengths[b] = keep;
     int32_t* from = e.from + (int64_t)blockIdx.x * e.most;
     int32_t* to = e.to + (int64_t)blockIdx.x * e.most;
     int count = 0;
-    if (n <= e.budget) {  // everything is kept
-        if (e.into) {
-            count = n;
-            for (int j = threadIdx.x; j < n; j += kSelect) from[j] = to[j] = j;
+    // Of the first `keep` places those without a page stay empty, and as many fewer
+    // tokens are kept.  In place there are never fewer tokens than places, as those
+    // below the budget lie in them; for other pages there may be.
+    bool select = n > e.budget;
+    // How many of the first `tokens` of a row have no page; the thread's first page
+    // was read before.
+    const auto without_page = [&](const int32_t* r, int tokens, int page, int* sum) {
+        for (int k = threadIdx.x; k << e.page_shift < tokens; k += kSelect) {
+            if (k >= kSelect) page = r[k];
+            if ((uint32_t)page >= (uint32_t)e.c.pages)
+                atomicAdd(sum, min(e.c.page_size, tokens - (k << e.page_shift)));
         }
-    } else {
+    };
+    int to_page = 0;
+    if (select || e.into) {
+        hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
+        if (threadIdx.x == 0) absent = gaps = 0;
+        const bool mine = (int)threadIdx.x << e.page_shift < keep;
+        if (e.into && mine) to_page = other[threadIdx.x];
+        __syncthreads();
+        if (!select) {  // everything is kept, in its order, where every page is there
+            const int page = mine ? row[threadIdx.x] : 0;
+            without_page(other, keep, to_page, &gaps);
+            without_page(row, n, page, &absent);
+            __syncthreads();
+            select = absent | gaps;
+            __syncthreads();
+            if (threadIdx.x == 0) absent = gaps = 0;  // counted again with the keys
+            __syncthreads();
+            if (!select) {
+                count = n;
+                for (int j = threadIdx.x; j < n; j += kSelect) from[j] = to[j] = j;
+            }
+        }
+    }
+    if (select) {
         const int pieces = (n + kPiece - 1) / kPiece;
         // keys of a lane, in fours
         const int each = pieces > 1 ? kKeys : (n + 4 * kSelect - 1) / (4 * kSelect) * 4;
@@ -230,6 +272,14 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                     m[u] = *reinterpret_cast<const vec<float, 4>*>(e.c.mass + at);
                     p[u] = *reinterpret_cast<const vec<int, 4>*>(e.c.position + at);
                 }
+            if (count) {
+                const int stop = e.into ? limit : min(limit, keep);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int lost = min(e.c.page_size, stop - ((page0 + 64 * u + lane) << e.page_shift));
+                    if (page[u] < 0 && lost > 0) atomicAdd(&absent, lost);
+                }
+            }
             wave_order();  // other lanes have read the last piece's keys
 #pragma unroll
             for (int u = 0; u < kKeys / 4; u++)
@@ -255,11 +305,10 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             }
         };
         uint32_t above = 0;  // the digits found so far
-        int room = e.budget; // tokens to keep of those that share them
+        int room = 0;        // tokens to keep of those that share them
         int in_bin = 0;      // and how many do
-        hist[threadIdx.x] = hist[threadIdx.x + kSelect] = 0;
-        __syncthreads();
         if (pieces == 1) load(0, true);  // the first digit is counted on the way
+        if (e.into) without_page(other, keep, to_page, &gaps);
         for (int shift = 21, bits = 11;; shift = shift == 21 ? 10 : 0) {
             for (int piece = 0; piece < pieces; piece++) {
                 if (pieces > 1) load(piece, shift == 21);
@@ -270,6 +319,13 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
                     });
             }
             __syncthreads();
+            if (shift == 21) {
+                // tokens that there are, and places for them
+                room = e.into ? min(n - absent, keep - gaps) : keep - absent;
+                if (e.into && h == 0 && threadIdx.x == 0 && room < keep - gaps)
+                    e.new_lengths[b] = room ? nth_place(e, other, room - 1) + 1 : 0;
+                if (room == 0) break;
+            }
             // the bin that holds the room-th largest: a sum from the top over
             // the threads, two bins each
             const int low = hist[2 * threadIdx.x], high = hist[2 * threadIdx.x + 1];
@@ -298,9 +354,10 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
         // early those are all that there are, else they are equal to it.
         const bool all = room == in_bin;
         above = max(above, 1u);  // not what stands behind the last token
+        const bool holes = absent && !e.into;
         // Lane i of a wave decides about its i-th 64 tokens, all bits at once.
         uint32_t ties = 0, lists[2] = {0, 0};  // of the pieces so far
-        for (int piece = 0; piece < pieces; piece++) {
+        for (int piece = 0; room && piece < pieces; piece++) {
             if (pieces > 1) load(piece, false);
             uint64_t more = 0, same = 0;
             over_keys([&](int i, uint32_t r) {
@@ -315,7 +372,13 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             }
             const int start = first + 64 * lane;  // of the lane's 64 tokens
             const uint64_t kept = more | same, low = low_bits(e.budget - start);
-            const uint64_t listed[2] = {e.into ? kept : low_bits(limit - start) & low & ~kept,
+            uint64_t there = low_bits(limit - start);
+            if (holes)
+                over_keys([&](int i, uint32_t r) {
+                    const uint64_t x = __ballot(r > 1);
+                    if (lane == i) there &= x;
+                });
+            const uint64_t listed[2] = {e.into ? kept : there & low & ~kept,
                                         e.into ? 0 : kept & ~low};
             // at most 32768 of each in a piece: both sums in one word
             const uint32_t before = before_of(__popcll(listed[0]) | __popcll(listed[1]) << 16, waves, &sum);
@@ -342,6 +405,10 @@ __global__ void __launch_bounds__(kSelect) select_kernel(Evict e, bool moves_her
             }
         }
         count = lists[0];
+        if (gaps) {  // of the other pages: to the places that there are
+            __syncthreads();
+            for (int i = threadIdx.x; i < count; i += kSelect) to[i] = nth_place(e, other, i);
+        }
     }
     if (!moves_here) {
         if (threadIdx.x == 0) e.count[blockIdx.x] = count;

@@ -261,12 +261,14 @@ class PagedCache:
         """Cuts every sequence longer than budget to that many tokens, each kv
         head by itself: those with position >= seen - recent (seen: int32, the
         tokens that each sequence has seen so far) are kept first, then those of
-        the largest mass, ties to the lower index.  Returns the new lengths,
-        min(lengths, budget).  By default in place: tokens kept beyond the
-        budget move into the freed places below it, so the pages must belong to
-        one sequence alone; the pages beyond the new lengths are free.  into: a
-        table of other pages, which all kept tokens are copied to in order,
-        while the sequences' own pages stay as they are."""
+        the largest mass, ties to the lower index; tokens without a page are
+        never kept, and where places have none as many fewer tokens are.  Returns
+        the new lengths, min(lengths, budget).  By default in place: tokens kept
+        beyond the budget move into the freed places below it, so the pages must
+        belong to one sequence alone; the pages beyond the new lengths are free.
+        into: a table of other pages, which all kept tokens are copied to in
+        order, while the sequences' own pages stay as they are; a new length is
+        less where tokens without a page leave fewer."""
         if self.mass is None:
             raise ValueError("the cache was made without track")
         self._ints("table", table, torch.int32, (None, None))
