@@ -42,3 +42,20 @@ def test_evict_in_pieces(kv, length, budget_of):
             at[np.setdiff1d(at, kept)] = kept[kept >= budget]
             for x, y in zip((mass, position, k), got):
                 assert np.array_equal(y[h, :budget], x[h][at])
+
+
+def test_attend_in_a_compiled_program(kv):
+    """A compiled program breaks at the call and makes it; a traced one is
+    refused, as it would go on without the kernel."""
+    c = kv.PagedCache.allocate(8, 2, 64, 16, torch.bfloat16)
+    c.k.normal_()
+    c.v.normal_()
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    n = torch.tensor([50, 20], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 6, 64, device="cuda").bfloat16()
+    want = c.attend(q * 2, table, n) + 1
+    run = torch.compile(lambda q: c.attend(q * 2, table, n) + 1, backend="eager")
+    for _ in range(3):
+        assert torch.equal(run(q), want)
+    with pytest.raises(ValueError):
+        torch.jit.trace(lambda q: c.attend(q, table, n) + 1, (q,), check_trace=False)

@@ -62,3 +62,117 @@ def test_new_lengths_next_to_what_is_read(kv, lib):
 def test_evict_workspace_is_aligned(kv, lib):
     assert evict(kv, lib, work=0x150004) == EARG
     assert evict(kv, lib, work=0x150008) == EARG
+
+
+# ------------------------------------------------- calls that something watches
+class Counted:
+    """Stands for the library: counts the calls that would launch."""
+    _kv_bound = True
+
+    def __init__(self, answer=0):
+        self.calls, self.answer = 0, answer
+
+    def vramc_kv_attend_workspace(self, *args):
+        return 64
+
+    vramc_kv_evict_workspace = vramc_kv_attend_workspace
+
+    def launch(self, *args):
+        self.calls += 1
+        return self.answer
+
+    vramc_kv_append = vramc_kv_read = vramc_kv_attend = vramc_kv_evict = launch
+
+
+@pytest.fixture
+def host(kv, rans, monkeypatch):
+    """Caches of CPU tensors over a library that only counts."""
+    monkeypatch.setattr(rans, "_device", lambda: -1)
+    monkeypatch.setattr(rans, "_stream", lambda: 0)
+
+    def make(dtype=torch.float32, answer=0):
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "is_available", lambda: True)
+            m.setattr(torch.Tensor, "is_cuda", True)
+            return kv.PagedCache.allocate(8, 2, 64, 16, dtype, track=True, device="cpu", lib=Counted(answer))
+    return make
+
+
+def operations(c):
+    """Every operation as a function of one tensor of its arguments."""
+    table = torch.zeros(3, 2, dtype=torch.int32)
+    n = torch.full((3,), 20, dtype=torch.int32)
+    slots = torch.arange(3)
+    k = torch.zeros(3, 2, 64, dtype=c.dtype)
+    return {
+        "attend": (lambda q: c.attend(q, table, n), torch.zeros(3, 4, 64, dtype=c.dtype)),
+        "append k": (lambda x: c.append(x, k, slots, n), k),
+        "append v": (lambda x: c.append(k, x, slots, n), k.clone()),
+        "read": (lambda s: c.read(s), slots),
+        "evict": (lambda t: c.evict(t, n, n, 7), table),
+    }
+
+
+NAMES = ("attend", "append k", "append v", "read", "evict")
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tracers_are_refused(host, name):
+    """A traced call would leave a program without the kernel: uninitialised
+    memory in place of its output."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    c = host()
+    call, x = operations(c)[name]
+    call(x)
+    assert c.lib.calls == 1
+    for trace in (lambda: torch.jit.trace(lambda t: (call(t), t + 1)[1], (x,), check_trace=False),
+                  lambda: make_fx(lambda t: (call(t), t + 1)[1])(x)):
+        with pytest.raises(ValueError, match="watch"):
+            trace()
+    assert c.lib.calls == 1
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_modes_and_levels_are_refused(host, name):
+    """Forward mode would drop the tangent, vmap and function and dispatch modes
+    would not see the call; the mode of a default device watches nothing."""
+    from torch.autograd import forward_ad
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    c = host()
+    call, x = operations(c)[name]
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="watch"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)) if x.is_floating_point() else x)
+    with pytest.raises(ValueError, match="watch"):
+        torch.func.vmap(lambda t: (call(x), t)[1])(torch.zeros(2))
+    for mode in (Function, Dispatch):
+        with mode(), pytest.raises(ValueError, match="watch"):
+            call(x)
+    assert c.lib.calls == 0
+    with torch.device("cpu"), torch.no_grad():
+        call(x)
+    with torch.inference_mode():
+        call(x)
+    assert c.lib.calls == 2
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_under_the_compiler_calls_run_as_they_are(host, name):
+    """A compiled program breaks at a call and makes it."""
+    c = host()
+    call, x = operations(c)[name]
+    run = torch.compile(lambda t: (call(t + 0), t + 1)[1], backend="eager")
+    for i in range(1, 4):
+        assert torch.equal(run(x), x + 1)
+        assert c.lib.calls == i
+    torch._dynamo.reset()

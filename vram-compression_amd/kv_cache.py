@@ -15,14 +15,17 @@ PagedCache holds that cache:
 A sequence's tokens lie in the pages that its row of `table` names, in order;
 which pages are free is the program's to keep.  Every operation is a
 hand-written HIP kernel in librans_hip.so (include/vramc_kv.h), runs on the
-current stream and allocates from torch.  There is no CPU fallback, and no
-gradient: what is called under one is refused.
+current stream and allocates from torch.  There is no CPU fallback, and nothing
+that torch could watch: calls under a gradient, forward mode, vmap, a tracer, a
+dispatch or a function mode are refused (a compiled program breaks at a call
+and makes it).
 """
 import ctypes
 
 import torch
 
 import rans
+from rans_linear import _watched
 
 MX_BLOCK = 32  # columns that share a scale byte
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -149,6 +152,10 @@ class PagedCache:
     # ------------------------------------------------------------- arguments
     # The checks run on every token step: messages are made only for a failure.
     def _stream(self):
+        """The current stream, for a call that nothing watches."""
+        if _watched():
+            raise ValueError("forward mode, vmap, a tracer or a dispatch or function mode watches this "
+                             "call, and the cache's operations are hidden from them")
         if rans._device() != self._index:
             raise ValueError(f"the cache is on {self.device}, the current device is another")
         return rans._stream()
@@ -196,6 +203,7 @@ class PagedCache:
         head_dim) at any strides, into slots (int64; page * page_size + place,
         -1 for none).  positions (int32): the tokens' positions, for a tracked
         cache, whose mass starts at 0."""
+        stream = self._stream()
         k, v = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
         n = k.shape[0]
         if v.shape[0] != n:
@@ -209,14 +217,15 @@ class PagedCache:
             at = positions.data_ptr()
         rc = self.lib.vramc_kv_append(self._ref, k.data_ptr(), k.stride(0), k.stride(1),
                                       v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), at,
-                                      n, self._stream())
+                                      n, stream)
         assert rc == 0, f"HIP error {rc}"
 
     def read(self, slots):
         """The keys and values in slots (int64), (tokens, kv_heads, head_dim)
         of the cache's dtype; zeros for a slot outside the cache."""
+        stream = self._stream()
         self._ints("slots", slots, torch.int64, (None,))
-        n, stream = slots.shape[0], self._stream()
+        n = slots.shape[0]
         k = torch.empty((n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
         rc = self.lib.vramc_kv_read(self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), stream)
@@ -232,6 +241,7 @@ class PagedCache:
         summed over the query heads of its kv head, is added to mass; by default
         where the cache has it.  The table's width bounds the lengths: one cut
         to the pages in use (table[:, :n]) spares what longer ones would need."""
+        stream = self._stream()
         q = self._rows("q", q, None)
         batch, heads, _ = q.shape
         if heads <= 0 or heads % self.kv_heads:
@@ -242,7 +252,7 @@ class PagedCache:
             track = self.mass is not None
         elif track and self.mass is None:
             raise ValueError("the cache was made without track")
-        stream, width = self._stream(), table.shape[1]
+        width = table.shape[1]
         out = torch.empty_like(q) if q.is_contiguous() else \
             torch.empty((batch, heads, self.head_dim), dtype=self.dtype, device=self.device)
         need = self.lib.vramc_kv_attend_workspace(self._ref, heads, width, batch, track)
@@ -271,6 +281,7 @@ class PagedCache:
         less where tokens without a page leave fewer."""
         if self.mass is None:
             raise ValueError("the cache was made without track")
+        stream = self._stream()
         self._ints("table", table, torch.int32, (None, None))
         batch, width = table.shape
         self._ints("lengths", lengths, torch.int32, (batch,))
@@ -285,7 +296,6 @@ class PagedCache:
             other, row, wide = into.data_ptr(), into.stride(0), into.shape[1]
             if wide * self.page_size < min(budget, width * self.page_size):
                 raise ValueError(f"into has no room for {budget} tokens")
-        stream = self._stream()
         need = self.lib.vramc_kv_evict_workspace(self._ref, width, batch, budget, into is not None)
         if need < 0:
             raise ValueError(f"{batch} sequences over {width} pages: too many ({need})")

@@ -72,16 +72,22 @@ def _function_mode(n):
     return any(type(torch._C._get_function_stack_at(i)) is not DeviceContext for i in range(n))
 
 
+def _watched():
+    """Whether a forward-mode level, vmap, a tracer, a dispatch or a function mode
+    is on that an operation outside torch would be hidden from."""
+    if (forward_ad._current_level >= 0 or _peek_functorch() is not None
+            or torch._C._get_tracing_state() is not None
+            or torch._C._len_torch_dispatch_stack() > 0):
+        return True
+    modes = torch._C._len_torch_function_stack()
+    return modes > 0 and _function_mode(modes)
+
+
 def _plain(*tensors):
     """Whether the tensors (or None) are ordinary ones of the current GPU that
     nothing else watches: no gradient, forward-mode, vmap, tracing, dispatch or
     function mode that an operation outside torch would be hidden from."""
-    if (torch.compiler.is_compiling() or forward_ad._current_level >= 0
-            or _peek_functorch() is not None or torch._C._get_tracing_state() is not None
-            or torch._C._len_torch_dispatch_stack() > 0):
-        return False
-    modes = torch._C._len_torch_function_stack()
-    if modes and _function_mode(modes):
+    if torch.compiler.is_compiling() or _watched():
         return False
     device = rans._device()
     for t in tensors:
