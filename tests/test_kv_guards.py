@@ -176,3 +176,21 @@ def test_under_the_compiler_calls_run_as_they_are(host, name):
         assert torch.equal(run(x), x + 1)
         assert c.lib.calls == i
     torch._dynamo.reset()
+
+
+@pytest.mark.parametrize("which", ["k", "v", "mass"])
+@pytest.mark.parametrize("name", NAMES)
+def test_a_cache_that_requires_a_gradient_is_refused(host, name, which):
+    """Its output would have no gradient for what it was computed from, and its
+    writes pass autograd by; without gradients it is a cache like any other."""
+    c = host()
+    call, x = operations(c)[name]
+    getattr(c, which).requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        call(x)
+    assert c.lib.calls == 0
+    with torch.no_grad():
+        call(x)
+    getattr(c, which).requires_grad_(False)
+    call(x)
+    assert c.lib.calls == 2

@@ -156,6 +156,10 @@ class PagedCache:
         if _watched():
             raise ValueError("forward mode, vmap, a tracer or a dispatch or function mode watches this "
                              "call, and the cache's operations are hidden from them")
+        if torch.is_grad_enabled() and (self.k.requires_grad or self.v.requires_grad or (
+                self.mass is not None and self.mass.requires_grad)):
+            raise ValueError("the cache's tensors require a gradient, and its operations have none: "
+                             "detach them or use torch.no_grad()")
         if rans._device() != self._index:
             raise ValueError(f"the cache is on {self.device}, the current device is another")
         return rans._stream()
