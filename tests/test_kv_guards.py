@@ -194,3 +194,15 @@ def test_a_cache_that_requires_a_gradient_is_refused(host, name, which):
     getattr(c, which).requires_grad_(False)
     call(x)
     assert c.lib.calls == 2
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_what_the_library_answers_is_raised(host, name):
+    """A refusal of the library is a ValueError, an error of HIP a RuntimeError,
+    neither an assertion that optimised Python leaves out."""
+    call, x = operations(host(answer=EARG))[name]
+    with pytest.raises(ValueError, match=str(EARG)):
+        call(x)
+    call, x = operations(host(answer=2))[name]
+    with pytest.raises(RuntimeError, match="HIP error 2"):
+        call(x)

@@ -75,6 +75,14 @@ def _check(ok, message):
         raise ValueError(message)
 
 
+def _failed(name, rc):
+    """Raises what a return value of the library says."""
+    if rc < 0:
+        raise ValueError(f"{name}: refused by the library ({rc}): more than one launch holds, or a tensor "
+                         "less aligned than the kernels read")
+    raise RuntimeError(f"{name}: HIP error {rc}")
+
+
 class PagedCache:
     """Keys and values of past tokens in pages on the GPU.
 
@@ -222,7 +230,8 @@ class PagedCache:
         rc = self.lib.vramc_kv_append(self._ref, k.data_ptr(), k.stride(0), k.stride(1),
                                       v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), at,
                                       n, stream)
-        assert rc == 0, f"HIP error {rc}"
+        if rc:
+            _failed("append", rc)
 
     def read(self, slots):
         """The keys and values in slots (int64), (tokens, kv_heads, head_dim)
@@ -233,7 +242,8 @@ class PagedCache:
         k = torch.empty((n, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
         rc = self.lib.vramc_kv_read(self._ref, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), stream)
-        assert rc == 0, f"HIP error {rc}"
+        if rc:
+            _failed("read", rc)
         return k, v
 
     def attend(self, q, table, lengths, scale=None, track=None):
@@ -268,7 +278,8 @@ class PagedCache:
             table.stride(0), width, lengths.data_ptr(), batch,
             self.head_dim ** -0.5 if scale is None else scale, track, out.data_ptr(),
             work.data_ptr(), need, stream)
-        assert rc == 0, f"HIP error {rc}"
+        if rc:
+            _failed("attend", rc)
         return out
 
     def evict(self, table, lengths, seen, budget, recent=0, into=None):
@@ -309,5 +320,6 @@ class PagedCache:
             self._ref, table.data_ptr(), table.stride(0), width, lengths.data_ptr(),
             seen.data_ptr(), batch, budget, recent, other, row, wide, out.data_ptr(),
             work.data_ptr(), need, stream)
-        assert rc == 0, f"HIP error {rc}"
+        if rc:
+            _failed("evict", rc)
         return out
