@@ -59,3 +59,37 @@ def test_attend_in_a_compiled_program(kv):
         assert torch.equal(run(q), want)
     with pytest.raises(ValueError):
         torch.jit.trace(lambda q: c.attend(q, table, n) + 1, (q,), check_trace=False)
+
+
+@pytest.mark.parametrize("dtype,mx,dim", [(torch.float32, False, 64), (torch.float32, False, 96),
+                                          (torch.bfloat16, False, 192), (torch.float16, True, 96),
+                                          (torch.bfloat16, True, 256)])
+def test_caches_aligned_to_16_bytes_only(kv, dtype, mx, dim):
+    """What a cache's tensors have to be aligned to, and no more: every operation
+    gives what it gives on tensors of their own."""
+    heads, page, pages = 2, 16, 9
+
+    def off(shape, dt):  # 16 bytes behind an address of 512
+        n = int(np.prod(shape)) * dt.itemsize
+        t = torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[16:]
+        assert t.data_ptr() % 32 == 16
+        return t.view(dt).view(shape)
+
+    a = kv.PagedCache.allocate(pages, heads, dim, page, dtype, mx=mx, track=True)
+    names = [w for w in ("k", "v", "k_scale", "v_scale", "mass", "position") if getattr(a, w) is not None]
+    b = kv.PagedCache(**{w: off(tuple(getattr(a, w).shape), getattr(a, w).dtype) for w in names}, dtype=dtype)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    k, v = (torch.randn(100, heads, dim, device="cuda", generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(2, 6, dim, device="cuda", generator=g).to(dtype)
+    slots = torch.randperm(pages * page, device="cuda", generator=g)[:100]
+    at = torch.arange(100, dtype=torch.int32, device="cuda")
+    order = torch.randperm(pages, device="cuda", generator=g).int()
+    table, into = order[:8].view(2, 4), order[8:].view(1, 1)
+    n = torch.tensor([60, 33], dtype=torch.int32, device="cuda")
+    got = []
+    for c in (a, b):
+        c.append(k, v, slots, at)
+        got.append([*c.read(slots), c.attend(q, table, n), c.evict(table[:1], n[:1], n[:1], 9, 3, into),
+                    c.evict(table, n, n, 30, 7)] + [getattr(c, w) for w in names])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)

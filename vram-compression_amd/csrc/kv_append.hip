@@ -21,6 +21,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPer = 8;  // values of a thread
 
+// Eight values where they lie in a cache, whose tensors are aligned to 16 bytes: as
+// one vector, eight floats would promise 32.
+template <typename T>
+struct Lying {
+    vec<uint32_t, 4> part[kPer * sizeof(T) / 16];
+};
+
 // The largest magnitude of eight values, as the bits of a float: magnitudes of a
 // float format sort as their bits do, infinity and NaN above all.
 template <typename T>
@@ -74,7 +81,10 @@ template <typename T, bool MX>
 __device__ __forceinline__ void store(vec<T, kPer> x, void* held, uint8_t* scales, int64_t at, int per_row,
                                       int seg) {
     if constexpr (!MX) {
-        __builtin_nontemporal_store(x, reinterpret_cast<vec<T, kPer>*>(static_cast<T*>(held)) + at * per_row + seg);
+        const auto from = __builtin_bit_cast(Lying<T>, x);
+        auto* to = static_cast<Lying<T>*>(held) + at * per_row + seg;
+#pragma unroll
+        for (size_t i = 0; i < sizeof(T) / 2; i++) __builtin_nontemporal_store(from.part[i], &to->part[i]);
     } else {
         // a block's threads are four neighbours of a wave
         uint32_t most = largest(x);
@@ -97,7 +107,7 @@ struct Held {
     __device__ __forceinline__ void load(const void* held, const uint8_t* scales, int64_t at, int per_row,
                                          int seg) {
         if constexpr (!MX) {
-            x = *reinterpret_cast<const vec<T, kPer>*>(static_cast<const T*>(held) + (at * per_row + seg) * kPer);
+            x = __builtin_bit_cast(vec<T, kPer>, static_cast<const Lying<T>*>(held)[at * per_row + seg]);
         } else {
             codes = static_cast<const uint32_t*>(held)[at * per_row + seg];
             scale = scales[at * (per_row / 4) + seg / 4];
