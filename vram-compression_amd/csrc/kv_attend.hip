@@ -136,13 +136,15 @@ __device__ __forceinline__ global_ptr shared_address(const void* p, int64_t off)
     return (global_ptr)at;
 }
 
-// BYTES bytes of memory in registers, from an address aligned to 4 or to BYTES.
+// BYTES bytes of memory in registers, from an address aligned to the largest power of
+// two that divides BYTES, or to 16.
 template <int BYTES>
 struct Raw {
     uint32_t w[BYTES < 4 ? 1 : BYTES / 4];
 };
-template <int N>
-using words = uint32_t __attribute__((ext_vector_type(N), aligned(4)));
+// Three words have no more alignment than one (as an alias of a template the
+// attribute would be dropped, and 16 bytes promised).
+typedef uint32_t three_words __attribute__((ext_vector_type(3), aligned(4)));
 template <int BYTES>
 __device__ __forceinline__ Raw<BYTES> load_raw(global_ptr p) {
     Raw<BYTES> r;
@@ -154,11 +156,15 @@ __device__ __forceinline__ Raw<BYTES> load_raw(global_ptr p) {
         r.w[0] = *reinterpret_cast<const __attribute__((address_space(1))) uint16_t*>(p);
     } else if constexpr (BYTES == 4) {
         r.w[0] = *reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(p);
+    } else if constexpr (BYTES == 12) {
+        const auto x = *reinterpret_cast<const __attribute__((address_space(1))) three_words*>(p);
+#pragma unroll
+        for (int j = 0; j < 3; j++) r.w[j] = x[j];
     } else {
-        constexpr int N = BYTES / 4 <= 4 ? BYTES / 4 : BYTES % 16 == 0 ? 4 : 2;  // words of a load
+        constexpr int N = BYTES % 16 == 0 ? 4 : 2;  // words of a load
 #pragma unroll
         for (int i = 0; i < BYTES / 4; i += N) {
-            const auto x = *reinterpret_cast<const __attribute__((address_space(1))) words<N>*>(p + 4 * i);
+            const auto x = *reinterpret_cast<const __attribute__((address_space(1))) vec<uint32_t, N>*>(p + 4 * i);
 #pragma unroll
             for (int j = 0; j < N; j++) r.w[i + j] = x[j];
         }
