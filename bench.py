@@ -55,20 +55,21 @@ DEFAULT_TILING = (3, 1792, 1)
 # is scaled by what it reads for an elementwise kernel that reads and writes
 # 256 MiB: reads x2.0, writes x1.0.  Commands and counts:
 # profiles/rans_w64_gemv_1536x8960_3.25b.md.  Keyed by (R, C, S, word fetch)
-# and by the hash of the library sources they were measured on
-# (library_source_hash): with other sources the line reports traffic null.
-PMC_TRAFFIC_KIB = {(3, 1792, 1, "refill"): dict(source_hash="861bba18cbfa", commit="c2970d4",
+# and by the hash of the library sources that the kernel and its streams are
+# built from (gemv_source_hash): with other ones the line reports traffic null.
+PMC_TRAFFIC_KIB = {(3, 1792, 1, "refill"): dict(source_hash="f957635d3232", commit="c2970d4",
                                                 fetch_kib=3444.1, write_kib=12.0)}
 PMC_FETCH_FACTOR, PMC_WRITE_FACTOR = 2.0, 1.0
 
 
 library_source_hash = B.library_source_hash
+gemv_source_hash = B.gemv_source_hash
 
 
 def pmc_traffic(R, C, S, word_fetch, src_hash):
     """(HBM bytes per launch, note) of the headline kernel for this tiling
     and word fetch from the rocprofv3 counters, or (None, why) when no
-    counter figure exists or it was measured on other library sources."""
+    counter figure exists or it was measured on other sources of the kernel (src_hash)."""
     pmc = PMC_TRAFFIC_KIB.get((R, C, S, word_fetch))
     if pmc is None:
         return None, "no counter figure for this tiling"
@@ -346,6 +347,7 @@ def main():
         print(json.dumps({"profile": True, "R": R, "C": C, "S": S, "flags": flags,
                           "launches": args.warmup + args.steps, "profiled_launches": args.steps,
                           "library_source_hash": library_source_hash(),
+                          "gemv_source_hash": gemv_source_hash(),
                           "copies": ncopy, "algorithmic_bytes_per_launch": alg,
                           "compressed_bytes": comp, "calibration_copy_bytes": 256 << 20}), flush=True)
         return
@@ -524,7 +526,7 @@ def main():
     achieved = alg / (t_rot * 1e-6) / 1e9
     fetch_name = {rans.F_WORDS_ALWAYS: "always", rans.F_WORDS_REFILL: "refill"}.get(measure.flags & 3)
     src_hash = library_source_hash()
-    traffic, traffic_note = pmc_traffic(R, C, S, fetch_name, src_hash)
+    traffic, traffic_note = pmc_traffic(R, C, S, fetch_name, gemv_source_hash())
     out = {
         "metric": METRIC,
         "value": ROWS * COLS * 2 / t_rot / 1e3,

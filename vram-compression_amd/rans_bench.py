@@ -315,15 +315,30 @@ def test():
     print("ok  int4 baseline")
 
 
+def _source_hash(paths):
+    h = hashlib.sha256()
+    for path in paths:
+        with open(path, "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()[:12]
+
+
 def library_source_hash():
     """First 12 hex digits of the SHA-256 of the library's sources and
     header (rans.SOURCES, rans.HEADERS, in that order): names the build a
     measurement belongs to."""
-    h = hashlib.sha256()
-    for path in rans.SOURCES + rans.HEADERS:
-        with open(path, "rb") as f:
-            h.update(f.read())
-    return h.hexdigest()[:12]
+    return _source_hash(rans.SOURCES + rans.HEADERS)
+
+
+# What the GEMV kernels and the streams that they read are built from.
+GEMV_SOURCES = [os.path.join(rans.CSRC, f) for f in ("rans_gemv.hip", "rans_device.h", "w64_host.cpp")] + [
+    os.path.join(rans.INCLUDE, "vramc_rans.h")]
+
+
+def gemv_source_hash():
+    """The same over GEMV_SOURCES: names what a measurement of the GEMV belongs
+    to, whatever else the library holds."""
+    return _source_hash(GEMV_SOURCES)
 
 
 BENCH_FILE = "kernel_bench_mi355x.json"
