@@ -93,3 +93,30 @@ def test_caches_aligned_to_16_bytes_only(kv, dtype, mx, dim):
                     c.evict(table, n, n, 30, 7)] + [getattr(c, w) for w in names])
     for x, y in zip(*got):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dim,heads", [(96, 8), (192, 4), (256, 4)])
+def test_attend_in_f32_is_as_exact_as_f32(kv, dim, heads):
+    """The error against 64 bits, in the 2-norm, is at most half again that of
+    elementary f32 operations on the same numbers."""
+    for seed in range(4):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        c = kv.PagedCache.allocate(3 * 56, heads, dim, 32, torch.float32)
+        c.k.normal_(generator=g)
+        c.v.normal_(generator=g)
+        table = torch.randperm(3 * 56, device="cuda", generator=g).int().view(3, 56)
+        n = torch.tensor([1777, 1500, 900], dtype=torch.int32, device="cuda")
+        q = 2 * torch.randn(3, heads, dim, device="cuda", generator=g)
+        got = c.attend(q, table, n).double()
+        far = torch.zeros(2, dtype=torch.float64, device="cuda")
+        for b in range(3):
+            k, v = (x[table[b].long()].transpose(0, 1).flatten(1, 2)[:, :int(n[b])] for x in (c.k, c.v))
+
+            def plain(t):
+                w = torch.softmax((q[b].to(t)[:, None] @ k.to(t).transpose(1, 2).contiguous()) * dim ** -0.5, -1)
+                return (w @ v.to(t))[:, 0].double()
+
+            want = plain(torch.float64)
+            far += torch.stack([(got[b] - want).square().sum(), (plain(torch.float32) - want).square().sum()])
+        own, elementary = far.sqrt().tolist()
+        assert own <= 1.5 * elementary, (seed, own / elementary)
