@@ -206,3 +206,14 @@ def test_what_the_library_answers_is_raised(host, name):
     call, x = operations(host(answer=2))[name]
     with pytest.raises(RuntimeError, match="HIP error 2"):
         call(x)
+
+
+@pytest.mark.parametrize("which", ["k", "v", "k_scale", "v_scale", "mass", "position"])
+def test_the_tensors_of_a_cache_stay_its_own(host, which):
+    """The kernels write where the tensors lay when the cache was made: another
+    tensor in the place of one would leave them writing to freed memory."""
+    c = host()
+    held = getattr(c, which)
+    with pytest.raises(AttributeError):
+        setattr(c, which, torch.zeros(1) if held is None else torch.zeros_like(held))
+    assert getattr(c, which) is held

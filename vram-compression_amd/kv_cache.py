@@ -91,7 +91,16 @@ class PagedCache:
     scale byte for every 32 columns, uint8 (.., head_dim / 32) (bf16 or f16
     values; the MXFP4 format, 4.25 bits a value).  mass (f32) and position
     (int32), (pages, kv_heads, page_size), where tokens' accumulated weights are
-    tracked.  The tensors are used as they are, not copied."""
+    tracked.  The tensors are used as they are, not copied, and a cache keeps those
+    that it was made of."""
+
+    # The descriptor holds their addresses: not to be assigned.
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+    mass = property(lambda self: self._mass)
+    position = property(lambda self: self._position)
 
     def __init__(self, k, v, dtype=torch.bfloat16, k_scale=None, v_scale=None, mass=None,
                  position=None, lib=None):
@@ -124,8 +133,8 @@ class PagedCache:
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
             if t.data_ptr() % 16 and not name.endswith("scale"):
                 raise ValueError(f"{name} must be 16-byte aligned")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.mass, self.position, self.dtype, self.device = mass, position, dtype, k.device
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._mass, self._position, self.dtype, self.device = mass, position, dtype, k.device
         self._index = k.get_device()
         self.lib = bind(lib or rans._host_lib())
         ptr = {n: t.data_ptr() for n, t, _, _ in want}
@@ -164,8 +173,8 @@ class PagedCache:
         if _watched():
             raise ValueError("forward mode, vmap, a tracer or a dispatch or function mode watches this "
                              "call, and the cache's operations are hidden from them")
-        if torch.is_grad_enabled() and (self.k.requires_grad or self.v.requires_grad or (
-                self.mass is not None and self.mass.requires_grad)):
+        if torch.is_grad_enabled() and (self._k.requires_grad or self._v.requires_grad or (
+                self._mass is not None and self._mass.requires_grad)):
             raise ValueError("the cache's tensors require a gradient, and its operations have none: "
                              "detach them or use torch.no_grad()")
         if rans._device() != self._index:
@@ -222,7 +231,7 @@ class PagedCache:
             raise ValueError(f"{n} keys and {v.shape[0]} values")
         self._ints("slots", slots, torch.int64, (n,))
         at = None
-        if self.mass is not None:
+        if self._mass is not None:
             if positions is None:
                 raise ValueError("a tracked cache needs the tokens' positions")
             self._ints("positions", positions, torch.int32, (n,))
@@ -263,8 +272,8 @@ class PagedCache:
         self._ints("table", table, torch.int32, (batch, None))
         self._ints("lengths", lengths, torch.int32, (batch,))
         if track is None:
-            track = self.mass is not None
-        elif track and self.mass is None:
+            track = self._mass is not None
+        elif track and self._mass is None:
             raise ValueError("the cache was made without track")
         width = table.shape[1]
         out = torch.empty_like(q) if q.is_contiguous() else \
@@ -294,7 +303,7 @@ class PagedCache:
         into: a table of other pages, which all kept tokens are copied to in
         order, while the sequences' own pages stay as they are; a new length is
         less where tokens without a page leave fewer."""
-        if self.mass is None:
+        if self._mass is None:
             raise ValueError("the cache was made without track")
         stream = self._stream()
         self._ints("table", table, torch.int32, (None, None))
