@@ -65,6 +65,8 @@ def quantize_uniform(weight, bits, iters=40, sample=1 << 22, seed=0):
 _DTYPES = rans._X_CODES
 _peek_functorch = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack",
                           lambda: None)
+_tracing, _function_modes = torch._C._get_tracing_state, torch._C._len_torch_function_stack
+_dispatch_modes = torch._C._len_torch_dispatch_stack
 
 
 def _function_mode(n):
@@ -75,11 +77,10 @@ def _function_mode(n):
 def _watched():
     """Whether a forward-mode level, vmap, a tracer, a dispatch or a function mode
     is on that an operation outside torch would be hidden from."""
-    if (forward_ad._current_level >= 0 or _peek_functorch() is not None
-            or torch._C._get_tracing_state() is not None
-            or torch._C._len_torch_dispatch_stack() > 0):
+    if (forward_ad._current_level >= 0 or _peek_functorch() is not None or _tracing() is not None
+            or _dispatch_modes() > 0):
         return True
-    modes = torch._C._len_torch_function_stack()
+    modes = _function_modes()
     return modes > 0 and _function_mode(modes)
 
 
