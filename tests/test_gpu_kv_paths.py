@@ -120,3 +120,97 @@ def test_attend_in_f32_is_as_exact_as_f32(kv, dim, heads):
             far += torch.stack([(got[b] - want).square().sum(), (plain(torch.float32) - want).square().sum()])
         own, elementary = far.sqrt().tolist()
         assert own <= 1.5 * elementary, (seed, own / elementary)
+
+
+@pytest.mark.parametrize("dtype,mx,group,track", [("bf16", False, 3, True), ("bf16", True, 5, False),
+                                                  ("f16", True, 1, True), ("f32", False, 2, False),
+                                                  ("f16", False, 18, True)])
+def test_attend_more_sequences_than_threads(kv, dtype, mx, group, track):
+    """600 and 1100 sequences, empty ones among them and at both ends: a thread
+    of a workgroup counts several, and a share begins in any of them."""
+    import test_gpu_kv_cache as T
+    for batch in (600, 1100):
+        rng = np.random.default_rng(batch)
+        lengths = [0 if i < 3 or i > batch - 5 or rng.random() < 0.3 else int(rng.integers(1, 150)) for i in range(batch)]
+        lengths[batch // 2] = 2500
+        pages = sum(-(-n // 16) for n in lengths)
+        c = T.make(kv, dtype, mx, 64, 16, 2, pages, seed=batch, track=track)
+        table, n = T.tables(lengths, 16, pages, seed=batch)
+        q = torch.randn(batch, 2 * group, 64, device="cuda").to(T.DTYPES[dtype])
+        got = T.check_attend(kv, c, dtype, q, table, n)
+        assert torch.equal(c.attend(q, table, n), got)
+
+
+@pytest.mark.parametrize("dtype,mx", [("bf16", False), ("f16", False), ("f32", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("dim,group", [(64, 2), (96, 2), (192, 2), (256, 2), (64, 24), (96, 24), (128, 24),
+                                       (192, 32), (256, 40)])
+def test_attend_joins_many_parts(kv, dtype, mx, dim, group):
+    """One sequence for many workgroups: every width's join, of 16 heads and of 32."""
+    import test_gpu_kv_cache as T
+    c = T.make(kv, dtype, mx, dim, 32, 1, 110, seed=dim + group)
+    table, n = T.tables([3500], 32, 110, seed=group)
+    q = torch.randn(1, group, dim, device="cuda").to(T.DTYPES[dtype])
+    T.check_attend(kv, c, dtype, q, table, n)
+
+
+def test_4_bit_rounding_of_f16_at_its_edges(kv):
+    """Ties, powers of two, saturation, subnormals, zeros and blocks that are not
+    finite, for every exponent of f16."""
+    import test_gpu_kv_cache as T
+    base = np.array([0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7, 7.5, 7.9921875, 0.5, 1, 1.5, 2, 3, 4, 0.2490234375,
+                     0.251, 0.749, 0.751, 2.49, 2.51, 4.99, 5.01, 0.1, 0.01, 1e-3, 1e-5, 0, 0], np.float64)
+    rows = [np.concatenate([base, -base[::-1]]) * 2.0 ** e for e in range(-26, 14)]
+    rows += [np.concatenate([base / 2, np.full(32, 65504.0)]), np.full(64, 2.0 ** -24), np.full(64, -0.0)]
+    x = torch.tensor(np.array(rows)).clamp(-65504, 65504).half()
+    x[4, 3], x[6, 40], x[8, 0] = np.inf, np.nan, -np.inf
+    tokens = len(rows)
+    c = kv.PagedCache.allocate(-(-tokens // 16), 1, 64, 16, torch.float16, mx=True)
+    x = x.cuda()[:, None]
+    slots = torch.arange(tokens, device="cuda")
+    c.append(x, x.flip(2), slots)
+    k, v = c.read(slots)
+    want = T.rounded(x.double().cpu().numpy())
+    assert np.array_equal(T.opened(c, "k").transpose(0, 2, 1, 3).reshape(-1, 64)[:tokens], want[:, 0], equal_nan=True)
+    want = torch.from_numpy(want).half().double().numpy()  # below f16's smallest step
+    assert np.array_equal(k.double().cpu().numpy(), want, equal_nan=True)
+    assert np.array_equal(v.flip(2).double().cpu().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+def test_4_bit_blocks_that_are_nan_in_live_tokens(kv, dtype, dim):
+    """A NaN block of keys spoils the outputs of its kv head and sequence, one of
+    values its 32 columns there, and neither anything else."""
+    import test_gpu_kv_cache as T
+    c = T.make(kv, dtype, True, dim, 16, 2, 24, seed=dim)
+    table, n = T.tables([150, 200], 16, 24, seed=dim)
+    q = torch.randn(2, 6, dim, device="cuda").to(T.DTYPES[dtype])
+    mass = c.mass.clone()
+    want = c.attend(q, table, n)
+    after = c.mass.clone()
+    last = dim // 32 - 1
+    c.v_scale[table[0, 3], 0, 5, last] = 255
+    c.v_scale[table[1, 7], 1, 2, 0] = 255
+    c.mass.copy_(mass)
+    got = c.attend(q, table, n)
+    spoiled = torch.zeros_like(got, dtype=torch.bool)
+    spoiled[0, :3, 32 * last:] = spoiled[1, 3:, :32] = True
+    assert torch.isnan(got[spoiled]).all() and torch.equal(got[~spoiled], want[~spoiled])
+    assert torch.equal(c.mass, after)
+    c.v_scale.clamp_(max=129)
+    c.k_scale[table[0, 0], 1, 0, last] = 255
+    c.mass.copy_(mass)
+    got = c.attend(q, table, n)
+    spoiled.zero_()
+    spoiled[0, 3:] = True
+    # what the new block's scale of 129 in place of the old one changes is in no other row
+    same = torch.ones_like(spoiled)
+    same[0] = same[1, 3:] = False
+    assert torch.isnan(got[spoiled]).all() and torch.isfinite(got[~spoiled]).all()
+    assert torch.equal(got[same], want[same])
+    theirs = torch.zeros_like(c.mass, dtype=torch.bool)
+    theirs[table[0, :10].long(), 1] = True
+    assert torch.equal(c.mass[~theirs], after[~theirs])
+    place = torch.arange(160, device="cuda").view(10, 16) < 150
+    assert torch.isnan(c.mass[table[0, :10].long(), 1][place]).all()
+    assert torch.equal(c.mass[table[0, :10].long(), 1][~place], mass[table[0, :10].long(), 1][~place])
