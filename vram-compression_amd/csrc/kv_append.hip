@@ -1,9 +1,10 @@
 // New tokens' keys and values into the pages of a cache, and back.
 //
 // Both are passes over their bytes, and HBM bounds them: 32768 tokens of 8 heads
-// of 128 columns into 4-bit pages 38.9 us (4.5 TB/s; a large copy reaches 5.0),
-// back 26.0 us (6.6 TB/s, mostly writes), in bf16 53.2 and 42.4 us (5.0 and 6.3
-// TB/s); one token of each of 16 sequences 3.0 and 2.7 us.
+// of 128 columns into 4-bit pages 37.8 us (4.6 TB/s; a large copy reaches 5.0), in
+// bf16 53.9 us (5.0 TB/s).  Back, behind such an append, whose bytes fill the
+// caches, 32.0 us (5.3 TB/s, mostly writes) and 45.6 us (5.9 TB/s), and 25.5 and
+// 42.4 us again and again.  One token of each of 16 sequences 2.5 and 2.0 us.
 //
 // One thread takes eight values of a token's head, 16 bytes of a 16-bit type; a
 // workgroup takes neighbouring tokens of one head, whose rows lie behind each
@@ -173,8 +174,9 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t to = (r.token * c.kv_heads + r.head) * per_row + seg;
     auto *kp = reinterpret_cast<vec<T, kPer>*>(k) + to, *vp = reinterpret_cast<vec<T, kPer>*>(v) + to;
     // From 4-bit pages nearly all traffic is these stores: past the caches, 32768
-    // tokens of 8 heads of 128 columns take 26.0 us against 31.4.  Where as much is
-    // read as written it is the other way round (48.9 us against 42.4).
+    // tokens of 8 heads of 128 columns, again and again, take 26.0 us against 31.4.
+    // Where as much is read as written it is the other way round (48.9 us against
+    // 42.4).
     if constexpr (MX) {
         __builtin_nontemporal_store(x, kp);
         __builtin_nontemporal_store(y, vp);

@@ -36,9 +36,9 @@
 //
 // Measured: 16 sequences of up to 32768 tokens, 40 query heads over 8 of 128
 // columns: 269 us in bf16 (1.61 GB, 6.0 TB/s; VALU 10% busy, matrix cores 6%), 85
-// us from 4 bits (0.43 GB, 5.0 TB/s; 51% and 21%), and 5 us to join.  Short calls
-// are latency: one sequence of 32768 tokens over 2 heads 10.9 and 4.0 us, of 5
-// tokens 5.5 and 1.9.
+// us from 4 bits (0.43 GB, 5.0 TB/s; 50% and 21%), and 5 us to join.  A kernel that
+// only reads reaches 5.9 to 6.1 TB/s over 2 to 4 GiB.  Short calls are latency: one
+// sequence of 32768 tokens over 2 heads 11.5 and 4.0 us, of 5 tokens 5.5 and 2.1.
 #include "kv_device.h"
 
 namespace {
@@ -46,7 +46,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kUnit = 128;        // keys that work is dealt in: a step of every wave
-constexpr int kCus = 256;
+constexpr int kCus = 256;         // of an MI355X that is not partitioned
 constexpr float kLog2e = 1.4426950408889634f;
 
 // The reference is set this far below the largest score so far, and again when
@@ -66,7 +66,6 @@ struct Attend {
     int q_heads, group;
     const int32_t* table;
     int64_t table_row;
-    int table_width;
     const int32_t* lengths;
     int batch;
     float scale;
@@ -310,11 +309,12 @@ struct Values {
 };
 
 // Tiles of query heads that a wave takes at once: two where a kv head has more
-// than 16 and the registers hold their queries and sums beside the keys, so that
-// up to 32 heads read the cache once (16 sequences of up to 16384 tokens, 32
-// heads of 128 columns: 36 us against 42; 24 of 64 in f32 54 against 71).  4-bit
-// pages are cheap to read and dear to convert with fewer waves at it: one tile
-// (24 heads of 128 columns 35 us against 41).
+// than 16 and the registers hold their queries and sums beside the keys (all but
+// two registers of them, for 128 columns of 16 bits), so that up to 32 heads read
+// the cache once (16 sequences of up to 16384 tokens, 32 heads of 128 columns: 36
+// us against 42; 24 of 64 in f32 54 against 71).  4-bit pages are cheap to read and
+// dear to convert with fewer waves at it: one tile (24 heads of 128 columns 35 us
+// against 41).
 constexpr int pair_of(int size, bool mx, int dim, int group) {
     return group > 16 && !mx && size * dim <= (size == 4 ? 512 : 384) ? 2 : 1;
 }
@@ -960,8 +960,8 @@ extern "C" int vramc_kv_attend(const vramc_kv_cache* c, const void* q, int64_t q
     };
     const int64_t size = c->dtype == RANS_X_F32 ? 4 : 2;
     const bool wide = ((uintptr_t)q | (uintptr_t)(q_seq * size) | (uintptr_t)(q_head * size)) % 16 == 0;
-    Attend a{*c, q, q_seq, q_head, wide, q_heads, q_heads / c->kv_heads, table, table_row, table_width,
-             lengths, batch, scale, out, p.tile, (int)(p.groups / c->kv_heads), (int)p.groups,
+    Attend a{*c, q, q_seq, q_head, wide, q_heads, q_heads / c->kv_heads, table, table_row, lengths, batch,
+             scale, out, p.tile, (int)(p.groups / c->kv_heads), (int)p.groups,
              __builtin_ctz(c->page_size), table_width * c->page_size, nullptr, nullptr, nullptr, nullptr, nullptr};
     a.parts = static_cast<float*>(take(p.parts));
     a.part_sums = static_cast<float2*>(take(p.part_sums));

@@ -16,9 +16,9 @@
 //
 // Selection is bound by the latency of its steps (reads, digits, lists) on one
 // workgroup a head, moving by HBM: 8 heads of 4 sequences of 32768 tokens cut to
-// 4096 take 22 us and then 134 MB, read and written, 30 us (4.4 TB/s); 2 heads of
-// 64 sequences of 2049 cut to 2048 8.9 us in one launch, where two take 12.1.  One
-// sequence of 131072 tokens, in pieces, takes 134 us in all.
+// 4096 take 23 us and then 134 MB, read and written, 30 us (4.4 TB/s); 2 heads of
+// 64 sequences of 2049 cut to 2048 10.9 us in one launch, where two take 12.6.  One
+// sequence of 131072 tokens, in pieces, cut to 16384 takes 151 us in all.
 #include "kv_device.h"
 
 namespace {
