@@ -214,3 +214,30 @@ def test_4_bit_blocks_that_are_nan_in_live_tokens(kv, dtype, dim):
     place = torch.arange(160, device="cuda").view(10, 16) < 150
     assert torch.isnan(c.mass[table[0, :10].long(), 1][place]).all()
     assert torch.equal(c.mass[table[0, :10].long(), 1][~place], mass[table[0, :10].long(), 1][~place])
+
+
+@pytest.mark.parametrize("dtype,mx", [("bf16", False), ("f16", False), ("f32", False), ("bf16", True), ("f16", True)])
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 20)])
+@pytest.mark.parametrize("octaves", [14, 22, 27, 31])
+def test_attend_light_tokens_alone_in_a_column(kv, dtype, mx, dim, group, octaves):
+    """The heavy tokens' values are zero, so that outputs are what tokens of
+    2^-octaves of their weight add up to: those keep their bits too."""
+    import test_gpu_kv_cache as T
+    page, pages, length = 32, 8, 230
+    c = T.make(kv, dtype, mx, dim, page, 1, pages, seed=octaves, track=False)
+    table, n = T.tables([length], page, pages, seed=octaves)
+    g = torch.Generator(device="cuda").manual_seed(octaves)
+    score = -octaves * np.log(2.0) - torch.rand(length, device="cuda", generator=g)
+    heavy = torch.randperm(length, device="cuda", generator=g)[:5]
+    score[heavy] = 0
+    k = torch.zeros(length, 1, dim, device="cuda")
+    k[:, 0, 0] = score
+    v = 2 + 4 * torch.rand(length, 1, dim, device="cuda", generator=g)
+    if dtype != "bf16":
+        v = v * 2.0 ** 13 * torch.where(torch.rand(v.shape, device="cuda", generator=g) < 0.5, -1, 1)
+    v[heavy] = 0
+    slots = c.slots(table, torch.zeros(length, device="cuda"), torch.arange(length, device="cuda"))
+    c.append(k.to(T.DTYPES[dtype]), v.to(T.DTYPES[dtype]), slots)
+    q = torch.zeros(1, group, dim, device="cuda").to(T.DTYPES[dtype])
+    q[..., 0] = 1
+    T.check_attend(kv, c, dtype, q, table, n, scale=1.0)
