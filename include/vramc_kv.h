@@ -11,7 +11,8 @@
  * 0, a hipError_t, or a negative RANS_E* code for arguments refused before
  * anything is launched (RANS_EUNSUPPORTED: a type or size without a kernel,
  * RANS_EWORKSPACE: workspace missing or too small, RANS_EARG: a null pointer,
- * a size out of range or a pointer less aligned than its kernel reads).
+ * a size out of range, a pointer less aligned than its kernel reads, or an
+ * output over what the call reads where that is said to be refused).
  *
  * Layout.  Keys and values are [pages][kv_heads][page_size][head_dim],
  * contiguous.  With mx = 0 they are values of dtype.  With mx = 1 they are
