@@ -1,9 +1,10 @@
 /*
  * vramc_kv.h -- C ABI of the key-value cache in librans_hip.so: pages of keys
  * and values in the model's type or in microscaled 4-bit floating point, the
- * attention of one new token over them, and eviction by accumulated weight.
- * No reference counterpart: snuri00/vram-compression stops at the weights;
- * this is the other part of a served model's memory.
+ * attention of one new token over them, eviction by accumulated weight, and the
+ * choice of the pages that a query attends to.  No reference counterpart:
+ * snuri00/vram-compression stops at the weights; this is the other part of a
+ * served model's memory.
  *
  * Conventions are those of vramc_rans.h: every pointer in the descriptor is a
  * device pointer owned by the caller, launches are asynchronous on the
@@ -106,6 +107,33 @@ int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int64_t table_
                    int budget, int recent, const int32_t* into, int64_t into_row, int into_width,
                    int32_t* new_lengths, void* workspace, int64_t workspace_bytes,
                    hipStream_t stream);
+
+/* The smallest and largest key of each column of n pages (a number that is no page
+ * of the cache is skipped): bounds[page][kv_head][0 and 1][head_dim] of dtype,
+ * 16-byte aligned, over all places of the page; NaN in both where a column has a
+ * key that is not finite. */
+int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, void* bounds,
+                   hipStream_t stream);
+
+/* The pages of each sequence that its query attends to, for each kv head by itself:
+ * all of them where there are at most `count`, or else the first `first`, the last
+ * `last` and those of the largest score,
+ *   score = max over the kv head's query heads of sum_d max(q_d lo_d, q_d hi_d),
+ * which no q . k of the page exceeds, lo and hi its bounds; in 64 bits, ties to the
+ * lower index, a score that is not a number before all others, an entry that is no
+ * page behind all (any pages where a query is not finite).  0 <= first, 1 <= last, first + last <= count.  lengths are cut
+ * to 0 and table_width * page_size.
+ * chosen[b*kv_heads + h][count]: the pages in order of the sequence's, page * kv_heads
+ * + h (a page of the same tensors taken as a cache of pages * kv_heads pages of one
+ * head), -1 for an entry that is none and behind the last; held[b*kv_heads + h]: the
+ * tokens in them, so that vramc_kv_attend takes both as table and lengths.
+ * workspace: vramc_kv_select_workspace bytes, no content expected, 16-byte aligned. */
+int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int table_width, int batch, int count);
+int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, const void* q, int64_t q_seq,
+                    int64_t q_head, int q_heads, const int32_t* table, int64_t table_row,
+                    int table_width, const int32_t* lengths, int batch, int count, int first,
+                    int last, int32_t* chosen, int32_t* held, void* workspace,
+                    int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

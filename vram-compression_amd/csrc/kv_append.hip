@@ -20,42 +20,6 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 8;  // values of a thread
-
-// Eight values where they lie in a cache, whose tensors are aligned to 16 bytes: as
-// one vector, eight floats would promise 32.
-template <typename T>
-struct Lying {
-    vec<uint32_t, 4> part[kPer * sizeof(T) / 16];
-};
-
-// The largest magnitude of eight values, as the bits of a float: magnitudes of a
-// float format sort as their bits do, infinity and NaN above all.
-template <typename T>
-__device__ __forceinline__ uint32_t largest(vec<T, kPer> x) {
-    const auto bits = __builtin_bit_cast(vec<uint16_t, kPer>, x) & (uint16_t)0x7fff;
-    const auto a = __builtin_elementwise_max(bits.lo, bits.hi);
-    const auto b = __builtin_elementwise_max(a.lo, a.hi);
-    return __float_as_uint((float)__builtin_bit_cast(T, (uint16_t)max(b[0], b[1])));
-}
-
-// Eight codes of x / unit, unit a power of two.
-template <typename T>
-__device__ __forceinline__ uint32_t mx_codes(vec<T, kPer> x, float unit) {
-    const vec<T, 2> a = x.s01, b = x.s23, c = x.s45, d = x.s67;
-    uint32_t r = 0;
-    if constexpr (std::is_same_v<T, __bf16>) {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, a, unit, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, b, unit, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, c, unit, 2);
-        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, d, unit, 3);
-    } else {
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, a, unit, 0);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, b, unit, 1);
-        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, c, unit, 2);
-        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, d, unit, 3);
-    }
-}
 
 // What a thread's row is: a token of a head, and where it lies in the cache.
 struct Row {
@@ -73,31 +37,6 @@ __device__ __forceinline__ Row row_of(const vramc_kv_cache& c, int page_shift,
     r.there = slot >= 0 && slot < (int64_t)c.pages << page_shift;
     r.at = (((slot >> page_shift) * c.kv_heads + r.head) << page_shift) + (slot & (c.page_size - 1));
     return r;
-}
-
-// Eight values of a row of the cache, written past the caches, which the tokens
-// of a long append would only pass through (32768 tokens of 8 heads of 128
-// columns in bf16 53.2 us against 55.1, in 4 bits 38.9 against 40.4).
-template <typename T, bool MX>
-__device__ __forceinline__ void store(vec<T, kPer> x, void* held, uint8_t* scales, int64_t at, int per_row,
-                                      int seg) {
-    if constexpr (!MX) {
-        const auto from = __builtin_bit_cast(Lying<T>, x);
-        auto* to = static_cast<Lying<T>*>(held) + at * per_row + seg;
-#pragma unroll
-        for (size_t i = 0; i < sizeof(T) / 2; i++) __builtin_nontemporal_store(from.part[i], &to->part[i]);
-    } else {
-        // a block's threads are four neighbours of a wave
-        uint32_t most = largest(x);
-        most = max(most, (uint32_t)__shfl_xor((int)most, 1));
-        most = max(most, (uint32_t)__shfl_xor((int)most, 2));
-        // the scale's byte, floor(log2(most)) - 2 + 127, from the exponent's bits
-        const int bits = (int)(most >> 23);
-        const int byte = bits == 255 ? 255 : max(bits - 2, 0);
-        const uint32_t codes = mx_codes(x, __uint_as_float((uint32_t)byte << 23));
-        __builtin_nontemporal_store(byte == 255 ? 0u : codes, static_cast<uint32_t*>(held) + at * per_row + seg);
-        if (seg % 4 == 0) scales[at * (per_row / 4) + seg / 4] = (uint8_t)byte;
-    }
 }
 
 // Eight values of a row of the cache, read.

@@ -1,7 +1,7 @@
-// What the key-value cache's kernels share: the 4-bit format's conversions and
-// the checks of a cache's descriptor.  Everything sits in an anonymous
-// namespace: each .hip file is a translation unit of its own.  The layout is
-// documented in include/vramc_kv.h.
+// What the key-value cache's kernels share: the 4-bit format's conversions, the
+// writing of rows and the checks of a cache's descriptor.  Everything sits in an
+// anonymous namespace: each .hip file is a translation unit of its own.  The
+// layout is documented in include/vramc_kv.h.
 #ifndef VRAMC_KV_DEVICE_H
 #define VRAMC_KV_DEVICE_H
 
@@ -50,6 +50,68 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
     return x;
+}
+
+constexpr int kPer = 8;  // values of a thread that copies rows
+
+// Eight values where they lie in a cache, whose tensors are aligned to 16 bytes: as
+// one vector, eight floats would promise 32.
+template <typename T>
+struct Lying {
+    vec<uint32_t, 4> part[kPer * sizeof(T) / 16];
+};
+
+// The largest magnitude of eight values, as the bits of a float: magnitudes of a
+// float format sort as their bits do, infinity and NaN above all.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(vec<T, kPer> x) {
+    const auto bits = __builtin_bit_cast(vec<uint16_t, kPer>, x) & (uint16_t)0x7fff;
+    const auto a = __builtin_elementwise_max(bits.lo, bits.hi);
+    const auto b = __builtin_elementwise_max(a.lo, a.hi);
+    return __float_as_uint((float)__builtin_bit_cast(T, (uint16_t)max(b[0], b[1])));
+}
+
+// Eight codes of x / unit, unit a power of two.
+template <typename T>
+__device__ __forceinline__ uint32_t mx_codes(vec<T, kPer> x, float unit) {
+    const vec<T, 2> a = x.s01, b = x.s23, c = x.s45, d = x.s67;
+    uint32_t r = 0;
+    if constexpr (std::is_same_v<T, __bf16>) {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, a, unit, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, b, unit, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, c, unit, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, d, unit, 3);
+    } else {
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, a, unit, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, b, unit, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, c, unit, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(r, d, unit, 3);
+    }
+}
+
+// Eight values of a row of the cache, written past the caches, which the tokens
+// of a long append would only pass through (32768 tokens of 8 heads of 128
+// columns in bf16 53.2 us against 55.1, in 4 bits 38.9 against 40.4).
+template <typename T, bool MX>
+__device__ __forceinline__ void store(vec<T, kPer> x, void* held, uint8_t* scales, int64_t at, int per_row,
+                                      int seg) {
+    if constexpr (!MX) {
+        const auto from = __builtin_bit_cast(Lying<T>, x);
+        auto* to = static_cast<Lying<T>*>(held) + at * per_row + seg;
+#pragma unroll
+        for (size_t i = 0; i < sizeof(T) / 2; i++) __builtin_nontemporal_store(from.part[i], &to->part[i]);
+    } else {
+        // a block's threads are four neighbours of a wave
+        uint32_t most = largest(x);
+        most = max(most, (uint32_t)__shfl_xor((int)most, 1));
+        most = max(most, (uint32_t)__shfl_xor((int)most, 2));
+        // the scale's byte, floor(log2(most)) - 2 + 127, from the exponent's bits
+        const int bits = (int)(most >> 23);
+        const int byte = bits == 255 ? 255 : max(bits - 2, 0);
+        const uint32_t codes = mx_codes(x, __uint_as_float((uint32_t)byte << 23));
+        __builtin_nontemporal_store(byte == 255 ? 0u : codes, static_cast<uint32_t*>(held) + at * per_row + seg);
+        if (seg % 4 == 0) scales[at * (per_row / 4) + seg / 4] = (uint8_t)byte;
+    }
 }
 
 // The checks of every entry point.

@@ -1,0 +1,308 @@
+// RMS norms of queries and keys for each head and their rotation by positions, in
+// one pass, the keys and values into tensors or into the pages of a cache.
+//
+// Every value is read and written once, and HBM bounds it.  A thread takes eight
+// columns of a head, 16 bytes of a 16-bit type, a row of the workgroup's threads
+// one head, so that the norm is a sum over at most 32 lanes.  The columns that its
+// own rotate with are read again, from the caches, by the same thread: no exchange.
+//
+// A workgroup takes some tokens of one kind (queries, keys or values) with all
+// their heads.  The angles are the same for all heads of a token: one thread makes
+// each, to LDS.  position * turns is the angle in full turns, so that what it has
+// of whole ones falls away exactly in 64 bits, and 32 hold the rest.
+#include "kv_device.h"
+
+#include "../../include/vramc_rotary.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Rows of one kind: `heads` of each token; how workgroups take them.
+struct Kind {
+    const void* x;
+    int64_t token, head;     // strides
+    const void* weight;
+    void* out;
+    int heads;
+    bool wide;               // rows can be read 16 bytes at a time
+    int shift;               // a workgroup has 2^shift tokens,
+    bool tokens_first;       // neighbouring rows of threads neighbouring tokens (or heads) of them,
+    int splits, passes;      // and takes `passes` of the steps of one of `splits`
+    uint32_t blocks;
+};
+
+struct Rotate {
+    Kind kind[3];            // queries, keys, values
+    const double* turns;
+    int pairs, dim, lanes;   // lanes: of a row, a power of two
+    float amplitude, eps;
+    bool weight_f32;
+    const int32_t* positions;
+    int tokens;
+    // where keys and values go into a cache
+    vramc_kv_cache c;
+    int page_shift;
+    const int64_t* slots;
+};
+
+// Eight values as they lie, rows aligned to 16 bytes where they are wide.
+template <typename T>
+__device__ __forceinline__ vec<T, kPer> load(const T* p, bool wide) {
+    if (wide) return __builtin_bit_cast(vec<T, kPer>, *reinterpret_cast<const Lying<T>*>(p));
+    vec<T, kPer> x;
+#pragma unroll
+    for (int j = 0; j < kPer; j++) x[j] = p[j];
+    return x;
+}
+
+template <typename T>
+__device__ __forceinline__ vec<float, kPer> floats(vec<T, kPer> x) {
+    if constexpr (std::is_same_v<T, float>) return x;
+    else return __builtin_convertvector(x, vec<float, kPer>);
+}
+
+// The sum over the lanes of a row, 8 to 32: within each half of 16 lanes by moves
+// that mirror it, then over the halves.
+__device__ __forceinline__ float row_sum(float x, int lanes) {
+    const auto add = [&](auto control) {
+        x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), control(), 0xf, 0xf, true));
+    };
+    add([] { return 0xb1; });   // quad_perm:[1,0,3,2]
+    add([] { return 0x4e; });   // quad_perm:[2,3,0,1]
+    add([] { return 0x141; });  // row_half_mirror
+    if (lanes >= 16) add([] { return 0x140; });  // row_mirror
+    if (lanes == 32) x += __shfl_xor(x, 16);
+    return x;
+}
+
+enum Into { kTensor, kPlain, kMx };
+
+template <typename T, bool INTERLEAVED, Into INTO>
+__global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a) {
+    extern __shared__ __attribute__((aligned(16))) float angles[];  // [token][cosines, sines][pairs]
+    // this workgroup's kind, tokens and steps
+    const int which = blockIdx.x < a.kind[0].blocks ? 0 : blockIdx.x - a.kind[0].blocks < a.kind[1].blocks ? 1 : 2;
+    const Kind& k = a.kind[which];
+    const uint32_t block = blockIdx.x - (which > 0 ? a.kind[0].blocks : 0) - (which > 1 ? a.kind[1].blocks : 0);
+    const int tile = block / k.splits, part = block - tile * k.splits;
+    const int first = tile << k.shift, tokens = min(a.tokens - first, 1 << k.shift);
+    const int thread = threadIdx.y * a.lanes + threadIdx.x;
+    if (which < 2) {
+        for (int i = thread; i < tokens * a.pairs; i += kThreads) {
+            const int t = i / a.pairs, j = i - t * a.pairs;
+            const double turn = (double)a.positions[first + t] * a.turns[j];
+            float sine, cosine;
+            sincospif(2.f * (float)(turn - __builtin_rint(turn)), &sine, &cosine);
+            angles[2 * t * a.pairs + j] = cosine * a.amplitude;
+            angles[(2 * t + 1) * a.pairs + j] = sine * a.amplitude;
+        }
+        __syncthreads();
+    }
+    const int seg = threadIdx.x, column = kPer * seg, per_row = a.dim / kPer;
+    const bool inside = seg < per_row, turned = inside && column < 2 * a.pairs;
+    // the columns that these rotate with, the angles of both, and which way
+    const bool second = !INTERLEAVED && column >= a.pairs;
+    const int other = !turned ? column : second ? column - a.pairs : column + a.pairs;
+    const int angle = INTERLEAVED ? column / 2 : second ? column - a.pairs : column;
+    const bool norm = which < 2 && k.weight;
+    vec<float, kPer> w = {}, w_other = {};
+    if (norm && inside) {
+        const auto take = [&](int at) {
+            if (a.weight_f32) return load(static_cast<const float*>(k.weight) + at, true);
+            return floats(load(static_cast<const T*>(k.weight) + at, true));
+        };
+        w = take(column);
+        if constexpr (!INTERLEAVED) w_other = take(other);
+    }
+    const float share = 1.f / a.dim;
+    const int rows = k.heads << k.shift, step = blockDim.y;
+    int row = part * k.passes * step + threadIdx.y;
+    // the row's token and head, and how far a step goes
+    int t, head, t_step, head_step;
+    if (k.tokens_first) {
+        t = row & ((1 << k.shift) - 1), head = row >> k.shift, t_step = 0, head_step = step >> k.shift;
+    } else {
+        t = row / k.heads, head = row - t * k.heads, t_step = step / k.heads, head_step = step - t_step * k.heads;
+    }
+    for (int i = 0; i < k.passes && row < rows; i++, row += step) {
+        if (t < tokens) {  // lanes beyond the row take part in its sum
+            const T* in = static_cast<const T*>(k.x) + (first + t) * k.token + head * k.head;
+            vec<T, kPer> raw = {}, raw_other = {}, y;
+            if (inside) {
+                raw = load(in + column, k.wide);
+                if constexpr (!INTERLEAVED)
+                    if (which < 2) raw_other = load(in + other, k.wide);
+            }
+            int64_t at = -1;
+            if (INTO != kTensor && which > 0) {
+                const int64_t slot = a.slots[first + t];
+                if (slot >= 0 && slot < (int64_t)a.c.pages << a.page_shift)
+                    at = (((slot >> a.page_shift) * a.c.kv_heads + head) << a.page_shift) + (slot & (a.c.page_size - 1));
+            }
+            if (which == 2) {
+                y = raw;
+            } else {
+                vec<float, kPer> x = floats(raw), z;
+                float scale = 1.f;
+                if (norm) {
+                    float squares = 0.f;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++) squares += x[j] * x[j];
+                    scale = rsqrtf(row_sum(squares, a.lanes) * share + a.eps);
+                    x *= w;
+                }
+                if (turned) {
+                    const float* cs = angles + 2 * t * a.pairs + angle;
+                    if constexpr (INTERLEAVED) {
+#pragma unroll
+                        for (int j = 0; j < kPer; j += 2) {
+                            const float cosine = cs[j / 2], sine = cs[a.pairs + j / 2];
+                            z[j] = x[j] * cosine - x[j + 1] * sine;
+                            z[j + 1] = x[j + 1] * cosine + x[j] * sine;
+                        }
+                    } else {
+                        vec<float, kPer> x_other = floats(raw_other);
+                        if (norm) x_other *= w_other;
+#pragma unroll
+                        for (int j = 0; j < kPer; j++) {
+                            const float sine = cs[a.pairs + j];
+                            z[j] = x[j] * cs[j] + x_other[j] * (second ? sine : -sine);
+                        }
+                    }
+                } else {
+                    z = x;
+                }
+                z *= scale;
+                if constexpr (std::is_same_v<T, float>) y = z;
+                else y = __builtin_convertvector(z, vec<T, kPer>);
+            }
+            if (!inside) {
+            } else if (INTO == kTensor || which == 0) {
+                auto* out = static_cast<Lying<T>*>(k.out) + ((int64_t)(first + t) * k.heads + head) * per_row + seg;
+                *out = __builtin_bit_cast(Lying<T>, y);
+            } else if constexpr (INTO != kTensor) {
+                if (at >= 0) {  // a block's threads share it
+                    store<T, INTO == kMx>(y, which == 1 ? a.c.k : a.c.v, which == 1 ? a.c.k_scale : a.c.v_scale, at,
+                                          per_row, seg);
+                    if (which == 1 && a.c.mass && seg == 0) {
+                        a.c.mass[at] = 0.f;
+                        a.c.position[at] = a.positions[first + t];
+                    }
+                }
+            }
+        }
+        t += t_step, head += head_step;
+        if (!k.tokens_first && head >= k.heads) head -= k.heads, t++;
+    }
+}
+
+int check(const vramc_rotary* r, const vramc_rotary_rows* x) {
+    if (!r || !x || !r->turns) return RANS_EARG;
+    switch (r->head_dim) {
+        case 64: case 96: case 128: case 192: case 256: break;
+        default: return RANS_EUNSUPPORTED;
+    }
+    if (r->pairs <= 0 || r->pairs % 8 || 2 * r->pairs > r->head_dim) return RANS_EUNSUPPORTED;
+    if (x->dtype != RANS_X_F32 && x->dtype != RANS_X_BF16 && x->dtype != RANS_X_F16) return RANS_EUNSUPPORTED;
+    const bool weights = x->q_weight || x->k_weight;
+    if (weights && x->weight_dtype != RANS_X_F32 && x->weight_dtype != x->dtype) return RANS_EUNSUPPORTED;
+    if (x->q_heads < 0 || x->k_heads < 0 || !(x->eps >= 0) || x->tokens < 0) return RANS_EARG;
+    if (x->q_token < 0 || x->q_head < 0 || x->k_token < 0 || x->k_head < 0) return RANS_EARG;
+    // rows are counted in 32 bits, and a launch has fewer than 2^32 threads
+    const int64_t most = (int64_t)(x->q_heads > x->k_heads ? x->q_heads : x->k_heads);
+    if (x->tokens > (1 << 26) || most > (1 << 16) || x->tokens * most > (1 << 26)) return RANS_EARG;
+    if (x->tokens && (!x->positions || (x->q_heads && !x->q) || (x->k_heads && !x->k))) return RANS_EARG;
+    if (((uintptr_t)x->q_weight | (uintptr_t)x->k_weight) % 16) return RANS_EARG;
+    return 0;
+}
+
+// Whether a dense output shares memory with rows that are read.
+bool overlap(const void* out, int64_t bytes, const void* x, int64_t token, int64_t head, int64_t tokens, int64_t heads,
+             int64_t dim, int64_t size) {
+    if (!bytes || !tokens || !heads) return false;
+    const int64_t all = ((tokens - 1) * token + (heads - 1) * head + dim) * size;
+    return (uintptr_t)out < (uintptr_t)x + all && (uintptr_t)x < (uintptr_t)out + bytes;
+}
+
+template <typename T>
+Kind kind_of(const vramc_rotary& r, const void* x, int64_t token, int64_t head, int heads, const void* weight, void* out,
+             int64_t tokens, int lanes, bool pages) {
+    Kind k{x, token, head, weight, out, heads, false, 0, false, 1, 0, 0};
+    if (!heads || !tokens) return k;
+    constexpr int64_t size = sizeof(T);
+    k.wide = ((uintptr_t)x | (uintptr_t)(token * size) | (uintptr_t)(head * size)) % 16 == 0;
+    const int step = kThreads / lanes;
+    if (tokens >= 1024) {
+        if (pages) k.shift = __builtin_ctz(step), k.tokens_first = true;
+        else k.shift = tokens >= 8192 ? 3 : 2;
+    }
+    const int steps = ((heads << k.shift) + step - 1) / step;
+    k.splits = k.shift ? 1 : steps;
+    k.passes = k.shift ? steps : 1;
+    k.blocks = (uint32_t)((tokens + (1 << k.shift) - 1) >> k.shift) * (uint32_t)k.splits;
+    return k;
+}
+
+template <typename T, Into INTO>
+int launch(const vramc_rotary& r, const vramc_rotary_rows& x, const vramc_kv_cache* c, const void* v, int64_t v_token,
+           int64_t v_head, const int64_t* slots, void* q_out, void* k_out, hipStream_t stream) {
+    const int lanes = r.head_dim <= 64 ? 8 : r.head_dim <= 128 ? 16 : 32;
+    constexpr bool pages = INTO != kTensor;
+    Rotate a{};
+    a.kind[0] = kind_of<T>(r, x.q, x.q_token, x.q_head, x.q_heads, x.q_weight, q_out, x.tokens, lanes, false);
+    a.kind[1] = kind_of<T>(r, x.k, x.k_token, x.k_head, x.k_heads, x.k_weight, k_out, x.tokens, lanes, pages);
+    a.kind[2] = kind_of<T>(r, v, v_token, v_head, pages ? x.k_heads : 0, nullptr, nullptr, x.tokens, lanes, pages);
+    a.turns = r.turns, a.pairs = r.pairs, a.dim = r.head_dim, a.lanes = lanes;
+    a.amplitude = r.amplitude, a.eps = x.eps, a.weight_f32 = x.weight_dtype == RANS_X_F32;
+    a.positions = x.positions, a.tokens = (int)x.tokens;
+    if (pages) a.c = *c, a.page_shift = __builtin_ctz(c->page_size), a.slots = slots;
+    const int64_t blocks = (int64_t)a.kind[0].blocks + a.kind[1].blocks + a.kind[2].blocks;
+    if (blocks == 0) return 0;
+    if (blocks > kMaxThreads / kThreads) return RANS_EARG;
+    const int shift = a.kind[0].shift > a.kind[1].shift ? a.kind[0].shift : a.kind[1].shift;
+    const size_t lds = (size_t)(8 * r.pairs) << shift;
+    const dim3 grid((unsigned)blocks), block((unsigned)lanes, (unsigned)(kThreads / lanes));
+    if (r.interleaved) hipLaunchKernelGGL((rotate_kernel<T, true, INTO>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL((rotate_kernel<T, false, INTO>), grid, block, lds, stream, a);
+    return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int vramc_rotary_apply(const vramc_rotary* r, const vramc_rotary_rows* x, void* q_out, void* k_out,
+                                  hipStream_t stream) {
+    if (const int rc = check(r, x)) return rc;
+    if (x->tokens == 0) return 0;
+    if ((x->q_heads && !q_out) || (x->k_heads && !k_out) || ((uintptr_t)q_out | (uintptr_t)k_out) % 16) return RANS_EARG;
+    const int64_t size = x->dtype == RANS_X_F32 ? 4 : 2, dim = r->head_dim;
+    const struct { const void* at; int64_t bytes; } outs[] = {{q_out, x->tokens * x->q_heads * dim * size},
+                                                              {k_out, x->tokens * x->k_heads * dim * size}};
+    for (const auto& o : outs)
+        if (overlap(o.at, o.bytes, x->q, x->q_token, x->q_head, x->tokens, x->q_heads, dim, size) ||
+            overlap(o.at, o.bytes, x->k, x->k_token, x->k_head, x->tokens, x->k_heads, dim, size))
+            return RANS_EARG;
+    const auto go = [&](auto fn) { return fn(*r, *x, nullptr, nullptr, 0, 0, nullptr, q_out, k_out, stream); };
+    if (x->dtype == RANS_X_F32) return go(launch<float, kTensor>);
+    return x->dtype == RANS_X_BF16 ? go(launch<__bf16, kTensor>) : go(launch<_Float16, kTensor>);
+}
+
+extern "C" int vramc_rotary_append(const vramc_rotary* r, const vramc_rotary_rows* x, const vramc_kv_cache* c,
+                                   const void* v, int64_t v_token, int64_t v_head, const int64_t* slots, void* q_out,
+                                   hipStream_t stream) {
+    if (const int rc = check(r, x)) return rc;
+    if (const int rc = check_cache(c)) return rc;
+    if (c->head_dim != r->head_dim || c->dtype != x->dtype || c->kv_heads != x->k_heads || v_token < 0 || v_head < 0)
+        return RANS_EARG;
+    if (x->tokens == 0) return 0;
+    if (!v || !slots || (x->q_heads && !q_out) || (uintptr_t)q_out % 16) return RANS_EARG;
+    const int64_t size = x->dtype == RANS_X_F32 ? 4 : 2, dim = r->head_dim, bytes = x->tokens * x->q_heads * dim * size;
+    if (overlap(q_out, bytes, x->q, x->q_token, x->q_head, x->tokens, x->q_heads, dim, size) ||
+        overlap(q_out, bytes, x->k, x->k_token, x->k_head, x->tokens, x->k_heads, dim, size) ||
+        overlap(q_out, bytes, v, v_token, v_head, x->tokens, x->k_heads, dim, size))
+        return RANS_EARG;
+    const auto go = [&](auto fn) { return fn(*r, *x, c, v, v_token, v_head, slots, q_out, nullptr, stream); };
+    if (x->dtype == RANS_X_F32) return go(launch<float, kPlain>);
+    if (x->dtype == RANS_X_BF16) return c->mx ? go(launch<__bf16, kMx>) : go(launch<__bf16, kPlain>);
+    return c->mx ? go(launch<_Float16, kMx>) : go(launch<_Float16, kPlain>);
+}

@@ -1,6 +1,7 @@
 """The key-value cache of a served model on MI355X: pages of keys and values
-in the model's type or in 4 bits, the attention of one new token over them, and
-eviction by accumulated attention weight.
+in the model's type or in 4 bits, the attention of one new token over them (all of
+them, or the pages that its query can give the largest scores), and eviction by
+accumulated attention weight.
 
 The weights are one part of a served model's memory, the cache of past tokens
 the other; the reference stops at the weights (README.md:39 names model
@@ -13,7 +14,7 @@ PagedCache holds that cache:
     lengths = cache.evict(table, lengths, seen, budget, recent)
 
 A sequence's tokens lie in the pages that its row of `table` names, in order;
-which pages are free is the program's to keep.  Every operation is a
+which pages are free is the program's to keep, or kv_pages.PagePool's.  Every operation is a
 hand-written HIP kernel in librans_hip.so (include/vramc_kv.h), runs on the
 current stream and allocates from torch.  There is no CPU fallback, and nothing
 that torch could watch: calls under a gradient, forward mode, vmap, a tracer, a
@@ -33,7 +34,8 @@ HEAD_DIMS = (64, 96, 128, 192, 256)
 _DTYPES = rans._X_CODES
 
 EXPORTS = ("vramc_kv_append", "vramc_kv_read", "vramc_kv_attend_workspace", "vramc_kv_attend",
-           "vramc_kv_evict_workspace", "vramc_kv_evict")
+           "vramc_kv_evict_workspace", "vramc_kv_evict", "vramc_kv_bound",
+           "vramc_kv_select_workspace", "vramc_kv_select")
 
 
 class KvCacheDesc(ctypes.Structure):
@@ -61,13 +63,22 @@ def bind(lib):
                              I64, P], I32),
         "vramc_kv_evict_workspace": ([D, I32, I32, I32, I32], I64),
         "vramc_kv_evict": ([D, P, I64, I32, P, P, I32, I32, I32, P, I64, I32, P, P, I64, P], I32),
+        "vramc_kv_bound": ([D, P, I64, P, P], I32),
+        "vramc_kv_select_workspace": ([D, I32, I32, I32], I64),
+        "vramc_kv_select": ([D, P, P, I64, I64, I32, P, I64, I32, P, I32, I32, I32, I32, P, P, P, I64, P],
+                            I32),
     }
+    set_types(lib, sig)
+    lib._kv_bound = True
+    return lib
+
+
+def set_types(lib, sig):
+    """Sets the argument and result types of {name: (arguments, result)}."""
     for name, (args, res) in sig.items():
         f = getattr(lib, name)
         f.argtypes = args
         f.restype = res
-    lib._kv_bound = True
-    return lib
 
 
 def _check(ok, message):
@@ -83,7 +94,33 @@ def _failed(name, rc):
     raise RuntimeError(f"{name}: HIP error {rc}")
 
 
-class PagedCache:
+class Calls:
+    """What the calls of something on the GPU (device, its number _index) check of
+    their arguments.  The checks run on every token step: messages are made only for
+    a failure."""
+
+    def _stream(self):
+        """The current stream, for a call that nothing watches."""
+        if _watched():
+            raise ValueError("forward mode, vmap, a tracer or a dispatch or function mode watches this "
+                             "call, and the cache's operations are hidden from them")
+        if rans._device() != self._index:
+            raise ValueError(f"the tensors are on {self.device}, the current device is another")
+        return rans._stream()
+
+    def _ints(self, name, t, dtype, shape):
+        """Checks integers of a shape (None for any size) whose last dimension
+        is dense."""
+        got = t.shape
+        if (t.dtype is not dtype or t.get_device() != self._index or len(got) != len(shape)
+                or (got[0] != shape[0] and shape[0] is not None)
+                or (got[-1] > 1 and t.stride(-1) != 1)):
+            want = tuple("n" if n is None else n for n in shape)
+            raise ValueError(f"{name} must be {want} of {dtype} on {self.device}, its last dimension "
+                             f"dense; got {tuple(got)} of {t.dtype} on {t.device}, strides {t.stride()}")
+
+
+class PagedCache(Calls):
     """Keys and values of past tokens in pages on the GPU.
 
     k, v: (pages, kv_heads, page_size, head_dim) of dtype (bf16, f16 or f32),
@@ -91,8 +128,9 @@ class PagedCache:
     scale byte for every 32 columns, uint8 (.., head_dim / 32) (bf16 or f16
     values; the MXFP4 format, 4.25 bits a value).  mass (f32) and position
     (int32), (pages, kv_heads, page_size), where tokens' accumulated weights are
-    tracked.  The tensors are used as they are, not copied, and a cache keeps those
-    that it was made of."""
+    tracked.  bounds: (pages, kv_heads, 2, head_dim) of dtype, where queries choose the
+    pages that they attend to.  The tensors are used as they are, not copied, and a
+    cache keeps those that it was made of."""
 
     # The descriptor holds their addresses: not to be assigned.
     k = property(lambda self: self._k)
@@ -101,9 +139,10 @@ class PagedCache:
     v_scale = property(lambda self: self._v_scale)
     mass = property(lambda self: self._mass)
     position = property(lambda self: self._position)
+    bounds = property(lambda self: self._bounds)
 
     def __init__(self, k, v, dtype=torch.bfloat16, k_scale=None, v_scale=None, mass=None,
-                 position=None, lib=None):
+                 position=None, lib=None, bounds=None):
         if not torch.cuda.is_available():
             raise RuntimeError("PagedCache needs a ROCm GPU (gfx950); no CPU fallback exists")
         _check(k.dim() == 4, "k must be (pages, kv_heads, page_size, head_dim)")
@@ -126,6 +165,8 @@ class PagedCache:
         _check((mass is None) == (position is None), "mass and position come together")
         if mass is not None:
             want += [("mass", mass, torch.float32, lead), ("position", position, torch.int32, lead)]
+        if bounds is not None:
+            want.append(("bounds", bounds, dtype, (*lead[:2], 2, self.head_dim)))
         for name, t, dt, shape in want:
             if not (t.is_cuda and t.device == k.device and t.dtype is dt and t.shape == shape
                     and t.is_contiguous()):
@@ -134,10 +175,11 @@ class PagedCache:
             if t.data_ptr() % 16 and not name.endswith("scale"):
                 raise ValueError(f"{name} must be 16-byte aligned")
         self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
-        self._mass, self._position, self.dtype, self.device = mass, position, dtype, k.device
-        self._index = k.get_device()
+        self._mass, self._position, self._bounds = mass, position, bounds
+        self.dtype, self.device, self._index = dtype, k.device, k.get_device()
+        self._heads = None
         self.lib = bind(lib or rans._host_lib())
-        ptr = {n: t.data_ptr() for n, t, _, _ in want}
+        ptr = {n: t.data_ptr() for n, t, _, _ in want if n != "bounds"}
         self._desc = KvCacheDesc(pages=self.pages, kv_heads=self.kv_heads,
                                  page_size=self.page_size, head_dim=self.head_dim,
                                  dtype=_DTYPES[dtype], mx=int(self.mx), **ptr)
@@ -146,9 +188,11 @@ class PagedCache:
 
     @classmethod
     def allocate(cls, pages, kv_heads, head_dim, page_size=64, dtype=torch.bfloat16, mx=False,
-                 track=False, device="cuda", lib=None):
+                 track=False, device="cuda", lib=None, bounds=False):
         """A cache of `pages` free pages.  mx: 4-bit storage; track: with mass
-        and position, which evict needs and attend and append then keep."""
+        and position, which evict needs and attend and append then keep; bounds:
+        with the pages' smallest and largest keys, which select needs and bound
+        makes."""
         if not torch.cuda.is_available():
             raise RuntimeError("PagedCache needs a ROCm GPU (gfx950); no CPU fallback exists")
         lead = (pages, kv_heads, page_size)
@@ -164,33 +208,17 @@ class PagedCache:
             k, v = (zeros(dtype, head_dim) for _ in range(2))
             scales = [None, None]
         more = [zeros(torch.float32), zeros(torch.int32)] if track else [None, None]
-        return cls(k, v, dtype, *scales, *more, lib=lib)
+        limits = torch.zeros(pages, kv_heads, 2, head_dim, dtype=dtype, device=device) if bounds else None
+        return cls(k, v, dtype, *scales, *more, lib=lib, bounds=limits)
 
     # ------------------------------------------------------------- arguments
-    # The checks run on every token step: messages are made only for a failure.
     def _stream(self):
-        """The current stream, for a call that nothing watches."""
-        if _watched():
-            raise ValueError("forward mode, vmap, a tracer or a dispatch or function mode watches this "
-                             "call, and the cache's operations are hidden from them")
         if torch.is_grad_enabled() and (self._k.requires_grad or self._v.requires_grad or (
-                self._mass is not None and self._mass.requires_grad)):
+                self._mass is not None and self._mass.requires_grad) or (
+                self._bounds is not None and self._bounds.requires_grad)):
             raise ValueError("the cache's tensors require a gradient, and its operations have none: "
                              "detach them or use torch.no_grad()")
-        if rans._device() != self._index:
-            raise ValueError(f"the cache is on {self.device}, the current device is another")
-        return rans._stream()
-
-    def _ints(self, name, t, dtype, shape):
-        """Checks integers of a shape (None for any size) whose last dimension
-        is dense."""
-        got = t.shape
-        if (t.dtype is not dtype or t.get_device() != self._index or len(got) != len(shape)
-                or (got[0] != shape[0] and shape[0] is not None)
-                or (got[-1] > 1 and t.stride(-1) != 1)):
-            want = tuple("n" if n is None else n for n in shape)
-            raise ValueError(f"{name} must be {want} of {dtype} on {self.device}, its last dimension "
-                             f"dense; got {tuple(got)} of {t.dtype} on {t.device}, strides {t.stride()}")
+        return super()._stream()
 
     def _rows(self, name, t, heads):
         """Checks rows x heads x head_dim values; a last dimension that is not
@@ -332,3 +360,90 @@ class PagedCache:
         if rc:
             _failed("evict", rc)
         return out
+
+    # ------------------------------------------------- attention over some pages
+    @property
+    def heads(self):
+        """The same tensors as a cache of pages * kv_heads pages of one kv head, page
+        * kv_heads + head: what a selection's page numbers mean."""
+        if self._heads is None:
+            n = self.pages * self.kv_heads
+            k, v, ks, vs, mass, position = (None if t is None else t.view(n, 1, self.page_size, -1)
+                                            for t in (self._k, self._v, self._k_scale, self._v_scale,
+                                                      self._mass, self._position))
+            if mass is not None:
+                mass, position = mass.squeeze(3), position.squeeze(3)
+            self._heads = PagedCache(k, v, self.dtype, ks, vs, mass, position, self.lib)
+        return self._heads
+
+    def bound(self, pages):
+        """Takes the smallest and largest key of each column, over all places, of the
+        pages (int32, any dimension but dense; what is no page of the cache is skipped)
+        into bounds.  select goes by the bounds of all but a sequence's last page: call
+        it for pages that have become full (kv_pages.PagePool.extend names them), and
+        for all of a sequence's after an eviction."""
+        if self._bounds is None:
+            raise ValueError("the cache was made without bounds")
+        stream = self._stream()
+        if pages.dtype is not torch.int32 or pages.get_device() != self._index or not pages.is_contiguous():
+            raise ValueError(f"pages must be a contiguous int32 tensor on {self.device}, got {pages.dtype} "
+                             f"{tuple(pages.shape)} on {pages.device}, strides {pages.stride()}")
+        rc = self.lib.vramc_kv_bound(self._ref, pages.data_ptr(), pages.numel(), self._bounds.data_ptr(),
+                                     stream)
+        if rc:
+            _failed("bound", rc)
+
+    def select(self, q, table, lengths, count, first=1, last=1):
+        """The pages that one new token of each sequence attends to, for each kv head by
+        itself: all where a sequence has at most `count`, else its first `first`, its
+        last `last` (one at least) and those whose keys can give a query head of the kv
+        head the largest score, by their bounds: max over the query heads of
+        sum_d max(q_d lo_d, q_d hi_d), ties to the lower index.  A page with a key that
+        is not finite comes before others, an entry that is no page behind.  Arguments
+        as attend's.  Returns (chosen, held) for attend_selected, int32: chosen
+        (sequences * kv_heads, min(count, table's width)), pages of `heads` in order of
+        the sequence's, -1 behind them, and held, the tokens in them."""
+        if self._bounds is None:
+            raise ValueError("the cache was made without bounds")
+        stream = self._stream()
+        q = self._rows("q", q, None)
+        batch, heads, _ = q.shape
+        if heads <= 0 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.kv_heads} kv heads")
+        self._ints("table", table, torch.int32, (batch, None))
+        self._ints("lengths", lengths, torch.int32, (batch,))
+        if not (first >= 0 and last >= 1 and first + last <= count < 2 ** 31):
+            raise ValueError(f"{count} pages with the first {first} and the last {last}: count is at least "
+                             "their sum, last at least 1")
+        width = table.shape[1]
+        if count >= width:  # all pages, whatever their scores
+            count, first, last = max(width, 1), 0, 1
+        rows = batch * self.kv_heads
+        need = self.lib.vramc_kv_select_workspace(self._ref, width, batch, count)
+        if need < 0:
+            raise ValueError(f"{batch} sequences of {self.kv_heads} kv heads over {width} pages: too many "
+                             f"({need})")
+        chosen = torch.empty((rows, count), dtype=torch.int32, device=self.device)
+        held = torch.empty(rows, dtype=torch.int32, device=self.device)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        rc = self.lib.vramc_kv_select(
+            self._ref, self._bounds.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), heads,
+            table.data_ptr(), table.stride(0), width, lengths.data_ptr(), batch, count, first, last,
+            chosen.data_ptr(), held.data_ptr(), work.data_ptr() if need else None, need, stream)
+        if rc:
+            _failed("select", rc)
+        return chosen, held
+
+    def attend_selected(self, q, chosen, held, scale=None, track=None):
+        """attend over the pages that select chose (which another query of the same
+        sequences may use too, as long as they hold the same tokens): q (sequences,
+        q_heads, head_dim).  scale is positive: pages are chosen for large scores."""
+        q = self._rows("q", q, None)
+        batch, heads, _ = q.shape
+        if heads <= 0 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads are no multiple of {self.kv_heads} kv heads")
+        if scale is not None and not scale > 0:
+            raise ValueError(f"scale {scale}: pages are chosen for large scores")
+        rows, group = batch * self.kv_heads, heads // self.kv_heads
+        out = self.heads.attend(q.reshape(rows, group, self.head_dim), chosen, held, scale, track)
+        return out.view(batch, heads, self.head_dim)

@@ -28,8 +28,9 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "librans_hip.so")
 SOURCES = [os.path.join(CSRC, f) for f in ("rans_gemv.hip", "rans_decode.hip", "rans_linear.hip", "rans_matmul.hip",
                                            "ref32_gemv.hip", "kv_append.hip", "kv_attend.hip",
-                                           "kv_evict.hip", "w64_host.cpp")]
-HEADERS = [os.path.join(INCLUDE, "vramc_rans.h"), os.path.join(INCLUDE, "vramc_kv.h"),
+                                           "kv_evict.hip", "kv_select.hip", "kv_pages.hip",
+                                           "kv_rotary.hip", "w64_host.cpp")]
+HEADERS = [os.path.join(INCLUDE, h) for h in ("vramc_rans.h", "vramc_kv.h", "vramc_pages.h", "vramc_rotary.h")] + [
            os.path.join(CSRC, "rans_device.h"), os.path.join(CSRC, "kv_device.h")]
 
 SCALE_BITS = 12
