@@ -3,9 +3,10 @@
 // A call is latency: a few reads of each sequence, two sums over all of them, and
 // 16 bytes for each token.  extend is one launch: every workgroup makes both sums
 // over all sequences by itself (4096 at most, 16 to a thread), which takes less
-// than a second launch, and then takes 1024 of the rows, whose sequences it finds in
+// than a second launch, and then takes some of the rows, whose sequences it finds in
 // LDS.  What is written (entries behind a sequence's pages, other tensors) nobody
-// reads, but for the stack's count, which the workgroup that ends last sets.
+// reads, but for the stack's count, which the workgroup that ends last sets.  One token
+// each of 64 sequences 3.5 us, and 4.7 to take pages back from their 512 entries each.
 #include "kv_device.h"
 
 #include "../../include/vramc_pages.h"
@@ -14,8 +15,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kRows = 4;                    // rows of a thread
+// Workgroups of extend, which takes more rows in turns: each ends with a count in one
+// place of memory (16 sequences of up to 8000 new tokens 7.1 us; 1024 workgroups, with a
+// fence before the count, 14.5).
+constexpr int kMaxBlocks = 256;
 constexpr int kMaxBatch = 4096;
+constexpr int kTurns = 4;                  // entries of a thread at once
 
 struct Extend {
     vramc_pages p;
@@ -49,81 +54,81 @@ __device__ __forceinline__ int64_t before_of(int64_t x, int64_t* waves) {
 
 __global__ void __launch_bounds__(kThreads) extend_kernel(Extend e) {
     extern __shared__ int32_t shared[];
-    int32_t *ends = shared, *from = shared + e.batch;  // from: pages before a sequence's, -1 without room
+    // first new tokens, then where a sequence's rows end; pages that it holds; pages
+    // taken before its own, -1 without room
+    int32_t *ends = shared, *held = shared + e.batch, *from = shared + 2 * e.batch;
     __shared__ int64_t waves[kWaves];
     __shared__ int taken;
     const int shift = e.page_shift, room = e.width << shift, each = (e.batch + kThreads - 1) / kThreads;
     const int b0 = min((int)threadIdx.x * each, e.batch), b1 = min(b0 + each, e.batch);
     const int have = min(max(*e.p.count, 0), e.p.pages);
-    const auto length_of = [&](int b) { return min(max(e.lengths[b], 0), room); };
-    const auto fresh_of = [&](int b) { return (int64_t)min((uint32_t)max(e.fresh[b], 0), (uint32_t)e.tokens + 1); };
     const auto pages_of = [&](int64_t n) { return (int)((n + (1 << shift) - 1) >> shift); };
-    // pages that a sequence wants whose rows end at `end`
-    const auto want = [&](int b, int64_t end, bool* fits) {
-        const int64_t n = length_of(b), all = n + fresh_of(b);
-        *fits = all <= room && end <= e.tokens;
-        return *fits ? pages_of(all) - pages_of(n) : 0;
+    // pages that a sequence of n tokens wants for m more, whose rows end at `end`
+    const auto want = [&](int n, int m, int64_t end, bool* fits) {
+        *fits = (int64_t)n + m <= room && end <= e.tokens;
+        return *fits ? pages_of(n + m) - pages_of(n) : 0;
     };
     if (threadIdx.x == 0) taken = 0;
     int64_t sum = 0, pages = 0;
     bool fits;
-    for (int b = b0; b < b1; b++) sum += fresh_of(b);
+    for (int b = b0; b < b1; b++) {
+        const int m = (int)min((uint32_t)max(e.fresh[b], 0), (uint32_t)e.tokens + 1);
+        held[b] = min(max(e.lengths[b], 0), room);
+        ends[b] = m;
+        sum += m;
+    }
     const int64_t start = before_of(sum, waves);
     sum = start;
-    for (int b = b0; b < b1; b++) pages += want(b, sum += fresh_of(b), &fits);
+    for (int b = b0; b < b1; b++) pages += want(held[b], ends[b], sum += ends[b], &fits);
     pages = before_of(pages, waves);
     sum = start;
     for (int b = b0; b < b1; b++) {
+        const int n = held[b], m = ends[b];
         if (blockIdx.x == 0) e.starts[b] = (int)min(sum, (int64_t)e.tokens);
-        sum += fresh_of(b);
-        const int need = want(b, sum, &fits);
+        sum += m;
+        const int need = want(n, m, sum, &fits);
         const bool served = fits && (need == 0 || pages + need <= have);
         ends[b] = (int)min(sum, (int64_t)e.tokens);
         from[b] = !served ? -1 : need ? (int)pages : 0;
         pages += need;
         if (served && need) atomicMax(&taken, (int)pages);  // those that are served come first
-        if (blockIdx.x == 0) e.new_lengths[b] = length_of(b) + (served ? (int)fresh_of(b) : 0);
+        if (blockIdx.x == 0) e.new_lengths[b] = n + (served ? m : 0);
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) e.starts[e.batch] = e.batch ? ends[e.batch - 1] : 0;
-#pragma unroll
-    for (int i = 0; i < kRows; i++) {
-        const int64_t row = ((int64_t)blockIdx.x * kRows + i) * kThreads + threadIdx.x;
-        if (row >= e.tokens) break;
+#pragma unroll 1
+    for (int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x; row < e.tokens; row += (int64_t)gridDim.x * kThreads) {
         const int t = (int)row;
         int b = 0;  // the first sequence that ends behind t
+#pragma unroll 1
         for (int n = e.batch; n > 0;) {
             const int half = n / 2;
             const bool behind = ends[b + half] <= t;
             b = behind ? b + half + 1 : b;
             n = behind ? n - half - 1 : half;
         }
-        int64_t slot = -1;
-        int position = 0, full = -1;
+        int page = -1, place = 0, position = 0;
         if (b < e.batch) {
-            const int in = t - (b ? ends[b - 1] : 0), n = length_of(b);
-            position = (int)((uint32_t)(e.seen ? e.seen[b] : n) + (uint32_t)in);
+            const int in = t - (b ? ends[b - 1] : 0), n = held[b];
             if (from[b] >= 0) {
-                const int index = n + in, old = pages_of(n), k = index >> shift, place = index & ((1 << shift) - 1);
+                const int index = n + in, old = pages_of(n), k = index >> shift;
+                place = index & ((1 << shift) - 1);
                 int32_t* entry = e.table + b * e.table_row + k;
-                int page = k < old ? *entry : e.p.free[have - 1 - (from[b] + k - old)];
+                page = *(k < old ? entry : e.p.free + (have - 1 - (from[b] + k - old)));
                 if ((uint32_t)page >= (uint32_t)e.p.pages) page = -1;
                 if (k >= old && place == 0) *entry = page;
-                if (page >= 0) {
-                    slot = ((int64_t)page << shift) + place;
-                    if (place == (1 << shift) - 1) full = page;
-                }
             }
+            position = (int)((uint32_t)(e.seen ? e.seen[b] : n) + (uint32_t)in);
         }
-        e.slots[t] = slot;
+        e.slots[t] = page < 0 ? -1 : ((int64_t)page << shift) + place;
         e.positions[t] = position;
-        e.filled[t] = full;
+        e.filled[t] = place == (1 << shift) - 1 ? page : -1;
     }
     __syncthreads();
     if (threadIdx.x) return;
     if (gridDim.x > 1) {  // the workgroups have all read the count when the last of them is here
-        __threadfence();
-        if (atomicAdd((uint32_t*)e.p.ticket, 1u) != gridDim.x - 1) return;
+        if (__hip_atomic_fetch_add((uint32_t*)e.p.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != gridDim.x - 1)
+            return;
         *e.p.ticket = 0;
     }
     *e.p.count = have - taken;
@@ -137,7 +142,7 @@ struct Release {
     int width;
     const int32_t* lengths;
     int batch;
-    int32_t *counts, *base;  // two launches: pages that each row gives back, and the stack's count before
+    int32_t *counts, *base;  // pages that each row gives back, and the stack's count before
 
     // entries that a row keeps
     __device__ __forceinline__ int kept(int b) const {
@@ -146,57 +151,6 @@ struct Release {
     }
     __device__ __forceinline__ bool is_page(int x) const { return (uint32_t)x < (uint32_t)p.pages; }
 };
-
-// Pieces of 64 entries of a row, kPieces to each of sixteen waves, in registers
-// between their count and their place on the stack.
-constexpr int kAll = 1024, kAllWaves = kAll / 64, kPieces = 32;
-
-__global__ void __launch_bounds__(kAll) release_kernel(Release r) {
-    __shared__ int waves[kAllWaves];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int per_row = (r.width + 63) / 64, all = per_row * r.batch, each = (all + kAllWaves - 1) / kAllWaves;
-    const int have = min(max(*r.p.count, 0), r.p.pages);
-    int x[kPieces], n = 0;
-    const auto place = [&](int u, int* b, int* i) {
-        const int s = wave * each + u;
-        *b = min(s, all - 1) / per_row;
-        *i = (s - *b * per_row) * 64 + lane;
-        return u < each && s < all && *i < r.width;
-    };
-#pragma unroll
-    for (int u = 0; u < kPieces; u++) {
-        if (u >= each) break;
-        int b, i;
-        const bool in = place(u, &b, &i);
-        const int entry = in ? r.table[b * r.table_row + i] : -1;
-        x[u] = i >= r.kept(b) ? entry : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kPieces; u++)
-        if (u < each) n += __popcll(__ballot(r.is_page(x[u])));
-    if (lane == 0) waves[wave] = n;
-    __syncthreads();
-    int at = have, total = have;
-#pragma unroll
-    for (int w = 0; w < kAllWaves; w++) {
-        at += w < wave ? waves[w] : 0;
-        total += waves[w];
-    }
-#pragma unroll
-    for (int u = 0; u < kPieces; u++) {
-        if (u >= each) break;
-        const uint64_t back = __ballot(r.is_page(x[u]));
-        const int to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(back >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)back, 0));
-        if (r.is_page(x[u]) && to < r.p.pages) r.p.free[to] = x[u];
-        if (x[u] != -1) {
-            int b, i;
-            place(u, &b, &i);
-            r.table[b * r.table_row + i] = -1;
-        }
-        at += __popcll(back);
-    }
-    if (threadIdx.x == 0) *r.p.count = min(total, r.p.pages);
-}
 
 // The sum over the workgroup.
 __device__ __forceinline__ int sum_of(int x, int* waves) {
@@ -211,8 +165,10 @@ __device__ __forceinline__ int sum_of(int x, int* waves) {
     return sum;
 }
 
-// Larger tables, a workgroup to a row: how many pages it gives back, and then those
-// behind what the rows before it do.
+// A workgroup to a row: how many pages it gives back, and then, in a second launch,
+// those behind what the rows before it do.  One workgroup that takes a small table
+// whole is no faster (one row of 8 entries 3.8 us against 3.6, 64 of 512 12.6 against
+// 4.7): it waits for its own reads.
 __global__ void __launch_bounds__(kThreads) release_count_kernel(Release r) {
     __shared__ int waves[kWaves];
     const int b = blockIdx.x;
@@ -230,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) release_count_kernel(Release r) {
 }
 
 __global__ void __launch_bounds__(kThreads) release_rows_kernel(Release r) {
-    __shared__ int waves[kWaves], found[kRows][kWaves];
+    __shared__ int waves[kWaves], found[kTurns][kWaves];
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mine = r.counts[b];
     if (mine == 0 && b != r.batch - 1) return;
     int before = 0;
@@ -239,23 +195,23 @@ __global__ void __launch_bounds__(kThreads) release_rows_kernel(Release r) {
     if (b == r.batch - 1 && threadIdx.x == 0) *r.p.count = min(at + mine, r.p.pages);
     if (mine == 0) return;
     int32_t* row = r.table + b * r.table_row;
-    for (int first = r.kept(b); first < r.width; first += kRows * kThreads) {
-        int x[kRows];
-        uint64_t back[kRows];
+    for (int first = r.kept(b); first < r.width; first += kTurns * kThreads) {
+        int x[kTurns];
+        uint64_t back[kTurns];
 #pragma unroll
-        for (int u = 0; u < kRows; u++) {
+        for (int u = 0; u < kTurns; u++) {
             const int i = first + u * kThreads + threadIdx.x;
             x[u] = i < r.width ? row[i] : -1;
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kRows; u++) {
+        for (int u = 0; u < kTurns; u++) {
             back[u] = __ballot(r.is_page(x[u]));
             if (lane == 0) found[u][wave] = __popcll(back[u]);
         }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < kRows; u++) {
+        for (int u = 0; u < kTurns; u++) {
             int to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(back[u] >> 32),
                                                     __builtin_amdgcn_mbcnt_lo((uint32_t)back[u], 0));
 #pragma unroll
@@ -291,10 +247,6 @@ bool overlap(const void* a, int64_t bytes, const int32_t* b, int64_t n) {
     return b && n > 0 && bytes > 0 && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)a + bytes;
 }
 
-bool one_launch(int table_width, int batch) {
-    return (int64_t)((table_width + 63) / 64) * batch <= kAllWaves * kPieces;
-}
-
 }  // namespace
 
 extern "C" int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t table_row,
@@ -318,14 +270,14 @@ extern "C" int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t 
             return RANS_EARG;
     const Extend e{*p, __builtin_ctz(p->page_size), table, table_row, table_width, lengths, fresh, seen, batch,
                    (int)tokens, slots, positions, filled, starts, new_lengths};
-    const int64_t blocks = (tokens + kRows * kThreads - 1) / (kRows * kThreads);
-    hipLaunchKernelGGL(extend_kernel, dim3(blocks ? (unsigned)blocks : 1), dim3(kThreads), (size_t)batch * 8, stream, e);
+    const int64_t blocks = (tokens + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL(extend_kernel, dim3(blocks == 0 ? 1 : blocks < kMaxBlocks ? (unsigned)blocks : kMaxBlocks), dim3(kThreads), (size_t)batch * 12, stream, e);
     return (int)hipGetLastError();
 }
 
 extern "C" int64_t vramc_pages_release_workspace(const vramc_pages* p, int table_width, int batch) {
     if (const int rc = check_table(p, table_width, table_width, batch)) return rc;
-    return one_launch(table_width, batch) ? 0 : 4 * ((int64_t)batch + 1);
+    return 4 * ((int64_t)batch + 1);
 }
 
 extern "C" int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t table_row,
@@ -334,16 +286,11 @@ extern "C" int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t
     if (const int rc = check_table(p, table_row, table_width, batch)) return rc;
     if (batch == 0 || table_width == 0) return 0;
     if (!table || !lengths) return RANS_EARG;
-    const int64_t need = vramc_pages_release_workspace(p, table_width, batch);
-    if (need && (!workspace || workspace_bytes < need)) return RANS_EWORKSPACE;
-    if (need && (uintptr_t)workspace % 16) return RANS_EARG;
+    if (!workspace || workspace_bytes < vramc_pages_release_workspace(p, table_width, batch)) return RANS_EWORKSPACE;
+    if ((uintptr_t)workspace % 16) return RANS_EARG;
     auto* counts = static_cast<int32_t*>(workspace);
     const Release r{*p, __builtin_ctz(p->page_size), table, table_row, table_width, lengths, batch, counts,
                     counts + batch};
-    if (!need) {
-        hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kAll), 0, stream, r);
-        return (int)hipGetLastError();
-    }
     hipLaunchKernelGGL(release_count_kernel, dim3((unsigned)batch), dim3(kThreads), 0, stream, r);
     if (const int rc = (int)hipGetLastError()) return rc;
     hipLaunchKernelGGL(release_rows_kernel, dim3((unsigned)batch), dim3(kThreads), 0, stream, r);

@@ -1,10 +1,15 @@
 // RMS norms of queries and keys for each head and their rotation by positions, in
 // one pass, the keys and values into tensors or into the pages of a cache.
 //
-// Every value is read and written once, and HBM bounds it.  A thread takes eight
-// columns of a head, 16 bytes of a 16-bit type, a row of the workgroup's threads
-// one head, so that the norm is a sum over at most 32 lanes.  The columns that its
-// own rotate with are read again, from the caches, by the same thread: no exchange.
+// Every value is read and written once, and HBM bounds it: 32768 tokens of 40 and 8
+// heads of 128 columns, bf16, 159 us, 5.06 TB/s (a large copy reaches 4.8), 16001
+// with their values into pages 98.7 us.  One token of 12 and 2 heads takes 3.3 us.
+//
+// A thread takes eight columns of a head, 16 bytes of a 16-bit type, a row of the
+// workgroup's threads one head, so that the norm is a sum over at most 32 lanes.  The
+// columns that its own rotate with are read again, from the caches, by the same
+// thread: no exchange.  The next row's are under way while a row is turned (163 us
+// without), and queries leave past the caches (168 us through them).
 //
 // A workgroup takes some tokens of one kind (queries, keys or values) with all
 // their heads.  The angles are the same for all heads of a token: one thread makes
@@ -27,7 +32,6 @@ struct Kind {
     int heads;
     bool wide;               // rows can be read 16 bytes at a time
     int shift;               // a workgroup has 2^shift tokens,
-    bool tokens_first;       // neighbouring rows of threads neighbouring tokens (or heads) of them,
     int splits, passes;      // and takes `passes` of the steps of one of `splits`
     uint32_t blocks;
 };
@@ -119,27 +123,38 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a) {
     const int rows = k.heads << k.shift, step = blockDim.y;
     int row = part * k.passes * step + threadIdx.y;
     // the row's token and head, and how far a step goes
-    int t, head, t_step, head_step;
-    if (k.tokens_first) {
-        t = row & ((1 << k.shift) - 1), head = row >> k.shift, t_step = 0, head_step = step >> k.shift;
-    } else {
-        t = row / k.heads, head = row - t * k.heads, t_step = step / k.heads, head_step = step - t_step * k.heads;
-    }
-    for (int i = 0; i < k.passes && row < rows; i++, row += step) {
-        if (t < tokens) {  // lanes beyond the row take part in its sum
+    int t = row / k.heads, head = row - t * k.heads;
+    const int t_step = step / k.heads, head_step = step - t_step * k.heads;
+    const int stop = min(rows, row + k.passes * step);
+    // a row's columns and those that they rotate with, and its place in the cache;
+    // the next row's are under way while a row is turned
+    vec<T, kPer> raw = {}, raw_other = {}, next = {}, next_other = {};
+    int64_t at = -1, next_at = -1;
+    const auto fetch = [&](int t, int head) {
+        if (t >= tokens) return;
+        if (inside) {
             const T* in = static_cast<const T*>(k.x) + (first + t) * k.token + head * k.head;
-            vec<T, kPer> raw = {}, raw_other = {}, y;
-            if (inside) {
-                raw = load(in + column, k.wide);
-                if constexpr (!INTERLEAVED)
-                    if (which < 2) raw_other = load(in + other, k.wide);
-            }
-            int64_t at = -1;
-            if (INTO != kTensor && which > 0) {
-                const int64_t slot = a.slots[first + t];
-                if (slot >= 0 && slot < (int64_t)a.c.pages << a.page_shift)
-                    at = (((slot >> a.page_shift) * a.c.kv_heads + head) << a.page_shift) + (slot & (a.c.page_size - 1));
-            }
+            next = load(in + column, k.wide);
+            if constexpr (!INTERLEAVED)
+                if (which < 2) next_other = load(in + other, k.wide);
+        }
+        if (INTO != kTensor && which > 0) {
+            const int64_t slot = a.slots[first + t];
+            next_at = slot >= 0 && slot < (int64_t)a.c.pages << a.page_shift
+                          ? (((slot >> a.page_shift) * a.c.kv_heads + head) << a.page_shift) + (slot & (a.c.page_size - 1))
+                          : -1;
+        }
+    };
+    if (row < stop) fetch(t, head);
+    while (row < stop) {
+        const int this_t = t, this_head = head;
+        raw = next, raw_other = next_other, at = next_at;
+        row += step;
+        t += t_step, head += head_step;
+        if (head >= k.heads) head -= k.heads, t++;
+        if (row < stop) fetch(t, head);
+        if (this_t < tokens) {  // lanes beyond the row take part in its sum
+            vec<T, kPer> y;
             if (which == 2) {
                 y = raw;
             } else {
@@ -153,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a) {
                     x *= w;
                 }
                 if (turned) {
-                    const float* cs = angles + 2 * t * a.pairs + angle;
+                    const float* cs = angles + 2 * this_t * a.pairs + angle;
                     if constexpr (INTERLEAVED) {
 #pragma unroll
                         for (int j = 0; j < kPer; j += 2) {
@@ -179,21 +194,21 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a) {
             }
             if (!inside) {
             } else if (INTO == kTensor || which == 0) {
-                auto* out = static_cast<Lying<T>*>(k.out) + ((int64_t)(first + t) * k.heads + head) * per_row + seg;
-                *out = __builtin_bit_cast(Lying<T>, y);
+                auto* out = static_cast<Lying<T>*>(k.out) + ((int64_t)(first + this_t) * k.heads + this_head) * per_row + seg;
+                const auto part = __builtin_bit_cast(Lying<T>, y);
+#pragma unroll
+                for (size_t j = 0; j < sizeof(T) / 2; j++) __builtin_nontemporal_store(part.part[j], &out->part[j]);
             } else if constexpr (INTO != kTensor) {
                 if (at >= 0) {  // a block's threads share it
                     store<T, INTO == kMx>(y, which == 1 ? a.c.k : a.c.v, which == 1 ? a.c.k_scale : a.c.v_scale, at,
                                           per_row, seg);
                     if (which == 1 && a.c.mass && seg == 0) {
                         a.c.mass[at] = 0.f;
-                        a.c.position[at] = a.positions[first + t];
+                        a.c.position[at] = a.positions[first + this_t];
                     }
                 }
             }
         }
-        t += t_step, head += head_step;
-        if (!k.tokens_first && head >= k.heads) head -= k.heads, t++;
     }
 }
 
@@ -226,17 +241,18 @@ bool overlap(const void* out, int64_t bytes, const void* x, int64_t token, int64
 }
 
 template <typename T>
-Kind kind_of(const vramc_rotary& r, const void* x, int64_t token, int64_t head, int heads, const void* weight, void* out,
-             int64_t tokens, int lanes, bool pages) {
-    Kind k{x, token, head, weight, out, heads, false, 0, false, 1, 0, 0};
+Kind kind_of(const void* x, int64_t token, int64_t head, int heads, const void* weight, void* out, int64_t tokens,
+             int lanes) {
+    Kind k{x, token, head, weight, out, heads, false, 0, 1, 0, 0};
     if (!heads || !tokens) return k;
     constexpr int64_t size = sizeof(T);
     k.wide = ((uintptr_t)x | (uintptr_t)(token * size) | (uintptr_t)(head * size)) % 16 == 0;
     const int step = kThreads / lanes;
-    if (tokens >= 1024) {
-        if (pages) k.shift = __builtin_ctz(step), k.tokens_first = true;
-        else k.shift = tokens >= 8192 ? 3 : 2;
-    }
+    // Tokens of a workgroup: more share less of the angles and end later.  40 and 8 heads
+    // of 128 columns, bf16: 512 tokens 6.7 us by two and 6.4 by one with its heads dealt
+    // to several workgroups, 1000 8.4 and 11.0; 2048 12.0 by two and 12.7 by four, 4096
+    // 20.5 and 18.6, 32768 175 and 159 (by eight 161).
+    k.shift = tokens >= 4096 ? 2 : tokens >= 512 ? 1 : 0;
     const int steps = ((heads << k.shift) + step - 1) / step;
     k.splits = k.shift ? 1 : steps;
     k.passes = k.shift ? steps : 1;
@@ -250,9 +266,9 @@ int launch(const vramc_rotary& r, const vramc_rotary_rows& x, const vramc_kv_cac
     const int lanes = r.head_dim <= 64 ? 8 : r.head_dim <= 128 ? 16 : 32;
     constexpr bool pages = INTO != kTensor;
     Rotate a{};
-    a.kind[0] = kind_of<T>(r, x.q, x.q_token, x.q_head, x.q_heads, x.q_weight, q_out, x.tokens, lanes, false);
-    a.kind[1] = kind_of<T>(r, x.k, x.k_token, x.k_head, x.k_heads, x.k_weight, k_out, x.tokens, lanes, pages);
-    a.kind[2] = kind_of<T>(r, v, v_token, v_head, pages ? x.k_heads : 0, nullptr, nullptr, x.tokens, lanes, pages);
+    a.kind[0] = kind_of<T>(x.q, x.q_token, x.q_head, x.q_heads, x.q_weight, q_out, x.tokens, lanes);
+    a.kind[1] = kind_of<T>(x.k, x.k_token, x.k_head, x.k_heads, x.k_weight, k_out, x.tokens, lanes);
+    a.kind[2] = kind_of<T>(v, v_token, v_head, pages ? x.k_heads : 0, nullptr, nullptr, x.tokens, lanes);
     a.turns = r.turns, a.pairs = r.pairs, a.dim = r.head_dim, a.lanes = lanes;
     a.amplitude = r.amplitude, a.eps = x.eps, a.weight_f32 = x.weight_dtype == RANS_X_F32;
     a.positions = x.positions, a.tokens = (int)x.tokens;

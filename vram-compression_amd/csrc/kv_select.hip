@@ -1,16 +1,17 @@
 // Which pages of a sequence a query attends to: the smallest and largest key of each
 // column of a page bound its scores, and those that can give the largest are taken.
 //
-// bound reads all keys of the pages once, and HBM bounds it.  A wave takes a page of
-// a head; values are compared as whole numbers that sort as they do, two of 16 bits
-// an instruction.
+// bound reads all keys of the pages once, and HBM bounds it: 2048 pages of 64 keys of 8
+// heads of 128 columns 48.6 us, 5.7 TB/s of reads.  A wave takes a page of a head;
+// values are compared as whole numbers that sort as they do, two of 16 bits an
+// instruction.
 //
-// select reads two rows a page and head, q_d lo_d or q_d hi_d being q_d mid_d +
-// |q_d| half_d whatever the sign: two multiply-adds a column and query head, in 64
-// bits, which MI355X makes at the rate of 32, so that which page is taken does not
-// depend on an order of sums.  A second launch, a workgroup to a kv head of a
-// sequence, finds the border by radix over the scores' bits, from the highest in
-// which they differ, and writes the pages in their order by counts of ballot bits.
+// select scores in 64 bits, so that which page is taken does not depend on an order of
+// sums.  That rate bounds it: 16 sequences of 512 pages of 8 heads, 5 query heads each,
+// 17 us where their bounds are read in 6.  A second launch, a workgroup to a kv head of
+// a sequence, finds the border by radix over the scores' bits, from the highest in
+// which they differ, and writes the pages in their order by counts of ballot bits (5
+// to 7 us: reads, three digits, lists, one after the other).
 #include "kv_device.h"
 
 #include <limits>
@@ -21,8 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 
 // ------------------------------------------------------------------ bounds
-constexpr int kEntries = 16;  // of the list, to a workgroup
-constexpr int kAhead = 8;     // loads of a wave under way
+constexpr int kManyEntries = 1 << 16;
 
 struct Bound {
     vramc_kv_cache c;
@@ -30,6 +30,7 @@ struct Bound {
     const int32_t* pages;
     int64_t n;
     void* bounds;
+    int each;                 // entries of the list to a wave
 };
 
 // Values as whole numbers that sort alike, and back: the bits below the sign are
@@ -53,7 +54,11 @@ struct Columns {
             codes = static_cast<const uint32_t*>(c.k)[row * per_row + seg];
             scale = c.k_scale[row * (per_row / 4) + seg / 4];
         } else {
-            x = static_cast<const Lying<T>*>(c.k)[row * per_row + seg];
+            // past the caches, as nobody reads them next: 2048 pages of 64 keys of 8 heads
+            // of 128 columns 48.6 us against 55.6
+            const auto* from = static_cast<const Lying<T>*>(c.k) + row * per_row + seg;
+#pragma unroll
+            for (size_t i = 0; i < sizeof(T) / 2; i++) x.part[i] = __builtin_nontemporal_load(&from->part[i]);
         }
     }
     __device__ __forceinline__ Whole whole() const {
@@ -77,7 +82,8 @@ __device__ __forceinline__ V shuffled(V x, int d) {
     return __builtin_bit_cast(V, w);
 }
 
-template <typename T, bool MX>
+// AHEAD: loads of a wave under way, of which a page's steps are a multiple.
+template <typename T, bool MX, int AHEAD>
 __global__ void __launch_bounds__(kThreads) bound_kernel(Bound a) {
     using C = Columns<T, MX>;
     using Whole = typename C::Whole;
@@ -87,25 +93,24 @@ __global__ void __launch_bounds__(kThreads) bound_kernel(Bound a) {
     const int per_row = a.c.head_dim / kPer, seg = lane & (a.lanes - 1), in_step = 64 / a.lanes;
     const int steps = a.c.page_size / in_step, first = lane / a.lanes;
     const bool inside = seg < per_row;
-    for (int e = 0; e < kEntries / kWaves; e++) {
-        const int64_t i = (int64_t)chunk * kEntries + e * kWaves + wave;
+    for (int e = 0; e < a.each; e++) {
+        const int64_t i = ((int64_t)chunk * a.each + e) * kWaves + wave;
         const int page = i < a.n ? a.pages[i] : -1;
         if (page < 0 || page >= a.c.pages) continue;
         const int64_t at = (int64_t)page * a.c.kv_heads + head, row = (at << a.page_shift) + first;
         Whole low = std::numeric_limits<typename C::Int>::max(), high = std::numeric_limits<typename C::Int>::min();
-        for (int s = 0; s < steps; s += kAhead) {
-            C x[kAhead];
+        if (inside)
+            for (int s = 0; s < steps; s += AHEAD) {
+                C x[AHEAD];
 #pragma unroll
-            for (int u = 0; u < kAhead; u++)  // beyond the last step the last again
-                if (inside) x[u].load(a.c, row + (int64_t)min(s + u, steps - 1) * in_step, per_row, seg);
+                for (int u = 0; u < AHEAD; u++) x[u].load(a.c, row + (int64_t)(s + u) * in_step, per_row, seg);
 #pragma unroll
-            for (int u = 0; u < kAhead; u++)
-                if (inside) {
+                for (int u = 0; u < AHEAD; u++) {
                     const Whole y = x[u].whole();
                     low = __builtin_elementwise_min(low, y);
                     high = __builtin_elementwise_max(high, y);
                 }
-        }
+            }
         for (int d = a.lanes; d < 64; d *= 2) {
             low = __builtin_elementwise_min(low, shuffled(low, d));
             high = __builtin_elementwise_max(high, shuffled(high, d));
@@ -120,15 +125,19 @@ __global__ void __launch_bounds__(kThreads) bound_kernel(Bound a) {
 }
 
 // ------------------------------------------------------------------ scores
-constexpr int kSets = 2;          // of pages that a wave scores at once, a page to each row of lanes
-constexpr int kHeads = 16;        // query heads in LDS at once
+// Query heads that vectors score; more the matrix cores, which take 16 as long as one.
+// Both launches of 16 sequences of 512 pages, 8 heads of 128 columns: 16.9 us by vectors
+// and 26.2 by matrices with one query head each, 23.3 and 26.6 with 5, 27.9 and 27.2 with
+// 8, 41.1 and 29.5 with 16; heads of 64 columns meet at 8 too, of 256 beyond it.
+constexpr int kFewHeads = 8;
+constexpr int kSets = 2;          // of pages that a wave of vectors scores at once, a page to each row of lanes
 constexpr int kMaxDim = 256;
 
 struct Select {
     const void* bounds;
     const void* q;
     int64_t q_seq, q_head;
-    int group, heads, dim, lanes, pages, page_shift;
+    int group, heads, pages, page_shift;
     const int32_t* table;
     int64_t table_row;
     int width;
@@ -151,6 +160,27 @@ __device__ __forceinline__ double wide(T x) {
     return (double)(float)x;
 }
 
+// The largest over 16 lanes.
+__device__ __forceinline__ double row_max(double x) {
+    const auto step = [&](auto control) {
+        auto w = __builtin_bit_cast(vec<int, 2>, x);
+#pragma unroll
+        for (int i = 0; i < 2; i++) w[i] = __builtin_amdgcn_update_dpp(0, w[i], control(), 0xf, 0xf, true);
+        x = fmax(x, __builtin_bit_cast(double, w));
+    };
+    step([] { return 0xb1; });   // quad_perm:[1,0,3,2]
+    step([] { return 0x4e; });   // quad_perm:[2,3,0,1]
+    step([] { return 0x141; });  // row_half_mirror
+    step([] { return 0x140; });  // row_mirror
+    return x;
+}
+
+// A page's score as a whole number that sorts alike; 0, below all, for no page.
+__device__ __forceinline__ uint64_t key_of(double score, int page) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, score + 0.0);  // -0 as 0
+    return page < 0 ? 0 : bits >> 63 ? ~bits : bits | 1ull << 63;
+}
+
 // The sum over the lanes of a row, 8 to 32.
 __device__ __forceinline__ double row_sum(double x, int lanes) {
     const auto add = [&](auto control) {
@@ -167,227 +197,316 @@ __device__ __forceinline__ double row_sum(double x, int lanes) {
     return x;
 }
 
+// Few query heads: a wave scores two pages on each row of its lanes, eight columns a
+// lane.  q_d lo_d or q_d hi_d is q_d (hi_d + lo_d) / 2 + |q_d| (hi_d - lo_d) / 2
+// whatever the sign: two multiply-adds a column and query head.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_kernel(Select a) {
-    __shared__ __attribute__((aligned(16))) double query[kHeads * kMaxDim];  // [head][pair of eight][lane][2]
+__global__ void __launch_bounds__(kThreads) score_few_kernel(Select a, int dim, int lanes) {
+    __shared__ __attribute__((aligned(16))) double query[kFewHeads * kMaxDim];  // halves, [head][pair of eight][lane][2]
     const int group_of = blockIdx.x / a.chunks, chunk = blockIdx.x - group_of * a.chunks;
     const int b = group_of / a.heads, h = group_of - b * a.heads;
-    const int n = a.pages_of(a.length_of(b));
-    const int in_set = 64 / a.lanes, start = chunk * (kWaves * kSets * in_set);
-    if (n <= a.count || start >= n) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int per_row = a.dim / kPer, seg = lane & (a.lanes - 1);
+    const int per_row = dim / kPer, seg = lane & (lanes - 1), in_set = 64 / lanes;
     const bool inside = seg < per_row;
-    int index[kSets], page[kSets];
+    const T* q = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)h * a.group * a.q_head;
+    // the first pages' numbers, while it is not known whether there are as many
+    const int first = (chunk * kWaves + wave) * kSets * in_set + lane / lanes;
+    int page[kSets];
+#pragma unroll
+    for (int s = 0; s < kSets; s++) page[s] = a.page(b, min(first + s * in_set, a.width - 1));
+    const int n = a.pages_of(a.length_of(b));
+    if (n <= a.count || chunk * kWaves * kSets * in_set >= n) return;
     Lying<T> raw[kSets][2];
 #pragma unroll
     for (int s = 0; s < kSets; s++) {
-        index[s] = start + (wave * kSets + s) * in_set + lane / a.lanes;
-        page[s] = index[s] < n ? a.page(b, index[s]) : -1;
-    }
+        const auto* from = static_cast<const Lying<T>*>(a.bounds) +
+                           2 * ((int64_t)max(page[s], 0) * a.heads + h) * per_row + (inside ? seg : 0);
 #pragma unroll
-    for (int s = 0; s < kSets; s++) {
-        const auto* from = static_cast<const Lying<T>*>(a.bounds) + 2 * ((int64_t)max(page[s], 0) * a.heads + h) * per_row + seg;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (inside) raw[s][i] = from[i * per_row];
-            else raw[s][i] = {};
+        for (int i = 0; i < 2; i++) raw[s][i] = from[i * per_row];
     }
-    double middle[kSets][kPer], half[kSets][kPer], best[kSets];
+    for (int i = threadIdx.x; i < a.group * dim; i += kThreads) {
+        const int g = i / dim, d = i - g * dim;
+        query[((g * (kPer / 2) + d % kPer / 2) * per_row + d / kPer) * 2 + d % 2] = 0.5 * wide(q[g * a.q_head + d]);
+    }
+    __syncthreads();
+    double sum[kSets][kPer], gap[kSets][kPer], best[kSets];
 #pragma unroll
     for (int s = 0; s < kSets; s++) {
         const auto low = __builtin_bit_cast(vec<T, kPer>, raw[s][0]), high = __builtin_bit_cast(vec<T, kPer>, raw[s][1]);
 #pragma unroll
         for (int j = 0; j < kPer; j++) {
-            middle[s][j] = 0.5 * (wide(high[j]) + wide(low[j]));
-            half[s][j] = 0.5 * (wide(high[j]) - wide(low[j]));
+            sum[s][j] = wide(high[j]) + wide(low[j]);
+            gap[s][j] = wide(high[j]) - wide(low[j]);
         }
         best[s] = -__builtin_inf();
     }
-    const int at = seg < per_row ? seg : 0;
-    for (int g0 = 0; g0 < a.group; g0 += kHeads) {
-        const int heads = min(kHeads, a.group - g0);
-        const T* q = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)(h * a.group + g0) * a.q_head;
-        if (g0) __syncthreads();
-        for (int i = threadIdx.x; i < heads * a.dim; i += kThreads) {
-            const int g = i / a.dim, d = i - g * a.dim;
-            query[((g * (kPer / 2) + d % kPer / 2) * per_row + d / kPer) * 2 + d % 2] = wide(q[g * a.q_head + d]);
+    const int at = inside ? seg : 0;
+#pragma unroll 1
+    for (int g = 0; g < a.group; g++) {
+        double x[kSets] = {}, y[kSets] = {};
+#pragma unroll
+        for (int p = 0; p < kPer / 2; p++) {
+            const auto v = *reinterpret_cast<const vec<double, 2>*>(query + ((g * (kPer / 2) + p) * per_row + at) * 2);
+#pragma unroll
+            for (int s = 0; s < kSets; s++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    x[s] = __builtin_fma(v[i], sum[s][2 * p + i], x[s]);
+                    y[s] = __builtin_fma(__builtin_fabs(v[i]), gap[s][2 * p + i], y[s]);
+                }
         }
-        __syncthreads();
-        for (int g = 0; g < heads; g++) {
-            double x[kSets] = {}, y[kSets] = {};
 #pragma unroll
-            for (int p = 0; p < kPer / 2; p++) {
-                const auto v = *reinterpret_cast<const vec<double, 2>*>(query + ((g * (kPer / 2) + p) * per_row + at) * 2);
-#pragma unroll
-                for (int s = 0; s < kSets; s++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        x[s] = __builtin_fma(v[i], middle[s][2 * p + i], x[s]);
-                        y[s] = __builtin_fma(__builtin_fabs(v[i]), half[s][2 * p + i], y[s]);
-                    }
-            }
-#pragma unroll
-            for (int s = 0; s < kSets; s++) {
-                const double score = row_sum(inside ? x[s] + y[s] : 0.0, a.lanes);
-                best[s] = score != score ? __builtin_inf() : fmax(best[s], score);
-            }
+        for (int s = 0; s < kSets; s++) {
+            const double score = row_sum(inside ? x[s] + y[s] : 0.0, lanes);
+            best[s] = score != score ? __builtin_inf() : fmax(best[s], score);
         }
     }
 #pragma unroll
     for (int s = 0; s < kSets; s++)
-        if (seg == 0 && index[s] < n) {  // 0 for no page: below all scores
-            const uint64_t bits = __builtin_bit_cast(uint64_t, best[s] + 0.0);  // -0 as 0
-            const uint64_t key = bits >> 63 ? ~bits : bits | 1ull << 63;
-            a.keys[(int64_t)group_of * a.width + index[s]] = page[s] < 0 ? 0 : key;
+        if (seg == 0 && first + s * in_set < n) a.keys[(int64_t)group_of * a.width + first + s * in_set] = key_of(best[s], page[s]);
+}
+
+// A wave scores 16 pages with 16 query heads: lane (n = lane % 16, g = lane / 16)
+// holds a quarter of the columns of page n's bounds, and reads those of head n from
+// LDS.  Which columns a product takes from each quarter does not matter, as long as
+// both sides take the same.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) score_kernel(Select a) {
+    constexpr int QUARTER = D / 4, LOADS = QUARTER / kPer;
+    __shared__ double query[D * 16];  // [column of a quarter][quarter][head]
+    const int group_of = blockIdx.x / a.chunks, chunk = blockIdx.x - group_of * a.chunks;
+    const int b = group_of / a.heads, h = group_of - b * a.heads;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+    const T* q = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)h * a.group * a.q_head;
+    const auto stage = [&](int first) {  // zeros for heads that there are not
+        for (int i = threadIdx.x; i < 16 * D; i += kThreads) {
+            const int head = i / D, d = i % D;
+            query[(d % QUARTER * 4 + d / QUARTER) * 16 + head] =
+                first + head < a.group ? wide(q[(first + head) * a.q_head + d]) : 0.0;
         }
+    };
+    // the page's number and its bounds, while it is not known whether there are as many
+    const int first = (chunk * kWaves + wave) * 16, page = a.page(b, min(first + (lane & 15), a.width - 1));
+    const int n = a.pages_of(a.length_of(b));
+    if (n <= a.count || chunk * kWaves * 16 >= n) return;
+    Lying<T> low[LOADS], high[LOADS];
+    const auto* from = static_cast<const Lying<T>*>(a.bounds) + ((int64_t)max(page, 0) * a.heads + h) * (2 * D / kPer) + g * LOADS;
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) low[i] = from[i], high[i] = from[D / kPer + i];
+    double best[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) best[e] = -__builtin_inf();
+    for (int g0 = 0; g0 < a.group; g0 += 16) {
+        if (g0) __syncthreads();
+        stage(g0);
+        __syncthreads();
+        vec<double, 4> score = {};
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const auto x = __builtin_bit_cast(vec<T, kPer>, low[i]), y = __builtin_bit_cast(vec<T, kPer>, high[i]);
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                const double v = query[(i * kPer + j) * 64 + lane];
+                score = __builtin_amdgcn_mfma_f64_16x16x4f64(wide(x[j]), v < 0 ? v : 0.0, score, 0, 0, 0);
+                score = __builtin_amdgcn_mfma_f64_16x16x4f64(wide(y[j]), v < 0 ? 0.0 : v, score, 0, 0, 0);
+            }
+        }
+        const bool live = g0 + (lane & 15) < a.group;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // of page 4e + g
+            const double s = score[e] != score[e] ? __builtin_inf() : score[e];
+            best[e] = fmax(best[e], row_max(live ? s : -__builtin_inf()));
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int in = 4 * e + g;
+        const int its = __shfl(page, in);
+        if ((lane & 15) == e && first + in < n) a.keys[(int64_t)group_of * a.width + first + in] = key_of(best[e], its);
+    }
 }
 
 // ------------------------------------------------------------------ choice
+// Loops stay loops here: a workgroup waits for every line of its code (7.6 us with the
+// keys in registers and everything unrolled, 6.0 so).
 constexpr int kChoose = 512;                // threads
 constexpr int kChooseWaves = kChoose / 64;
-constexpr int kKeys = 16;                   // keys of a thread
-constexpr int kPiece = kChoose * kKeys;
-constexpr int kDigit = 10, kBins = 1 << kDigit;
+constexpr int kPiece = 4096;                // keys in LDS at once
+constexpr int kParts = kPiece / 64;         // of a wave's width
+constexpr int kDigit = 10, kBins = 1 << kDigit, kLaneBins = kBins / 64;
 
 __device__ __forceinline__ uint64_t from_bit(uint64_t x, int bit) { return bit < 64 ? x >> bit : 0; }
 
 __global__ void __launch_bounds__(kChoose) choose_kernel(Select a) {
-    __shared__ int hist[kBins], found[3], waves[kChooseWaves];
-    __shared__ uint64_t ends[2][kChooseWaves];
-    __shared__ uint32_t counts[kKeys * kChooseWaves];  // above the border | at it << 16
-    __shared__ uint32_t sums[kKeys * kChooseWaves];
+    __shared__ uint64_t key[kPiece];
+    __shared__ int32_t page[kPiece];
+    // Every wave goes over the whole of what all have counted: one barrier a digit.
+    __shared__ __attribute__((aligned(16))) int hist[3][kBins];  // this digit's, the last one's, the next one's
+    __shared__ uint32_t ends[2][kChooseWaves];
+    __shared__ uint32_t counts[kParts];  // above the border | at it << 16
     const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tokens = a.length_of(b), n = a.pages_of(tokens), kept = min(n, a.count);
     int32_t* out = a.chosen + (int64_t)blockIdx.x * a.count;
     const auto entry = [&](int i) {
         const int page = a.page(b, i);
         return page < 0 ? -1 : page * a.heads + h;
     };
+    const uint64_t* keys = a.keys + (int64_t)blockIdx.x * a.width + a.first;
+    const auto load = [&](int piece, int size) {  // a thread reads what it wrote
+#pragma unroll 2
+        for (int i = threadIdx.x; i < size; i += kChoose) {
+            const uint64_t x = keys[piece * kPiece + i];
+            const int32_t y = entry(a.first + piece * kPiece + i);
+            key[i] = x, page[i] = y;
+        }
+    };
+    // the first keys, while it is not known how many there are
+    if (a.width > a.count) load(0, min(a.width - a.first, kPiece));
+    const int tokens = a.length_of(b), n = a.pages_of(tokens), kept = min(n, a.count);
     if (threadIdx.x == 0) a.held[blockIdx.x] = kept ? tokens - ((n - kept) << a.page_shift) : 0;
-    for (int i = kept + threadIdx.x; i < a.count; i += kChoose) out[i] = -1;
-    if (n <= a.count) {
-        for (int i = threadIdx.x; i < n; i += kChoose) out[i] = entry(i);
-        return;
-    }
-    for (int i = threadIdx.x; i < a.first; i += kChoose) out[i] = entry(i);
-    for (int i = threadIdx.x; i < a.last; i += kChoose) out[a.count - a.last + i] = entry(n - a.last + i);
+    // the pages at the ends, or all of them, and what is behind them
+    const int left = n <= a.count ? n : a.first, right = n <= a.count ? 0 : a.last;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < a.count; i += kChoose)
+        if (i < left || i >= a.count - right || i >= kept)
+            out[i] = i < left ? entry(i) : i >= kept ? -1 : entry(n - a.count + i);
     const int among = n - a.first - a.last;      // candidates,
     int room = a.count - a.first - a.last;       // of which so many are taken
-    if (room == 0) return;
-    const uint64_t* keys = a.keys + (int64_t)blockIdx.x * a.width + a.first;
+    if (n <= a.count || room == 0) return;
     const int pieces = (among + kPiece - 1) / kPiece;
-    uint64_t key[kKeys];
-    const auto there = [&](int piece, int u) { return piece * kPiece + u * kChoose + (int)threadIdx.x < among; };
-    const auto load = [&](int piece) {
-#pragma unroll
-        for (int u = 0; u < kKeys; u++)
-            if (there(piece, u)) key[u] = keys[piece * kPiece + u * kChoose + threadIdx.x];
-    };
-    // f(u, key, whether it is one) over a piece's keys, the same for all threads of a wave
-    const auto over = [&](int piece, auto f) {
-#pragma unroll
-        for (int u = 0; u < kKeys; u++)
-            if (piece * kPiece + u * kChoose < among) f(u, key[u], there(piece, u));
-    };
-    // the highest bit in which keys differ
-    uint64_t least = ~0ull, most = 0;
+    const auto size_of = [&](int piece) { return min(among - piece * kPiece, kPiece); };
+    for (int i = threadIdx.x; i < 3 * kBins; i += kChoose) (&hist[0][0])[i] = 0;
+    // the highest of the upper 32 bits in which keys differ, or the 32nd
+    uint32_t least = ~0u, most = 0;
+#pragma unroll 1
     for (int piece = 0; piece < pieces; piece++) {
-        load(piece);
-        over(piece, [&](int, uint64_t k, bool is) {
-            if (is) least = min(least, k), most = max(most, k);
-        });
+        if (piece) load(piece, size_of(piece));
+#pragma unroll 1
+        for (int i = threadIdx.x; i < size_of(piece); i += kChoose) {
+            const uint32_t x = (uint32_t)(key[i] >> 32);
+            least = min(least, x), most = max(most, x);
+        }
     }
 #pragma unroll
     for (int d = 32; d; d /= 2) {
-        least = min(least, (uint64_t)__shfl_xor((unsigned long long)least, d));
-        most = max(most, (uint64_t)__shfl_xor((unsigned long long)most, d));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d));
+        most = max(most, (uint32_t)__shfl_xor((int)most, d));
     }
     if (lane == 0) ends[0][wave] = least, ends[1][wave] = most;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kChooseWaves; w++) least = min(least, ends[0][w]), most = max(most, ends[1][w]);
-    int bit = least == most ? 0 : 64 - __builtin_clzll(least ^ most);
-    uint64_t above = from_bit(most, bit);  // what the border's keys have from that bit on
-    int at = among;                        // how many keys have it
-    while (bit > 0 && at > room) {
+    int bit = least == most ? 32 : 64 - __builtin_clz(least ^ most);
+    uint64_t above = bit < 64 ? (uint64_t)most >> (bit - 32) : 0;  // what the border's keys have from that bit on
+    int at = among;                                                // how many keys have it
+#pragma unroll 1
+    for (int turn = 0; bit > 0 && at > room; turn = turn == 2 ? 0 : turn + 1) {
         const int digit = min(bit, kDigit), low = bit - digit, bins = 1 << digit;
-        for (int i = threadIdx.x; i < kBins; i += kChoose) hist[i] = 0;
-        __syncthreads();
+#pragma unroll 1
         for (int piece = 0; piece < pieces; piece++) {
-            if (pieces > 1) load(piece);
-            over(piece, [&](int, uint64_t k, bool is) {
-                if (is && from_bit(k, bit) == above) atomicAdd(&hist[k >> low & (bins - 1)], 1);
-            });
+            if (pieces > 1) load(piece, size_of(piece));
+#pragma unroll 1
+            for (int i = threadIdx.x; i < size_of(piece); i += kChoose) {
+                const uint64_t x = key[i];
+                if (from_bit(x, bit) == above) atomicAdd(&hist[turn][x >> low & (bins - 1)], 1);
+            }
         }
         __syncthreads();
-        // from the top, two bins to a thread
-        const int top = bins - 1 - 2 * (int)threadIdx.x;
-        const int x = top >= 0 ? hist[top] : 0, y = top >= 1 ? hist[top - 1] : 0, both = wave_scan(x + y);
-        if (lane == 63) waves[wave] = both;
-        __syncthreads();
-        int before = both - x - y;
+        // the last digit's bins, which all have read now, for the digit behind the next
+        for (int i = threadIdx.x; i < kBins; i += kChoose) hist[turn == 0 ? 2 : turn - 1][i] = 0;
+        // the bin that holds the room-th from the top, 16 neighbouring bins to a lane
+        int x[kLaneBins], sum = 0;
 #pragma unroll
-        for (int w = 0; w < kChooseWaves; w++) before += w < wave ? waves[w] : 0;
-        if (before < room && before + x + y >= room) {
-            const bool second = before + x < room;
-            found[0] = second ? top - 1 : top;
-            found[1] = second ? before + x : before;
-            found[2] = second ? y : x;
+        for (int i = 0; i < kLaneBins; i += 4) {
+            const auto y = *reinterpret_cast<const vec<int, 4>*>(&hist[turn][(63 - lane) * kLaneBins + i]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum += x[i + j] = y[j];
         }
-        __syncthreads();
-        above = above << digit | (uint64_t)found[0];
-        room -= found[1];
-        at = found[2];
+        int before = wave_scan(sum) - sum;
+        const int owner = __builtin_ctzll(__ballot(before < room && before + sum >= room));
+        int bin = 0, count = 0;
+        bool found = false;
+#pragma unroll
+        for (int i = kLaneBins - 1; i >= 0; i--) {
+            const bool it = !found && before + x[i] >= room;
+            if (it) bin = (63 - lane) * kLaneBins + i, count = x[i];
+            found |= it;
+            if (!found) before += x[i];
+        }
+        bin = __builtin_amdgcn_readlane(bin, owner);
+        room -= __builtin_amdgcn_readlane(before, owner);
+        at = __builtin_amdgcn_readlane(count, owner);
+        above = above << digit | (uint64_t)bin;
         bit = low;
     }
     // those above the border, and the first `room` of those at it, in their order
-    uint32_t taken = 0;  // of the pieces before, packed alike
-    uint32_t equal = 0;
+    uint32_t taken = 0, equal = 0;  // of the pieces before
+#pragma unroll 1
     for (int piece = 0; piece < pieces; piece++) {
-        if (pieces > 1) load(piece);
-        __syncthreads();
-        over(piece, [&](int u, uint64_t k, bool is) {
-            const uint64_t x = from_bit(k, bit);
-            const uint32_t more = __popcll(__ballot(is && x > above)), same = __popcll(__ballot(is && x == above));
-            if (lane == 0) counts[u * kChooseWaves + wave] = more | same << 16;
-        });
-        __syncthreads();
-        const int parts = min(kKeys, (among - piece * kPiece + kChoose - 1) / kChoose) * kChooseWaves;
-        if (wave == 0) {  // two of them to a lane
-            const uint32_t x = 2 * lane < parts ? counts[2 * lane] : 0, y = 2 * lane + 1 < parts ? counts[2 * lane + 1] : 0;
-            const uint32_t sum = (uint32_t)wave_scan((int)(x + y));
-            sums[2 * lane] = sum - y;
-            sums[2 * lane + 1] = sum;
+        const int size = size_of(piece), parts = (size + 63) / 64;
+        if (pieces > 1) {
+            load(piece, size_of(piece));
+            __syncthreads();  // the last piece's counts have been read
+        }
+#pragma unroll 1
+        for (int i = threadIdx.x; i - lane < size; i += kChoose) {
+            const uint64_t x = i < size ? from_bit(key[i], bit) : 0;
+            const uint32_t more = __popcll(__ballot(i < size && x > above)), same = __popcll(__ballot(i < size && x == above));
+            if (lane == 0) counts[i / 64] = more | same << 16;
         }
         __syncthreads();
-        over(piece, [&](int u, uint64_t k, bool is) {
-            const uint64_t x = from_bit(k, bit);
-            const uint64_t more = __ballot(is && x > above), same = __ballot(is && x == above);
-            const int i = u * kChooseWaves + wave;
-            const uint32_t before = sums[i] - counts[i];
+        const uint32_t mine = lane < parts ? counts[lane] : 0, sum = (uint32_t)wave_scan((int)mine);
+#pragma unroll 1
+        for (int i = threadIdx.x; i - lane < size; i += kChoose) {
+            const uint64_t x = i < size ? from_bit(key[i], bit) : 0;
+            const uint64_t more = __ballot(i < size && x > above), same = __ballot(i < size && x == above);
+            const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(sum - mine), (i - lane) / 64);
             const auto below = [&](uint64_t mask) {
                 return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
             };
             const uint32_t like = equal + (before >> 16) + below(same);
-            if (is && (x > above || (x == above && like < (uint32_t)room)))
-                out[a.first + taken + (before & 0xffff) + below(more) + min(like, (uint32_t)room)] =
-                    entry(a.first + piece * kPiece + u * kChoose + threadIdx.x);
-        });
-        const uint32_t last = sums[parts - 1];
-        taken += last & 0xffff;
-        equal += last >> 16;
+            if (i < size && (x > above || (x == above && like < (uint32_t)room)))
+                out[a.first + taken + (before & 0xffff) + below(more) + min(like, (uint32_t)room)] = page[i];
+        }
+        const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        taken += all & 0xffff;
+        equal += all >> 16;
     }
 }
 
 int lanes_of(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
 
+// Workgroups that score a row of the table.
+int64_t chunks_of(int dim, int group, int table_width) {
+    const int pages = group <= kFewHeads ? kWaves * kSets * 64 / lanes_of(dim) : kWaves * 16;
+    return (table_width + pages - 1) / pages;
+}
+
+template <typename T>
+void score(const Select& a, int dim, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.chunks)), block(kThreads);
+    if (a.group <= kFewHeads) {
+        hipLaunchKernelGGL((score_few_kernel<T>), grid, block, 0, stream, a, dim, lanes_of(dim));
+        return;
+    }
+    switch (dim) {
+        case 64: hipLaunchKernelGGL((score_kernel<T, 64>), grid, block, 0, stream, a); break;
+        case 96: hipLaunchKernelGGL((score_kernel<T, 96>), grid, block, 0, stream, a); break;
+        case 128: hipLaunchKernelGGL((score_kernel<T, 128>), grid, block, 0, stream, a); break;
+        case 192: hipLaunchKernelGGL((score_kernel<T, 192>), grid, block, 0, stream, a); break;
+        default: hipLaunchKernelGGL((score_kernel<T, 256>), grid, block, 0, stream, a);
+    }
+}
+
 template <typename T, bool MX>
 int bound(const Bound& a, hipStream_t stream) {
-    const int64_t blocks = (a.n + kEntries - 1) / kEntries * a.c.kv_heads;
+    const int64_t blocks = (a.n + kWaves * a.each - 1) / (kWaves * a.each) * a.c.kv_heads;
     if (blocks > kMaxThreads / kThreads) return RANS_EARG;
-    hipLaunchKernelGGL((bound_kernel<T, MX>), dim3((unsigned)blocks), dim3(kThreads), 0, stream, a);
+    const dim3 grid((unsigned)blocks), block(kThreads);
+    const int steps = a.c.page_size * a.lanes / 64;
+    if (steps >= 8) hipLaunchKernelGGL((bound_kernel<T, MX, 8>), grid, block, 0, stream, a);
+    else if (steps == 4) hipLaunchKernelGGL((bound_kernel<T, MX, 4>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((bound_kernel<T, MX, 2>), grid, block, 0, stream, a);
     return (int)hipGetLastError();
 }
 
@@ -399,7 +518,8 @@ extern "C" int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int
     if (n < 0 || n > INT64_MAX / 65536) return RANS_EARG;
     if (n == 0) return 0;
     if (!pages || !bounds || (uintptr_t)bounds % 16) return RANS_EARG;
-    const Bound a{*c, __builtin_ctz(c->page_size), lanes_of(c->head_dim), pages, n, bounds};
+    const Bound a{*c, __builtin_ctz(c->page_size), lanes_of(c->head_dim), pages, n, bounds,
+                  n * c->kv_heads > kManyEntries ? 4 : 1};
     if (c->dtype == RANS_X_F32) return bound<float, false>(a, stream);
     if (c->dtype == RANS_X_BF16) return c->mx ? bound<__bf16, true>(a, stream) : bound<__bf16, false>(a, stream);
     return c->mx ? bound<_Float16, true>(a, stream) : bound<_Float16, false>(a, stream);
@@ -412,9 +532,8 @@ extern "C" int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int table_
         (int64_t)c->pages * c->kv_heads > INT32_MAX)
         return RANS_EARG;
     if (table_width <= count) return 0;
-    const int in_block = kWaves * kSets * 64 / lanes_of(c->head_dim);
-    const int64_t chunks = (table_width + in_block - 1) / in_block, rows = (int64_t)batch * c->kv_heads;
-    if (chunks * rows > kMaxThreads / kThreads) return RANS_EARG;
+    const int64_t rows = (int64_t)batch * c->kv_heads;
+    if (chunks_of(c->head_dim, 1, table_width) * rows > kMaxThreads / kThreads) return RANS_EARG;  // the most
     return rows * table_width * 8;
 }
 
@@ -431,18 +550,15 @@ extern "C" int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, cons
         return RANS_EARG;
     if (need && (!workspace || workspace_bytes < need)) return RANS_EWORKSPACE;
     if (need && (uintptr_t)workspace % 16) return RANS_EARG;
-    const int lanes = lanes_of(c->head_dim), in_block = kWaves * kSets * 64 / lanes;
-    const Select a{bounds, q, q_seq, q_head, q_heads / c->kv_heads, c->kv_heads, c->head_dim, lanes, c->pages,
+    const Select a{bounds, q, q_seq, q_head, q_heads / c->kv_heads, c->kv_heads, c->pages,
                    __builtin_ctz(c->page_size), table, table_row, table_width, lengths, batch, count, first, last,
-                   (table_width + in_block - 1) / in_block, static_cast<uint64_t*>(workspace), chosen, held};
-    const int64_t rows = (int64_t)batch * c->kv_heads;
+                   (int)chunks_of(c->head_dim, q_heads / c->kv_heads, table_width), static_cast<uint64_t*>(workspace), chosen, held};
     if (need) {
-        const dim3 grid((unsigned)(rows * a.chunks)), block(kThreads);
-        if (c->dtype == RANS_X_F32) hipLaunchKernelGGL((score_kernel<float>), grid, block, 0, stream, a);
-        else if (c->dtype == RANS_X_BF16) hipLaunchKernelGGL((score_kernel<__bf16>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((score_kernel<_Float16>), grid, block, 0, stream, a);
+        if (c->dtype == RANS_X_F32) score<float>(a, c->head_dim, stream);
+        else if (c->dtype == RANS_X_BF16) score<__bf16>(a, c->head_dim, stream);
+        else score<_Float16>(a, c->head_dim, stream);
         if (const int rc = (int)hipGetLastError()) return rc;
     }
-    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)rows), dim3(kChoose), 0, stream, a);
+    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)(batch * c->kv_heads)), dim3(kChoose), 0, stream, a);
     return (int)hipGetLastError();
 }

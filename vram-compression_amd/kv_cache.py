@@ -423,9 +423,8 @@ class PagedCache(Calls):
         if need < 0:
             raise ValueError(f"{batch} sequences of {self.kv_heads} kv heads over {width} pages: too many "
                              f"({need})")
-        chosen = torch.empty((rows, count), dtype=torch.int32, device=self.device)
-        held = torch.empty(rows, dtype=torch.int32, device=self.device)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        chosen, held = lengths.new_empty((rows, count)), lengths.new_empty(rows)
+        work = lengths.new_empty(need // 4) if need else None
         rc = self.lib.vramc_kv_select(
             self._ref, self._bounds.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), heads,
             table.data_ptr(), table.stride(0), width, lengths.data_ptr(), batch, count, first, last,

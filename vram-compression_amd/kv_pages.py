@@ -77,6 +77,9 @@ class PagePool(kv_cache.Calls):
         self.pages, self.page_size = pages, page_size
         self._free, self._count, self.device, self._index = free, count, free.device, free.get_device()
         self._ticket = torch.zeros(1, dtype=torch.int32, device=free.device)
+        self._long = torch.empty(0, dtype=torch.int64, device=free.device)  # what slots are made like
+        # of calls that run one after the other
+        self._work = torch.empty(MOST_SEQUENCES + 1, dtype=torch.int32, device=free.device)
         self.lib = bind(lib or rans._host_lib())
         self._desc = PagesDesc(pages, page_size, free.data_ptr(), count.data_ptr(), self._ticket.data_ptr())
         self._ref = ctypes.byref(self._desc)
@@ -113,10 +116,9 @@ class PagePool(kv_cache.Calls):
             self._ints("seen", seen, torch.int32, (batch,))
         if not 0 <= tokens < 2 ** 31 - 1:
             raise ValueError(f"{tokens} rows: 0 to 2**31 - 2")
-        device = self.device
-        slots = torch.empty(tokens, dtype=torch.int64, device=device)
+        slots = self._long.new_empty(tokens)
         # one allocation for what has 32 bits: positions, filled, starts, lengths
-        rest = torch.empty(2 * (tokens + batch) + 1, dtype=torch.int32, device=device)
+        rest = self._ticket.new_empty(2 * (tokens + batch) + 1)
         positions, filled, starts, lengths_out = rest.split_with_sizes((tokens, tokens, batch + 1, batch))
         rc = self.lib.vramc_pages_extend(
             self._ref, table.data_ptr(), table.stride(0), width, lengths.data_ptr(), new.data_ptr(),
@@ -133,12 +135,8 @@ class PagePool(kv_cache.Calls):
         batch, width = self._table(table, None)
         stream = self._stream()
         self._ints("lengths", lengths, torch.int32, (batch,))
-        need = self.lib.vramc_pages_release_workspace(self._ref, width, batch)
-        if need < 0:
-            raise ValueError(f"{batch} sequences over {width} pages: too many ({need})")
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         rc = self.lib.vramc_pages_release(self._ref, table.data_ptr(), table.stride(0), width,
-                                          lengths.data_ptr(), batch, work.data_ptr() if need else None,
-                                          need, stream)
+                                          lengths.data_ptr(), batch, self._work.data_ptr(),
+                                          4 * (MOST_SEQUENCES + 1), stream)
         if rc:
             kv_cache._failed("release", rc)

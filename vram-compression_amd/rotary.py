@@ -88,44 +88,62 @@ class Rotary(kv_cache.Calls):
                                 self._turns.data_ptr())
         self._ref = ctypes.byref(self._desc)
 
-    def _rows(self, name, t, tokens, dtype, heads=None):
-        """Checks tokens x heads x head_dim values; a last dimension that is not dense
-        is copied."""
-        got = t.shape
-        if (len(got) != 3 or got[2] != self.head_dim or t.dtype is not dtype or dtype not in _DTYPES
-                or got[0] != tokens or t.get_device() != self._index or (heads is not None and got[1] != heads)):
-            raise ValueError(f"{name} must be ({tokens}, {heads or 'heads'}, {self.head_dim}) of bf16, f16 or "
-                             f"f32, all of one type, on {self.device}, got {tuple(got)} of {t.dtype} on {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+    def _refuse(self, tokens, dtype, index, **rows):
+        """Says which of the rows is not as it has to be."""
+        _check(dtype in _DTYPES, f"no rotation of {dtype}: bf16, f16 or f32")
+        for name, t in rows.items():
+            got = tuple(t.shape)
+            if (len(got) != 3 or got[2] != self.head_dim or t.dtype is not dtype or got[0] != tokens
+                    or t.get_device() != index):
+                raise ValueError(f"{name} must be ({tokens}, heads, {self.head_dim}) of {dtype} on "
+                                 f"{self.device}, got {got} of {t.dtype} on {t.device}")
+
+    def _weight(self, name, w, dtype):
+        """Checks a norm's weight; its address and type."""
+        kind = w.dtype
+        if (w.shape != (self.head_dim,) or not w.is_contiguous() or w.get_device() != self._index
+                or (kind is not dtype and kind is not torch.float32) or w.data_ptr() % 16):
+            raise ValueError(f"{name} must be {self.head_dim} dense values of {dtype} or torch.float32 on "
+                             f"{self.device}, aligned to 16 bytes; got {tuple(w.shape)} of {kind} on {w.device}")
+        if w.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient; the rotation has none: detach it or use "
                              "torch.no_grad()")
-        return t if t.stride(2) == 1 else t.contiguous()
+        return w.data_ptr(), kind
 
     def _taken(self, q, k, positions, q_weight, k_weight, eps):
-        """Checks the arguments; the descriptor of the rows, and q and k as read."""
-        tokens, dtype = q.shape[0], q.dtype
-        q = self._rows("q", q, tokens, dtype)
-        k = self._rows("k", k, tokens, dtype)
+        """Checks the arguments; the descriptor of the rows, and q and k as they are
+        read (a last dimension that is not dense is copied)."""
+        dtype, index, qs, ks = q.dtype, self._index, q.shape, k.shape
+        tokens = qs[0] if qs else 0
+        if (dtype not in _DTYPES or len(qs) != 3 or len(ks) != 3 or qs[2] != self.head_dim
+                or ks[2] != self.head_dim or ks[0] != tokens or k.dtype is not dtype
+                or q.get_device() != index or k.get_device() != index):
+            self._refuse(tokens, dtype, index, q=q, k=k)
+        if (q.requires_grad or k.requires_grad) and torch.is_grad_enabled():
+            raise ValueError("q or k requires a gradient; the rotation has none: detach it or use "
+                             "torch.no_grad()")
         self._ints("positions", positions, torch.int32, (tokens,))
-        kind, at = dtype, [None, None]
-        for i, w in enumerate((q_weight, k_weight)):
-            if w is None:
-                continue
-            if (w.shape != (self.head_dim,) or not w.is_contiguous() or w.get_device() != self._index
-                    or (w.dtype is not dtype and w.dtype is not torch.float32)
-                    or (at[0] is not None and w.dtype is not kind) or w.data_ptr() % 16):
-                raise ValueError(f"weights must be {self.head_dim} dense values on {self.device}, both of "
-                                 f"{dtype} or both of torch.float32, aligned to 16 bytes; got {w.dtype} "
-                                 f"{tuple(w.shape)} on {w.device}")
-            if w.requires_grad and torch.is_grad_enabled():
-                raise ValueError("the weights require a gradient; the rotation has none: detach them or use "
-                                 "torch.no_grad()")
-            kind, at[i] = w.dtype, w.data_ptr()
+        q_at = k_at = None
+        kind = dtype
+        if q_weight is not None:
+            q_at, kind = self._weight("q_weight", q_weight, dtype)
+        if k_weight is not None:
+            k_at, k_kind = self._weight("k_weight", k_weight, dtype)
+            if q_at is not None and k_kind is not kind:
+                raise ValueError(f"the weights are of {kind} and {k_kind}: one type for both")
+            kind = k_kind
         if not eps >= 0:
             raise ValueError(f"eps {eps}: not negative")
-        rows = RowsDesc(q.data_ptr(), k.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                        q.shape[1], k.shape[1], at[0], at[1], _DTYPES[dtype], _DTYPES[kind], eps,
-                        positions.data_ptr(), tokens)
+        q_token, q_head, q_column = q.stride()
+        k_token, k_head, k_column = k.stride()
+        if q_column != 1:
+            q = q.contiguous()
+            q_token, q_head, _ = q.stride()
+        if k_column != 1:
+            k = k.contiguous()
+            k_token, k_head, _ = k.stride()
+        rows = RowsDesc(q.data_ptr(), k.data_ptr(), q_token, q_head, k_token, k_head, qs[1], ks[1], q_at, k_at,
+                        _DTYPES[dtype], _DTYPES[kind], eps, positions.data_ptr(), tokens)
         return rows, q, k
 
     def rotate(self, q, k, positions, q_weight=None, k_weight=None, eps=1e-6):
@@ -135,8 +153,7 @@ class Rotary(kv_cache.Calls):
         eps).  Computed in f32, angles in 64 bits, rounded once."""
         stream = self._stream()
         rows, q, k = self._taken(q, k, positions, q_weight, k_weight, eps)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=self.device)
+        q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
         rc = self.lib.vramc_rotary_apply(self._ref, ctypes.byref(rows), q_out.data_ptr(), k_out.data_ptr(),
                                          stream)
         if rc:
@@ -147,19 +164,28 @@ class Rotary(kv_cache.Calls):
         """rotate, with the keys and the values v (as k, any strides) written into slots
         (int64) of a cache, as PagedCache.append writes them; a tracked one takes the
         positions too.  Returns the queries, also of tokens without a slot (-1)."""
-        _check(cache.head_dim == self.head_dim and cache.dtype is q.dtype and cache._index == self._index,
-               f"a cache of {cache.dtype} heads of {cache.head_dim} on {cache.device} takes no {q.dtype} of "
-               f"{self.head_dim} on {self.device}")
+        if cache.head_dim != self.head_dim or cache.dtype is not q.dtype or cache._index != self._index:
+            raise ValueError(f"a cache of {cache.dtype} heads of {cache.head_dim} on {cache.device} takes no "
+                             f"{q.dtype} of {self.head_dim} on {self.device}")
         stream = cache._stream()
         rows, q, k = self._taken(q, k, positions, q_weight, k_weight, eps)
-        tokens, heads = k.shape[0], cache.kv_heads
-        if k.shape[1] != heads:
-            raise ValueError(f"keys of {k.shape[1]} heads and a cache of {heads}")
-        v = self._rows("v", v, tokens, q.dtype, heads)
+        shape = k.shape
+        tokens = shape[0]
+        if shape[1] != cache.kv_heads:
+            raise ValueError(f"keys of {shape[1]} heads and a cache of {cache.kv_heads}")
+        if v.shape != shape or v.dtype is not q.dtype or v.get_device() != self._index:
+            raise ValueError(f"v must be {tuple(shape)} of {q.dtype} on {self.device}, got {tuple(v.shape)} of "
+                             f"{v.dtype} on {v.device}")
+        if v.requires_grad and torch.is_grad_enabled():
+            raise ValueError("v requires a gradient; the cache has none: detach it or use torch.no_grad()")
         self._ints("slots", slots, torch.int64, (tokens,))
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        rc = self.lib.vramc_rotary_append(self._ref, ctypes.byref(rows), cache._ref, v.data_ptr(), v.stride(0),
-                                          v.stride(1), slots.data_ptr(), q_out.data_ptr(), stream)
+        v_token, v_head, v_column = v.stride()
+        if v_column != 1:
+            v = v.contiguous()
+            v_token, v_head, _ = v.stride()
+        q_out = q.new_empty(q.shape)
+        rc = self.lib.vramc_rotary_append(self._ref, ctypes.byref(rows), cache._ref, v.data_ptr(), v_token,
+                                          v_head, slots.data_ptr(), q_out.data_ptr(), stream)
         if rc:
             kv_cache._failed("append", rc)
         return q_out
