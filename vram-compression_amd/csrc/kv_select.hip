@@ -2,9 +2,9 @@
 // column of a page bound its scores, and those that can give the largest are taken.
 //
 // bound reads all keys of the pages once, and HBM bounds it: 2048 pages of 64 keys of 8
-// heads of 128 columns 48.6 us, 5.7 TB/s of reads.  A wave takes a page of a head;
-// values are compared as whole numbers that sort as they do, two of 16 bits an
-// instruction.
+// heads of 128 columns 47.4 us, 5.8 TB/s of reads; 20.5 from 4 bits, whose conversion
+// and comparisons keep the vectors busy.  A wave takes a page of a head; values are
+// compared as whole numbers that sort as they do, two of 16 bits an instruction.
 //
 // select scores in 64 bits, so that which page is taken does not depend on an order of
 // sums.  That rate bounds it: 16 sequences of 512 pages of 8 heads, 5 query heads each,
@@ -22,7 +22,9 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 
 // ------------------------------------------------------------------ bounds
-constexpr int kManyEntries = 1 << 16;
+// Waves of a call: more entries, of a prompt's tokens most of which fill no page, are
+// shared among them (one in 64 of 32768 entries of 8 heads 96 us with a wave to each).
+constexpr int kBoundWaves = 1 << 14;
 
 struct Bound {
     vramc_kv_cache c;
@@ -30,14 +32,24 @@ struct Bound {
     const int32_t* pages;
     int64_t n;
     void* bounds;
-    int each;                 // entries of the list to a wave
+    int64_t each;             // entries of the list to a wave
 };
 
 // Values as whole numbers that sort alike, and back: the bits below the sign are
-// turned over in negative ones.
+// turned over in negative ones, two of 16 bits at once (which the compiler takes apart
+// again unless it does not see where the signs come from).
 template <typename I>
 __device__ __forceinline__ vec<I, kPer> sorted(vec<I, kPer> x) {
-    return x ^ ((x >> (8 * sizeof(I) - 1)) & std::numeric_limits<I>::max());
+    constexpr int N = kPer * sizeof(I) / 4;
+    auto word = __builtin_bit_cast(vec<uint32_t, N>, x);
+    const auto sign = __builtin_bit_cast(vec<uint32_t, N>, x >> (8 * sizeof(I) - 1));
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t turn = sign[i];
+        asm("" : "+v"(turn));
+        word[i] ^= turn & (sizeof(I) == 4 ? 0x7fffffffu : 0x7fff7fffu);
+    }
+    return __builtin_bit_cast(std::remove_reference_t<decltype(x)>, word);
 }
 
 // A lane's eight columns of a row.
@@ -49,16 +61,28 @@ struct Columns {
     static constexpr Int kNaN = std::is_same_v<T, float> ? (Int)0x7fc00000 : std::is_same_v<T, __bf16> ? 0x7fc0 : 0x7e00;
     Lying<T> x;
     uint32_t codes, scale;
-    __device__ __forceinline__ void load(const vramc_kv_cache& c, int64_t row, int per_row, int seg) {
+    // where a lane's first row begins, and rows that all lanes are further
+    struct From {
+        const Lying<T>* x;
+        const uint32_t* codes;
+        const uint8_t* scale;
+        int per_row;
+        __device__ __forceinline__ From(const vramc_kv_cache& c, int64_t row, int n, int seg) : per_row(n) {
+            x = static_cast<const Lying<T>*>(c.k) + (row * n + seg);
+            codes = static_cast<const uint32_t*>(c.k) + (row * n + seg);
+            scale = c.k_scale + (row * (n / 4) + seg / 4);
+        }
+    };
+    __device__ __forceinline__ void load(const From& from, int rows) {
         if constexpr (MX) {
-            codes = static_cast<const uint32_t*>(c.k)[row * per_row + seg];
-            scale = c.k_scale[row * (per_row / 4) + seg / 4];
+            codes = from.codes[rows * from.per_row];
+            scale = from.scale[rows * (from.per_row / 4)];
         } else {
             // past the caches, as nobody reads them next: 2048 pages of 64 keys of 8 heads
             // of 128 columns 48.6 us against 55.6
-            const auto* from = static_cast<const Lying<T>*>(c.k) + row * per_row + seg;
+            const auto* at = from.x + rows * from.per_row;
 #pragma unroll
-            for (size_t i = 0; i < sizeof(T) / 2; i++) x.part[i] = __builtin_nontemporal_load(&from->part[i]);
+            for (size_t i = 0; i < sizeof(T) / 2; i++) x.part[i] = __builtin_nontemporal_load(&at->part[i]);
         }
     }
     __device__ __forceinline__ Whole whole() const {
@@ -93,33 +117,38 @@ __global__ void __launch_bounds__(kThreads) bound_kernel(Bound a) {
     const int per_row = a.c.head_dim / kPer, seg = lane & (a.lanes - 1), in_step = 64 / a.lanes;
     const int steps = a.c.page_size / in_step, first = lane / a.lanes;
     const bool inside = seg < per_row;
-    for (int e = 0; e < a.each; e++) {
-        const int64_t i = ((int64_t)chunk * a.each + e) * kWaves + wave;
-        const int page = i < a.n ? a.pages[i] : -1;
-        if (page < 0 || page >= a.c.pages) continue;
-        const int64_t at = (int64_t)page * a.c.kv_heads + head, row = (at << a.page_shift) + first;
-        Whole low = std::numeric_limits<typename C::Int>::max(), high = std::numeric_limits<typename C::Int>::min();
-        if (inside)
-            for (int s = 0; s < steps; s += AHEAD) {
-                C x[AHEAD];
+    // the wave's entries, up to 64 at once, and one page after the other of those that are
+    const int64_t start = ((int64_t)chunk * kWaves + wave) * a.each, stop = min(start + a.each, a.n);
+    for (int64_t i = start; i < stop; i += 64) {
+        const int entry = i + lane < stop ? a.pages[i + lane] : -1;
+        for (uint64_t some = __ballot((uint32_t)entry < (uint32_t)a.c.pages); some; some &= some - 1) {
+            const int page = __builtin_amdgcn_readlane(entry, __builtin_ctzll(some));
+            const int64_t at = (int64_t)page * a.c.kv_heads + head, row = (at << a.page_shift) + first;
+            Whole low = std::numeric_limits<typename C::Int>::max(), high = std::numeric_limits<typename C::Int>::min();
+            if (inside) {
+                const typename C::From from(a.c, row, per_row, seg);
+                for (int s = 0; s < steps; s += AHEAD) {
+                    C x[AHEAD];
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++) x[u].load(a.c, row + (int64_t)(s + u) * in_step, per_row, seg);
+                    for (int u = 0; u < AHEAD; u++) x[u].load(from, (s + u) * in_step);
 #pragma unroll
-                for (int u = 0; u < AHEAD; u++) {
-                    const Whole y = x[u].whole();
-                    low = __builtin_elementwise_min(low, y);
-                    high = __builtin_elementwise_max(high, y);
+                    for (int u = 0; u < AHEAD; u++) {
+                        const Whole y = x[u].whole();
+                        low = __builtin_elementwise_min(low, y);
+                        high = __builtin_elementwise_max(high, y);
+                    }
                 }
             }
-        for (int d = a.lanes; d < 64; d *= 2) {
-            low = __builtin_elementwise_min(low, shuffled(low, d));
-            high = __builtin_elementwise_max(high, shuffled(high, d));
-        }
-        // what is not finite lies at or beyond the infinities
-        const auto bad = (high >= C::kInfinite) | (low <= (typename C::Int)~C::kInfinite);
-        if (inside && lane < 2 * a.lanes) {  // the first row's lanes write the smallest, the second's the largest
-            const Whole y = bad ? (Whole)C::kNaN : sorted<typename C::Int>(lane < a.lanes ? low : high);
-            static_cast<Lying<T>*>(a.bounds)[(2 * at + lane / a.lanes) * per_row + seg] = __builtin_bit_cast(Lying<T>, y);
+            for (int d = a.lanes; d < 64; d *= 2) {
+                low = __builtin_elementwise_min(low, shuffled(low, d));
+                high = __builtin_elementwise_max(high, shuffled(high, d));
+            }
+            // what is not finite lies at or beyond the infinities
+            const auto bad = (high >= C::kInfinite) | (low <= (typename C::Int)~C::kInfinite);
+            if (inside && lane < 2 * a.lanes) {  // the first row's lanes write the smallest, the second's the largest
+                const Whole y = bad ? (Whole)C::kNaN : sorted<typename C::Int>(lane < a.lanes ? low : high);
+                static_cast<Lying<T>*>(a.bounds)[(2 * at + lane / a.lanes) * per_row + seg] = __builtin_bit_cast(Lying<T>, y);
+            }
         }
     }
 }
@@ -333,7 +362,7 @@ constexpr int kChoose = 512;                // threads
 constexpr int kChooseWaves = kChoose / 64;
 constexpr int kPiece = 4096;                // keys in LDS at once
 constexpr int kParts = kPiece / 64;         // of a wave's width
-constexpr int kDigit = 10, kBins = 1 << kDigit, kLaneBins = kBins / 64;
+constexpr int kDigit = 8, kBins = 1 << kDigit, kLaneBins = kBins / 64;  // 10 bits are fewer digits, and 1 us slower
 
 __device__ __forceinline__ uint64_t from_bit(uint64_t x, int bit) { return bit < 64 ? x >> bit : 0; }
 
@@ -414,7 +443,7 @@ __global__ void __launch_bounds__(kChoose) choose_kernel(Select a) {
         __syncthreads();
         // the last digit's bins, which all have read now, for the digit behind the next
         for (int i = threadIdx.x; i < kBins; i += kChoose) hist[turn == 0 ? 2 : turn - 1][i] = 0;
-        // the bin that holds the room-th from the top, 16 neighbouring bins to a lane
+        // the bin that holds the room-th from the top, neighbouring bins to a lane
         int x[kLaneBins], sum = 0;
 #pragma unroll
         for (int i = 0; i < kLaneBins; i += 4) {
@@ -504,8 +533,11 @@ int bound(const Bound& a, hipStream_t stream) {
     if (blocks > kMaxThreads / kThreads) return RANS_EARG;
     const dim3 grid((unsigned)blocks), block(kThreads);
     const int steps = a.c.page_size * a.lanes / 64;
-    if (steps >= 8) hipLaunchKernelGGL((bound_kernel<T, MX, 8>), grid, block, 0, stream, a);
-    else if (steps == 4) hipLaunchKernelGGL((bound_kernel<T, MX, 4>), grid, block, 0, stream, a);
+    // four rows of f32 fill as many registers as eight of 16 bits (108 us against 126), and
+    // 4-bit ones are bound by their conversion (20.5 us against 21.7)
+    constexpr bool EIGHT = sizeof(T) == 2 && !MX;
+    if (steps >= 8 && EIGHT) hipLaunchKernelGGL((bound_kernel<T, MX, EIGHT ? 8 : 4>), grid, block, 0, stream, a);
+    else if (steps >= 4) hipLaunchKernelGGL((bound_kernel<T, MX, 4>), grid, block, 0, stream, a);
     else hipLaunchKernelGGL((bound_kernel<T, MX, 2>), grid, block, 0, stream, a);
     return (int)hipGetLastError();
 }
@@ -519,7 +551,7 @@ extern "C" int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int
     if (n == 0) return 0;
     if (!pages || !bounds || (uintptr_t)bounds % 16) return RANS_EARG;
     const Bound a{*c, __builtin_ctz(c->page_size), lanes_of(c->head_dim), pages, n, bounds,
-                  n * c->kv_heads > kManyEntries ? 4 : 1};
+                  (n * c->kv_heads + kBoundWaves - 1) / kBoundWaves};
     if (c->dtype == RANS_X_F32) return bound<float, false>(a, stream);
     if (c->dtype == RANS_X_BF16) return c->mx ? bound<__bf16, true>(a, stream) : bound<__bf16, false>(a, stream);
     return c->mx ? bound<_Float16, true>(a, stream) : bound<_Float16, false>(a, stream);

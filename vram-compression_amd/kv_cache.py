@@ -212,12 +212,15 @@ class PagedCache(Calls):
         return cls(k, v, dtype, *scales, *more, lib=lib, bounds=limits)
 
     # ------------------------------------------------------------- arguments
-    def _stream(self):
+    def _without_gradient(self):
         if torch.is_grad_enabled() and (self._k.requires_grad or self._v.requires_grad or (
                 self._mass is not None and self._mass.requires_grad) or (
                 self._bounds is not None and self._bounds.requires_grad)):
             raise ValueError("the cache's tensors require a gradient, and its operations have none: "
                              "detach them or use torch.no_grad()")
+
+    def _stream(self):
+        self._without_gradient()
         return super()._stream()
 
     def _rows(self, name, t, heads):
@@ -309,7 +312,7 @@ class PagedCache(Calls):
         need = self.lib.vramc_kv_attend_workspace(self._ref, heads, width, batch, track)
         if need < 0:
             raise ValueError(f"{batch} sequences of {heads} heads over {width} pages: too many ({need})")
-        work = torch.empty(need, dtype=torch.uint8, device=self.device)
+        work = lengths.new_empty(-(-need // 4))
         rc = self.lib.vramc_kv_attend(
             self._ref, q.data_ptr(), q.stride(0), q.stride(1), heads, table.data_ptr(),
             table.stride(0), width, lengths.data_ptr(), batch,
@@ -437,6 +440,7 @@ class PagedCache(Calls):
         """attend over the pages that select chose (which another query of the same
         sequences may use too, as long as they hold the same tokens): q (sequences,
         q_heads, head_dim).  scale is positive: pages are chosen for large scores."""
+        self._without_gradient()  # of these tensors: the heads' are views
         q = self._rows("q", q, None)
         batch, heads, _ = q.shape
         if heads <= 0 or heads % self.kv_heads:

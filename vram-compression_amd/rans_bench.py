@@ -4,6 +4,7 @@
   python vram-compression_amd/rans_bench.py configs # the benchmark configurations
   python vram-compression_amd/rans_bench.py chain [grouped|separate|both] [LAYERS] [BATCH]
   python vram-compression_amd/rans_bench.py tokens [LAYERS] [BATCH] [BUDGET] [STEPS]
+  python vram-compression_amd/rans_bench.py serve [LAYERS] [BATCH] [LONGEST] [PAGES] [STEPS]
   python vram-compression_amd/rans_bench.py profile [ROWS COLS BITS DIST ESC R C N FETCH]
 
 Mirror of kernel/bench.py of snuri00/vram-compression (same function names
@@ -733,10 +734,12 @@ def chain(bits=3.25, layers=28, seed=0, iters=3, grouped=False, batch=1):
 
 
 class AttentionLayer(torch.nn.Module):
-    """A Qwen2.5-1.5B-shaped attention layer (random init, no rotary positions)
-    whose projections are rANS-coded and whose past is a PagedCache."""
+    """A Qwen2.5-1.5B-shaped attention layer (random init) whose projections are
+    rANS-coded and whose past is a PagedCache.  turn: a rotary.Rotary, by which it has
+    rotary positions behind norms of each head (as newer models of that size have them);
+    count: it attends to so many pages of a sequence, which its queries choose."""
 
-    def __init__(self, cache, hidden=1536, heads=12, bits=3.25):
+    def __init__(self, cache, hidden=1536, heads=12, bits=3.25, turn=None, count=0):
         super().__init__()
         import rans_linear
         wide = cache.kv_heads * cache.head_dim
@@ -745,27 +748,52 @@ class AttentionLayer(torch.nn.Module):
             setattr(self, name, torch.nn.Linear(hidden, rows, bias=False))
         self.o_proj = torch.nn.Linear(heads * cache.head_dim, hidden, bias=False)
         rans_linear.replace_linears(self, bits, tune=False)
-        self.cache, self.heads = cache, heads
+        self.cache, self.heads, self.turn, self.count = cache, heads, turn, count
+        if turn is not None:
+            for name in ("q_norm", "k_norm"):
+                self.register_buffer(name, torch.ones(cache.head_dim, dtype=cache.dtype, device=cache.device))
 
-    def forward(self, h, table, lengths, slots, positions):
-        """One new token of each sequence: h (sequences, hidden) in the cache's
-        dtype; lengths counts the new tokens, slots and positions are theirs."""
+    def write(self, h, slots, positions, filled=None):
+        """The queries of new tokens, h (tokens, hidden) in the cache's dtype, whose keys
+        and values go into slots; filled: pages that they make full."""
         c, n = self.cache, h.shape[0]
         x = torch.nn.functional.rms_norm(h, h.shape[-1:])
         q, k, v = (p(x).view(n, -1, c.head_dim) for p in (self.q_proj, self.k_proj, self.v_proj))
-        c.append(k, v, slots, positions)
-        return h + self.o_proj(c.attend(q, table, lengths).view(n, -1))
+        if self.turn is None:
+            c.append(k, v, slots, positions)
+        else:
+            q = self.turn.append(c, q, k, v, slots, positions, self.q_norm, self.k_norm)
+        if filled is not None and c.bounds is not None:
+            c.bound(filled)
+        return q
+
+    def forward(self, h, table, lengths, slots, positions, filled=None):
+        """One new token of each sequence: h (sequences, hidden) in the cache's
+        dtype; lengths counts the new tokens, slots and positions are theirs."""
+        c, q = self.cache, self.write(h, slots, positions, filled)
+        if self.count:
+            out = c.attend_selected(q, *c.select(q, table, lengths, self.count))
+        else:
+            out = c.attend(q, table, lengths)
+        return h + self.o_proj(out.view(h.shape[0], -1))
 
 
 class AttentionStack:
     """Layers whose caches hold the same sequences, each in pages of its own
     table row, and what a serving loop keeps of them: step() takes one token of
     every sequence through all layers and, where `slack` tokens have gathered
-    beyond the budget, drops as many from every layer by their weight."""
+    beyond the budget, drops as many from every layer by their weight.
+
+    pooled: the pages come from a kv_pages.PagePool and go back to it, so that sequences
+    need not be alike: write() takes prompts, finish() ends sequences.  turned and count:
+    as the layers' turn and count."""
 
     def __init__(self, layers=2, batch=4, budget=2048, slack=64, recent=256, page=64,
-                 dtype=torch.bfloat16, mx=True, track=True, bits=3.25, seed=0):
+                 dtype=torch.bfloat16, mx=True, track=True, bits=3.25, seed=0, pooled=False, turned=False,
+                 count=0):
         import kv_cache
+        import kv_pages
+        import rotary
         torch.manual_seed(seed)
         width = -(-(budget + slack) // page)
         self.budget, self.slack, self.recent, self.batch = budget, slack, recent, batch
@@ -773,23 +801,65 @@ class AttentionStack:
         self.rows = torch.arange(batch, device="cuda")
         self.lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
         self.seen = torch.zeros(batch, dtype=torch.int32, device="cuda")
-        self.held = 0  # tokens of every sequence, as the host knows them
-        self.layers = [AttentionLayer(kv_cache.PagedCache.allocate(batch * width, 2, 128, page, dtype, mx, track),
-                                      bits=bits) for _ in range(layers)]
+        self.held = 0  # tokens of the longest sequence, as the host knows them
+        self.pool = None
+        if pooled:
+            self.pool = kv_pages.PagePool(batch * width, page)
+            self.table.fill_(-1)
+            self.one = torch.ones(batch, dtype=torch.int32, device="cuda")
+        turn = rotary.Rotary(128, base=1e6) if turned else None
+        self.layers = [AttentionLayer(kv_cache.PagedCache.allocate(batch * width, 2, 128, page, dtype, mx, track,
+                                                                   bounds=count > 0),
+                                      bits=bits, turn=turn, count=count) for _ in range(layers)]
+
+    def _room(self, new, tokens):
+        """Slots, positions and filled pages of new tokens, which lengths and seen then
+        count."""
+        step = self.pool.extend(self.table, self.lengths, new, tokens, self.seen)
+        self.seen = self.seen + (step.lengths - self.lengths)
+        self.lengths = step.lengths
+        return step.slots, step.positions, step.filled
+
+    @torch.no_grad()
+    def write(self, h, new):
+        """Prompts: new[b] (a list) tokens of each sequence, h (their sum, hidden), whose
+        keys and values every layer keeps (what a prompt's tokens attend to is not
+        computed).  No sequence may then hold more than the budget."""
+        self.held += max(new)
+        room = self._room(torch.tensor(new, dtype=torch.int32, device="cuda"), h.shape[0])
+        for layer in self.layers:
+            layer.write(h, *room)
+
+    def finish(self, sequences):
+        """Ends sequences (rows); their pages are free again."""
+        self.lengths[sequences] = 0
+        self.seen[sequences] = 0
+        self.pool.release(self.table, self.lengths)
 
     @torch.no_grad()
     def step(self, h):
-        slots = self.layers[0].cache.slots(self.table, self.rows, self.lengths)
-        positions = self.seen.clone()
-        self.lengths += 1
-        self.seen += 1
+        if self.pool is None:
+            slots = self.layers[0].cache.slots(self.table, self.rows, self.lengths)
+            positions, filled = self.seen.clone(), None
+            if self.layers[0].count:  # pages whose last place is taken
+                page = self.layers[0].cache.page_size
+                filled = torch.where(slots % page == page - 1, slots // page, -1).int()
+            self.lengths += 1
+            self.seen += 1
+        else:
+            slots, positions, filled = self._room(self.one, self.batch)
         self.held += 1
         for layer in self.layers:
-            h = layer(h, self.table, self.lengths, slots, positions)
+            h = layer(h, self.table, self.lengths, slots, positions, filled)
         if self.held == self.budget + self.slack:
             for layer in self.layers:
                 left = layer.cache.evict(self.table, self.lengths, self.seen, self.budget, self.recent)
             self.lengths, self.held = left, self.budget
+            if self.pool is not None:
+                self.pool.release(self.table, self.lengths)
+            for layer in self.layers:
+                if layer.count:  # tokens have moved
+                    layer.cache.bound(self.table)
         return h
 
 
@@ -819,6 +889,44 @@ def tokens(layers=2, batch=4, budget=2048, steps=256):
              finite=bool(torch.isfinite(out).all()))
     print(json.dumps({k: (round(v, 4) if isinstance(v, float) else v) for k, v in r.items()}),
           flush=True)
+    return r
+
+
+def serve(layers=2, batch=4, longest=32768, count=64, steps=64):
+    """Tokens of `batch` conversations of different lengths, up to `longest`, through
+    Qwen2.5-1.5B-shaped attention layers with rANS-coded weights, norms and rotary
+    positions, their pages from a pool: attention over all tokens and over the `count`
+    pages that a query chooses.  Prints one JSON line."""
+    stack = AttentionStack(layers, batch, longest + steps + 64, mx=False, track=False, pooled=True, turned=True,
+                           count=count)
+    new = [longest * (i + 1) // batch for i in range(batch)]
+    h = torch.randn(sum(new), 1536, device="cuda").bfloat16()
+    stack.write(h, new)
+    h = h[:batch].clone()
+
+    def timed(count):
+        for layer in stack.layers:
+            layer.count = count
+        for _ in range(4):
+            stack.step(h)
+        torch.cuda.synchronize()
+        t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        t0.record()
+        for _ in range(steps // 2 - 4):
+            out = stack.step(h)
+        t1.record()
+        t1.synchronize()
+        return t0.elapsed_time(t1) / (steps // 2 - 4) / layers * 1e3, bool(torch.isfinite(out).all())
+
+    all_us, all_fine = timed(0)
+    few_us, few_fine = timed(count)
+    free = int(stack.pool.count)
+    stack.finish(list(range(batch)))
+    r = dict(config="Qwen2.5-1.5B-shaped attention layers, rANS weights, norms, rotary positions, pooled pages",
+             layers=layers, batch=batch, lengths=new, count=count, steps=steps,
+             us_per_step_and_layer_all_pages=all_us, us_per_step_and_layer_chosen_pages=few_us,
+             free_pages=free, free_pages_at_the_end=int(stack.pool.count), finite=all_fine and few_fine)
+    print(json.dumps({k: (round(v, 4) if isinstance(v, float) else v) for k, v in r.items()}), flush=True)
     return r
 
 
@@ -922,6 +1030,8 @@ if __name__ == "__main__":
         profile(*(t(v) for t, v in zip(types, sys.argv[2:])))
     elif sys.argv[1] == "tokens":
         tokens(*(int(v) for v in sys.argv[2:6]))
+    elif sys.argv[1] == "serve":
+        serve(*(int(v) for v in sys.argv[2:7]))
     elif sys.argv[1] == "chain":  # chain [grouped|separate|both] [layers] [batch]
         mode = sys.argv[2] if len(sys.argv) > 2 else "both"
         layers = int(sys.argv[3]) if len(sys.argv) > 3 else 28
