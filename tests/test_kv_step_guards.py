@@ -200,6 +200,8 @@ def test_rotation_writes_nothing_that_it_reads(kv, rotary, lib):
             assert lib.vramc_rotary_apply(r, x, at(out), far, None) == EARG
             assert lib.vramc_rotary_append(r, x, c, far, 256, 128, P, at(out), None) == EARG
         assert lib.vramc_rotary_apply(r, x, far, at(first), None) == EARG
+    assert lib.vramc_rotary_apply(r, x, far, far, None) == EARG
+    assert lib.vramc_rotary_apply(r, x, at(0x7000000 + 100 * 256 * 2 - 16), far, None) == EARG
     assert lib.vramc_rotary_append(r, x, c, far, 256, 128, P, far, None) == EARG
 
 

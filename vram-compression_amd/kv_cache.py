@@ -371,6 +371,7 @@ class PagedCache(Calls):
         * kv_heads + head: what a selection's page numbers mean."""
         if self._heads is None:
             n = self.pages * self.kv_heads
+            _check(n < 2 ** 31, f"{self.pages} pages of {self.kv_heads} heads: more than can be numbered")
             k, v, ks, vs, mass, position = (None if t is None else t.view(n, 1, self.page_size, -1)
                                             for t in (self._k, self._v, self._k_scale, self._v_scale,
                                                       self._mass, self._position))

@@ -895,31 +895,46 @@ def tokens(layers=2, batch=4, budget=2048, steps=256):
 def serve(layers=2, batch=4, longest=32768, count=64, steps=64):
     """Tokens of `batch` conversations of different lengths, up to `longest`, through
     Qwen2.5-1.5B-shaped attention layers with rANS-coded weights, norms and rotary
-    positions, their pages from a pool: attention over all tokens and over the `count`
-    pages that a query chooses.  Prints one JSON line."""
-    stack = AttentionStack(layers, batch, longest + steps + 64, mx=False, track=False, pooled=True, turned=True,
-                           count=count)
+    positions, their pages from a pool, a step captured in a graph: attention over all
+    tokens and over the `count` pages that a query chooses.  Prints one JSON line."""
+    stack = AttentionStack(layers, batch, longest + 2 * steps + 64, mx=False, track=False, pooled=True,
+                           turned=True, count=count)
     new = [longest * (i + 1) // batch for i in range(batch)]
     h = torch.randn(sum(new), 1536, device="cuda").bfloat16()
     stack.write(h, new)
-    h = h[:batch].clone()
+    h, lengths, seen = h[:batch].clone(), stack.lengths.clone(), stack.seen.clone()
+
+    @torch.no_grad()
+    def step():  # what a graph replays: lengths in place
+        room, x = stack.pool.extend(stack.table, lengths, stack.one, batch, seen), h
+        for layer in stack.layers:
+            x = layer(x, stack.table, room.lengths, room.slots, room.positions, room.filled)
+        seen.add_(room.lengths - lengths)
+        lengths.copy_(room.lengths)
+        return x
 
     def timed(count):
         for layer in stack.layers:
             layer.count = count
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
         for _ in range(4):
-            stack.step(h)
+            graph.replay()
         torch.cuda.synchronize()
         t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
         t0.record()
-        for _ in range(steps // 2 - 4):
-            out = stack.step(h)
+        for _ in range(steps):
+            graph.replay()
         t1.record()
         t1.synchronize()
-        return t0.elapsed_time(t1) / (steps // 2 - 4) / layers * 1e3, bool(torch.isfinite(out).all())
+        return t0.elapsed_time(t1) / steps / layers * 1e3, bool(torch.isfinite(out).all())
 
     all_us, all_fine = timed(0)
     few_us, few_fine = timed(count)
+    stack.lengths, stack.seen = lengths, seen
     free = int(stack.pool.count)
     stack.finish(list(range(batch)))
     r = dict(config="Qwen2.5-1.5B-shaped attention layers, rANS weights, norms, rotary positions, pooled pages",
