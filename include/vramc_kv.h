@@ -128,7 +128,8 @@ int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, voi
  * head), -1 for an entry that is none and behind the last; held[b*kv_heads + h]: the
  * tokens in them, so that vramc_kv_attend takes both as table and lengths.
  * workspace: vramc_kv_select_workspace bytes, no content expected, 16-byte aligned. */
-int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int table_width, int batch, int count);
+int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int q_heads, int table_width, int batch,
+                                  int count);
 int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, const void* q, int64_t q_seq,
                     int64_t q_head, int q_heads, const int32_t* table, int64_t table_row,
                     int table_width, const int32_t* lengths, int batch, int count, int first,

@@ -166,6 +166,12 @@ SELECTIONS = [  # dim, page, heads, group, lengths, more, count, first, last
     (128, 128, 4, 40, [2000, 100], 0, 6, 5, 1), (64, 256, 5, 7, [9999, 256, 257, 512], 2, 3, 0, 1),
     (64, 16, 1, 3, [140000], 0, 100, 1, 1), (64, 16, 2, 1, [8192 * 16 + 5, 40], 5, 5000, 1, 1),
     (128, 16, 2, 2, [50, 60], 0, 9, 1, 1),
+    # tables around those whose pages are scored where they are chosen from
+    (64, 16, 2, 7, [16 * 192, 16 * 191 - 1, 40], 0, 37, 0, 1), (64, 16, 1, 8, [16 * 193], 0, 37, 3, 4),
+    (64, 16, 1, 9, [16 * 192], 0, 100, 1, 1), (96, 16, 3, 5, [16 * 96, 16 * 95], 0, 95, 1, 1),
+    (128, 16, 2, 8, [16 * 97, 5], 0, 7, 2, 2), (128, 32, 2, 1, [32 * 33, 32 * 65, 32 * 9], 31, 8, 1, 7),
+    (192, 16, 2, 3, [16 * 48, 16 * 33, 1], 0, 17, 0, 2), (256, 16, 1, 8, [16 * 48 - 3], 0, 47, 0, 1),
+    (256, 16, 1, 2, [16 * 49], 0, 2, 1, 1),
 ]
 
 
@@ -223,8 +229,10 @@ def test_pages_that_are_none_and_keys_that_are_not_finite(kv):
     table[2, :] = -1
     n = torch.full((3,), 80 * 16 - 7, dtype=torch.int32, device="cuda")
     q = torch.randn(3, 4, 64, device="cuda", generator=gen(4)).bfloat16()
+    more = torch.cat((table, torch.full((3, 200), -1, dtype=torch.int32, device="cuda")), 1)  # scored apart
     for count in (2, 3, 5, 30, 39, 41, 60, 79):
         compare(c, q, table, n, count, 1, 1)
+        compare(c, q, more, n, count, 1, 1)
     c.bounds.fill_(math.nan)  # none has been made: by index
     compare(c, q, table, n, 9, 0, 2)
 

@@ -212,14 +212,14 @@ def test_bound_and_select_refuse(kv, lib):
                 (c, P, 3, at(0x10008)), (cache(kv, page_size=8), P, 3, P)):
         assert lib.vramc_kv_bound(*bad, None) in (EARG, EUNSUPPORTED)
     assert lib.vramc_kv_bound(c, None, 0, None, None) == 0
-    assert lib.vramc_kv_select_workspace(c, 8, 3, 8) == 0
-    need = lib.vramc_kv_select_workspace(c, 9, 3, 8)
-    assert need == 3 * 2 * 9 * 8
-    for width, batch, count in ((-1, 3, 8), (9, -1, 8), (9, 3, 0), (9, 3, -1), (1 << 27, 3, 8), (9, 1 << 24, 8),
-                                (9, 3, 1 << 28)):
-        assert lib.vramc_kv_select_workspace(c, width, batch, count) == EARG
-    assert lib.vramc_kv_select_workspace(cache(kv, pages=1 << 30), 9, 3, 8) == EARG  # page * heads beyond 32 bits
-    ok = [c, P, P, 512, 128, 4, P, 9, 9, P, 3, 8, 1, 1, P, P, P, need, None]
+    assert lib.vramc_kv_select_workspace(c, 4, 8, 3, 8) == 0  # all pages
+    need = lib.vramc_kv_select_workspace(c, 4, 900, 3, 8)
+    assert need == 3 * 2 * 900 * 8
+    for heads, width, batch, count in ((4, -1, 3, 8), (4, 9, -1, 8), (4, 9, 3, 0), (4, 9, 3, -1), (4, 1 << 27, 3, 8),
+                                       (4, 9, 1 << 24, 8), (4, 9, 3, 1 << 28), (3, 9, 3, 8), (0, 9, 3, 8), (-2, 9, 3, 8)):
+        assert lib.vramc_kv_select_workspace(c, heads, width, batch, count) == EARG
+    assert lib.vramc_kv_select_workspace(cache(kv, pages=1 << 30), 4, 9, 3, 8) == EARG  # page * heads beyond 32 bits
+    ok = [c, P, P, 512, 128, 4, P, 900, 900, P, 3, 8, 1, 1, P, P, P, need, None]
     for i, value, code in ((1, None, EARG), (1, at(0x10008), EARG), (2, None, EARG), (5, 3, EARG), (5, 0, EARG),
                            (6, None, EARG), (9, None, EARG), (11, 1, EARG), (12, -1, EARG), (13, 0, EARG),
                            (12, 2 ** 31 - 1, EARG), (14, None, EARG), (15, None, EARG), (16, None, EWORKSPACE),

@@ -8,10 +8,11 @@
 //
 // select scores in 64 bits, so that which page is taken does not depend on an order of
 // sums.  That rate bounds it: 16 sequences of 512 pages of 8 heads, 5 query heads each,
-// 17 us where their bounds are read in 6.  A second launch, a workgroup to a kv head of
+// 16 us where their bounds are read in 6.  A second launch, a workgroup to a kv head of
 // a sequence, finds the border by radix over the scores' bits, from the highest in
 // which they differ, and writes the pages in their order by counts of ballot bits (5
-// to 7 us: reads, three digits, lists, one after the other).
+// to 7 us: reads, digits, lists, one after the other); for small tables it makes the
+// scores too.
 #include "kv_device.h"
 
 #include <limits>
@@ -230,69 +231,93 @@ __device__ __forceinline__ double row_sum(double x, int lanes) {
 // lane.  q_d lo_d or q_d hi_d is q_d (hi_d + lo_d) / 2 + |q_d| (hi_d - lo_d) / 2
 // whatever the sign: two multiply-adds a column and query head.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) score_few_kernel(Select a, int dim, int lanes) {
-    __shared__ __attribute__((aligned(16))) double query[kFewHeads * kMaxDim];  // halves, [head][pair of eight][lane][2]
-    const int group_of = blockIdx.x / a.chunks, chunk = blockIdx.x - group_of * a.chunks;
-    const int b = group_of / a.heads, h = group_of - b * a.heads;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int per_row = dim / kPer, seg = lane & (lanes - 1), in_set = 64 / lanes;
-    const bool inside = seg < per_row;
-    const T* q = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)h * a.group * a.q_head;
-    // the first pages' numbers, while it is not known whether there are as many
-    const int first = (chunk * kWaves + wave) * kSets * in_set + lane / lanes;
+struct Few {
+    const Select& a;
+    int b, h, dim, lanes, per_row, in_set, seg;
+    bool inside;
     int page[kSets];
-#pragma unroll
-    for (int s = 0; s < kSets; s++) page[s] = a.page(b, min(first + s * in_set, a.width - 1));
-    const int n = a.pages_of(a.length_of(b));
-    if (n <= a.count || chunk * kWaves * kSets * in_set >= n) return;
     Lying<T> raw[kSets][2];
-#pragma unroll
-    for (int s = 0; s < kSets; s++) {
-        const auto* from = static_cast<const Lying<T>*>(a.bounds) +
-                           2 * ((int64_t)max(page[s], 0) * a.heads + h) * per_row + (inside ? seg : 0);
-#pragma unroll
-        for (int i = 0; i < 2; i++) raw[s][i] = from[i * per_row];
-    }
-    for (int i = threadIdx.x; i < a.group * dim; i += kThreads) {
-        const int g = i / dim, d = i - g * dim;
-        query[((g * (kPer / 2) + d % kPer / 2) * per_row + d / kPer) * 2 + d % 2] = 0.5 * wide(q[g * a.q_head + d]);
-    }
-    __syncthreads();
-    double sum[kSets][kPer], gap[kSets][kPer], best[kSets];
-#pragma unroll
-    for (int s = 0; s < kSets; s++) {
-        const auto low = __builtin_bit_cast(vec<T, kPer>, raw[s][0]), high = __builtin_bit_cast(vec<T, kPer>, raw[s][1]);
-#pragma unroll
-        for (int j = 0; j < kPer; j++) {
-            sum[s][j] = wide(high[j]) + wide(low[j]);
-            gap[s][j] = wide(high[j]) - wide(low[j]);
+
+    __device__ __forceinline__ Few(const Select& select, int sequence, int head, int d, int row_lanes)
+        : a(select), b(sequence), h(head), dim(d), lanes(row_lanes), per_row(d / kPer), in_set(64 / row_lanes),
+          seg(threadIdx.x & (row_lanes - 1)), inside(seg < d / kPer) {}
+    // halves of the queries to LDS, [head][pair of eight][lane][2]
+    __device__ __forceinline__ void stage(double* query, int threads) const {
+        const T* q = static_cast<const T*>(a.q) + b * a.q_seq + (int64_t)h * a.group * a.q_head;
+        for (int i = threadIdx.x; i < a.group * dim; i += threads) {
+            const int g = i / dim, d = i - g * dim;
+            query[((g * (kPer / 2) + d % kPer / 2) * per_row + d / kPer) * 2 + d % 2] = 0.5 * wide(q[g * a.q_head + d]);
         }
-        best[s] = -__builtin_inf();
     }
-    const int at = inside ? seg : 0;
-#pragma unroll 1
-    for (int g = 0; g < a.group; g++) {
-        double x[kSets] = {}, y[kSets] = {};
+    // the numbers of the lane's pages, from index `first` on, and their bounds
+    __device__ __forceinline__ void find(int first) {
 #pragma unroll
-        for (int p = 0; p < kPer / 2; p++) {
-            const auto v = *reinterpret_cast<const vec<double, 2>*>(query + ((g * (kPer / 2) + p) * per_row + at) * 2);
-#pragma unroll
-            for (int s = 0; s < kSets; s++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    x[s] = __builtin_fma(v[i], sum[s][2 * p + i], x[s]);
-                    y[s] = __builtin_fma(__builtin_fabs(v[i]), gap[s][2 * p + i], y[s]);
-                }
-        }
+        for (int s = 0; s < kSets; s++) page[s] = a.page(b, min(first + s * in_set, a.width - 1));
+    }
+    __device__ __forceinline__ void load() {
 #pragma unroll
         for (int s = 0; s < kSets; s++) {
-            const double score = row_sum(inside ? x[s] + y[s] : 0.0, lanes);
-            best[s] = score != score ? __builtin_inf() : fmax(best[s], score);
+            const auto* from = static_cast<const Lying<T>*>(a.bounds) +
+                               2 * ((int64_t)max(page[s], 0) * a.heads + h) * per_row + (inside ? seg : 0);
+#pragma unroll
+            for (int i = 0; i < 2; i++) raw[s][i] = from[i * per_row];
         }
     }
+    __device__ __forceinline__ void score(const double* query, double (&best)[kSets]) const {
+        double sum[kSets][kPer], gap[kSets][kPer];
 #pragma unroll
-    for (int s = 0; s < kSets; s++)
-        if (seg == 0 && first + s * in_set < n) a.keys[(int64_t)group_of * a.width + first + s * in_set] = key_of(best[s], page[s]);
+        for (int s = 0; s < kSets; s++) {
+            const auto low = __builtin_bit_cast(vec<T, kPer>, raw[s][0]), high = __builtin_bit_cast(vec<T, kPer>, raw[s][1]);
+#pragma unroll
+            for (int j = 0; j < kPer; j++) {
+                sum[s][j] = wide(high[j]) + wide(low[j]);
+                gap[s][j] = wide(high[j]) - wide(low[j]);
+            }
+            best[s] = -__builtin_inf();
+        }
+        const int at = inside ? seg : 0;
+#pragma unroll 1
+        for (int g = 0; g < a.group; g++) {
+            double x[kSets] = {}, y[kSets] = {};
+#pragma unroll
+            for (int p = 0; p < kPer / 2; p++) {
+                const auto v = *reinterpret_cast<const vec<double, 2>*>(query + ((g * (kPer / 2) + p) * per_row + at) * 2);
+#pragma unroll
+                for (int s = 0; s < kSets; s++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        x[s] = __builtin_fma(v[i], sum[s][2 * p + i], x[s]);
+                        y[s] = __builtin_fma(__builtin_fabs(v[i]), gap[s][2 * p + i], y[s]);
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < kSets; s++) {
+                const double score = row_sum(inside ? x[s] + y[s] : 0.0, lanes);
+                best[s] = score != score ? __builtin_inf() : fmax(best[s], score);
+            }
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) score_few_kernel(Select a, int dim, int lanes) {
+    __shared__ __attribute__((aligned(16))) double query[kFewHeads * kMaxDim];
+    const int group_of = blockIdx.x / a.chunks, chunk = blockIdx.x - group_of * a.chunks, b = group_of / a.heads;
+    Few<T> few(a, b, group_of - b * a.heads, dim, lanes);
+    const int wave = threadIdx.x >> 6, first = (chunk * kWaves + wave) * kSets * few.in_set + (threadIdx.x & 63) / lanes;
+    few.find(first);  // while it is not known whether there are as many
+    const int n = a.pages_of(a.length_of(b));
+    if (n <= a.count || chunk * kWaves * kSets * few.in_set >= n) return;
+    few.load();
+    few.stage(query, kThreads);
+    __syncthreads();
+    double best[kSets];
+    few.score(query, best);
+#pragma unroll
+    for (int s = 0; s < kSets; s++) {
+        const int i = first + s * few.in_set;
+        if (few.seg == 0 && i < n) a.keys[(int64_t)group_of * a.width + i] = key_of(best[s], few.page[s]);
+    }
 }
 
 // A wave scores 16 pages with 16 query heads: lane (n = lane % 16, g = lane / 16)
@@ -361,18 +386,26 @@ __global__ void __launch_bounds__(kThreads) score_kernel(Select a) {
 constexpr int kChoose = 512;                // threads
 constexpr int kChooseWaves = kChoose / 64;
 constexpr int kPiece = 4096;                // keys in LDS at once
-constexpr int kParts = kPiece / 64;         // of a wave's width
+// Small tables are scored where they are chosen from, by up to kFewHeads: so many pages
+// at most, and as many as a workgroup scores in one step and a half.  16 sequences of 8
+// heads of 128 columns, 5 query heads: 65 pages 9.2 us in one launch and 10.9 in two, 128
+// 10.9 and 10.8, 256 17.0 and 14.0; of 2 heads of 64, 7 query heads, 128 8.5 and 10.2, 256
+// 12.0 and 10.5.  Where the host waits, a launch and a workspace less are 4 us more.
+constexpr int kHerePages = 192, kHereLanes = 1536;
 constexpr int kDigit = 8, kBins = 1 << kDigit, kLaneBins = kBins / 64;  // 10 bits are fewer digits, and 1 us slower
 
 __device__ __forceinline__ uint64_t from_bit(uint64_t x, int bit) { return bit < 64 ? x >> bit : 0; }
 
-__global__ void __launch_bounds__(kChoose) choose_kernel(Select a) {
-    __shared__ uint64_t key[kPiece];
-    __shared__ int32_t page[kPiece];
+// HERE: the scores are made here, or else read.
+template <typename T, bool HERE>
+__global__ void __launch_bounds__(kChoose) choose_kernel(Select a, int dim, int lanes) {
+    constexpr int PIECE = HERE ? kHerePages : kPiece, PARTS = PIECE / 64;  // keys at once, waves of them
+    __shared__ uint64_t key[PIECE];
+    __shared__ int32_t page[PIECE];
     // Every wave goes over the whole of what all have counted: one barrier a digit.
     __shared__ __attribute__((aligned(16))) int hist[3][kBins];  // this digit's, the last one's, the next one's
     __shared__ uint32_t ends[2][kChooseWaves];
-    __shared__ uint32_t counts[kParts];  // above the border | at it << 16
+    __shared__ uint32_t counts[PARTS];  // above the border | at it << 16
     const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int32_t* out = a.chosen + (int64_t)blockIdx.x * a.count;
@@ -384,13 +417,13 @@ __global__ void __launch_bounds__(kChoose) choose_kernel(Select a) {
     const auto load = [&](int piece, int size) {  // a thread reads what it wrote
 #pragma unroll 2
         for (int i = threadIdx.x; i < size; i += kChoose) {
-            const uint64_t x = keys[piece * kPiece + i];
-            const int32_t y = entry(a.first + piece * kPiece + i);
+            const uint64_t x = keys[piece * PIECE + i];
+            const int32_t y = entry(a.first + piece * PIECE + i);
             key[i] = x, page[i] = y;
         }
     };
     // the first keys, while it is not known how many there are
-    if (a.width > a.count) load(0, min(a.width - a.first, kPiece));
+    if (!HERE && a.width > a.count) load(0, min(a.width - a.first, PIECE));
     const int tokens = a.length_of(b), n = a.pages_of(tokens), kept = min(n, a.count);
     if (threadIdx.x == 0) a.held[blockIdx.x] = kept ? tokens - ((n - kept) << a.page_shift) : 0;
     // the pages at the ends, or all of them, and what is behind them
@@ -402,8 +435,34 @@ __global__ void __launch_bounds__(kChoose) choose_kernel(Select a) {
     const int among = n - a.first - a.last;      // candidates,
     int room = a.count - a.first - a.last;       // of which so many are taken
     if (n <= a.count || room == 0) return;
-    const int pieces = (among + kPiece - 1) / kPiece;
-    const auto size_of = [&](int piece) { return min(among - piece * kPiece, kPiece); };
+    const int pieces = HERE ? 1 : (among + PIECE - 1) / PIECE;
+    const auto size_of = [&](int piece) { return min(among - piece * PIECE, PIECE); };
+    if constexpr (HERE) {
+        __shared__ __attribute__((aligned(16))) double query[kFewHeads * kMaxDim];
+        Few<T> few(a, b, h, dim, lanes);
+        const int step = kSets * few.in_set;  // of a wave
+        int first = wave * step + lane / lanes;
+        few.find(first);
+        few.load();
+        few.stage(query, kChoose);
+        __syncthreads();
+#pragma unroll 1
+        for (; first - lane / lanes < n; first += kChooseWaves * step) {
+            double best[kSets];
+            few.score(query, best);
+#pragma unroll
+            for (int s = 0; s < kSets; s++) {
+                const int i = first + s * few.in_set - a.first;
+                if (few.seg == 0 && i >= 0 && i < among) {
+                    key[i] = key_of(best[s], few.page[s]);
+                    page[i] = few.page[s] < 0 ? -1 : few.page[s] * a.heads + h;
+                }
+            }
+            few.find(first + kChooseWaves * step);
+            few.load();
+        }
+        __syncthreads();
+    }
     for (int i = threadIdx.x; i < 3 * kBins; i += kChoose) (&hist[0][0])[i] = 0;
     // the highest of the upper 32 bits in which keys differ, or the 32nd
     uint32_t least = ~0u, most = 0;
@@ -511,20 +570,31 @@ int64_t chunks_of(int dim, int group, int table_width) {
     return (table_width + pages - 1) / pages;
 }
 
+// Whether the workgroups that choose make the scores themselves.
+bool scored_here(int dim, int group, int table_width) {
+    return group <= kFewHeads && (int64_t)table_width * lanes_of(dim) <= kHereLanes;
+}
+
 template <typename T>
-void score(const Select& a, int dim, hipStream_t stream) {
-    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.chunks)), block(kThreads);
-    if (a.group <= kFewHeads) {
-        hipLaunchKernelGGL((score_few_kernel<T>), grid, block, 0, stream, a, dim, lanes_of(dim));
-        return;
+int select(const Select& a, int dim, hipStream_t stream) {
+    const int lanes = lanes_of(dim);
+    const dim3 chosen((unsigned)(a.batch * a.heads)), choose(kChoose);
+    if (a.width > a.count && scored_here(dim, a.group, a.width)) {
+        hipLaunchKernelGGL((choose_kernel<T, true>), chosen, choose, 0, stream, a, dim, lanes);
+        return (int)hipGetLastError();
     }
-    switch (dim) {
-        case 64: hipLaunchKernelGGL((score_kernel<T, 64>), grid, block, 0, stream, a); break;
-        case 96: hipLaunchKernelGGL((score_kernel<T, 96>), grid, block, 0, stream, a); break;
-        case 128: hipLaunchKernelGGL((score_kernel<T, 128>), grid, block, 0, stream, a); break;
-        case 192: hipLaunchKernelGGL((score_kernel<T, 192>), grid, block, 0, stream, a); break;
-        default: hipLaunchKernelGGL((score_kernel<T, 256>), grid, block, 0, stream, a);
+    if (a.width > a.count) {
+        const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.chunks)), block(kThreads);
+        if (a.group <= kFewHeads) hipLaunchKernelGGL((score_few_kernel<T>), grid, block, 0, stream, a, dim, lanes);
+        else if (dim == 64) hipLaunchKernelGGL((score_kernel<T, 64>), grid, block, 0, stream, a);
+        else if (dim == 96) hipLaunchKernelGGL((score_kernel<T, 96>), grid, block, 0, stream, a);
+        else if (dim == 128) hipLaunchKernelGGL((score_kernel<T, 128>), grid, block, 0, stream, a);
+        else if (dim == 192) hipLaunchKernelGGL((score_kernel<T, 192>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((score_kernel<T, 256>), grid, block, 0, stream, a);
+        if (const int rc = (int)hipGetLastError()) return rc;
     }
+    hipLaunchKernelGGL((choose_kernel<float, false>), chosen, choose, 0, stream, a, dim, lanes);  // of any type
+    return (int)hipGetLastError();
 }
 
 template <typename T, bool MX>
@@ -557,15 +627,16 @@ extern "C" int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int
     return c->mx ? bound<_Float16, true>(a, stream) : bound<_Float16, false>(a, stream);
 }
 
-extern "C" int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int table_width, int batch, int count) {
+extern "C" int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int q_heads, int table_width, int batch, int count) {
     if (const int rc = check_cache(c)) return rc;
-    if (table_width < 0 || batch < 0 || count <= 0 || (int64_t)table_width * c->page_size > kMaxTokens ||
-        (int64_t)batch * c->kv_heads > kMaxThreads / kChoose || (int64_t)count * c->page_size > kMaxTokens ||
-        (int64_t)c->pages * c->kv_heads > INT32_MAX)
+    if (q_heads <= 0 || q_heads % c->kv_heads || table_width < 0 || batch < 0 || count <= 0 ||
+        (int64_t)table_width * c->page_size > kMaxTokens || (int64_t)batch * c->kv_heads > kMaxThreads / kChoose ||
+        (int64_t)count * c->page_size > kMaxTokens || (int64_t)c->pages * c->kv_heads > INT32_MAX)
         return RANS_EARG;
-    if (table_width <= count) return 0;
+    const int group = q_heads / c->kv_heads;
+    if (table_width <= count || scored_here(c->head_dim, group, table_width)) return 0;
     const int64_t rows = (int64_t)batch * c->kv_heads;
-    if (chunks_of(c->head_dim, 1, table_width) * rows > kMaxThreads / kThreads) return RANS_EARG;  // the most
+    if (chunks_of(c->head_dim, group, table_width) * rows > kMaxThreads / kThreads) return RANS_EARG;
     return rows * table_width * 8;
 }
 
@@ -574,9 +645,9 @@ extern "C" int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, cons
                                int table_width, const int32_t* lengths, int batch, int count, int first,
                                int last, int32_t* chosen, int32_t* held, void* workspace,
                                int64_t workspace_bytes, hipStream_t stream) {
-    const int64_t need = vramc_kv_select_workspace(c, table_width, batch, count);
+    const int64_t need = vramc_kv_select_workspace(c, q_heads, table_width, batch, count);
     if (need < 0) return (int)need;
-    if (q_heads <= 0 || q_heads % c->kv_heads || first < 0 || last < 1 || (int64_t)first + last > count) return RANS_EARG;
+    if (first < 0 || last < 1 || (int64_t)first + last > count) return RANS_EARG;
     if (batch == 0) return 0;
     if (!bounds || (uintptr_t)bounds % 16 || !q || !lengths || !chosen || !held || (table_width && !table))
         return RANS_EARG;
@@ -585,12 +656,6 @@ extern "C" int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, cons
     const Select a{bounds, q, q_seq, q_head, q_heads / c->kv_heads, c->kv_heads, c->pages,
                    __builtin_ctz(c->page_size), table, table_row, table_width, lengths, batch, count, first, last,
                    (int)chunks_of(c->head_dim, q_heads / c->kv_heads, table_width), static_cast<uint64_t*>(workspace), chosen, held};
-    if (need) {
-        if (c->dtype == RANS_X_F32) score<float>(a, c->head_dim, stream);
-        else if (c->dtype == RANS_X_BF16) score<__bf16>(a, c->head_dim, stream);
-        else score<_Float16>(a, c->head_dim, stream);
-        if (const int rc = (int)hipGetLastError()) return rc;
-    }
-    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)(batch * c->kv_heads)), dim3(kChoose), 0, stream, a);
-    return (int)hipGetLastError();
+    if (c->dtype == RANS_X_F32) return select<float>(a, c->head_dim, stream);
+    return c->dtype == RANS_X_BF16 ? select<__bf16>(a, c->head_dim, stream) : select<_Float16>(a, c->head_dim, stream);
 }

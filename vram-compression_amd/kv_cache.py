@@ -64,7 +64,7 @@ def bind(lib):
         "vramc_kv_evict_workspace": ([D, I32, I32, I32, I32], I64),
         "vramc_kv_evict": ([D, P, I64, I32, P, P, I32, I32, I32, P, I64, I32, P, P, I64, P], I32),
         "vramc_kv_bound": ([D, P, I64, P, P], I32),
-        "vramc_kv_select_workspace": ([D, I32, I32, I32], I64),
+        "vramc_kv_select_workspace": ([D, I32, I32, I32, I32], I64),
         "vramc_kv_select": ([D, P, P, I64, I64, I32, P, I64, I32, P, I32, I32, I32, I32, P, P, P, I64, P],
                             I32),
     }
@@ -423,7 +423,7 @@ class PagedCache(Calls):
         if count >= width:  # all pages, whatever their scores
             count, first, last = max(width, 1), 0, 1
         rows = batch * self.kv_heads
-        need = self.lib.vramc_kv_select_workspace(self._ref, width, batch, count)
+        need = self.lib.vramc_kv_select_workspace(self._ref, heads, width, batch, count)
         if need < 0:
             raise ValueError(f"{batch} sequences of {self.kv_heads} kv heads over {width} pages: too many "
                              f"({need})")
