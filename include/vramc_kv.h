@@ -126,7 +126,8 @@ int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, voi
  * chosen[b*kv_heads + h][count]: the pages in order of the sequence's, page * kv_heads
  * + h (a page of the same tensors taken as a cache of pages * kv_heads pages of one
  * head), -1 for an entry that is none and behind the last; held[b*kv_heads + h]: the
- * tokens in them, so that vramc_kv_attend takes both as table and lengths.
+ * tokens in them, so that vramc_kv_attend takes both as table and lengths; neither
+ * shares memory with the other, lengths or table (RANS_EARG).
  * workspace: vramc_kv_select_workspace bytes, no content expected, 16-byte aligned. */
 int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int q_heads, int table_width, int batch,
                                   int count);

@@ -52,7 +52,8 @@ int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t table_row, 
 /* Puts the pages of entries at ceil(lengths[b] / page_size) and behind on the stack,
  * in order of the sequences and entries, and -1 in their place.  Entries that are
  * no page become -1 and go nowhere; what would not fit the stack (a page given back
- * twice) is dropped.  workspace: vramc_pages_release_workspace bytes, no content
+ * twice) is dropped.  The table shares no memory with lengths or the pool (RANS_EARG).
+ * workspace: vramc_pages_release_workspace bytes, no content
  * expected, 16-byte aligned, private to the call until its kernels have run. */
 int64_t vramc_pages_release_workspace(const vramc_pages* p, int table_width, int batch);
 int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t table_row, int table_width,

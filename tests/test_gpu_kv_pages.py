@@ -181,8 +181,9 @@ def test_a_page_given_back_twice_stays_inside(kv_pages, width):
 
 
 @pytest.mark.parametrize("batch,width", [(3, 64), (512, 64), (513, 64), (4, 8192), (4096, 1), (4096, 70), (1, 32768),
-                                         (1, 40000)])
-def test_release_of_large_tables(kv_pages, batch, width):
+                                         (1, 40000), (64, 256), (64, 260), (65, 4), (64, 4), (16, 1024), (1, 16384),
+                                         (1, 16388), (5, 1000), (1, 4), (17, 516), (63, 252)])
+def test_release_of_tables(kv_pages, batch, width):
     rng = np.random.default_rng(width)
     table = np.full((batch, width), -1)
     table[rng.random((batch, width)) < 0.4] = 0
@@ -210,19 +211,22 @@ def test_extend_of_many_sequences(kv_pages, batch):
     compare(pool, plain, got, table, step, plain.extend(table, lengths, new, tokens))
 
 
-def test_rows_of_a_wider_table(kv_pages):
-    """A table cut to the pages in use, and what lies beside it, which stays."""
-    wide = torch.full((4, 20), 77, dtype=torch.int32, device="cuda")
-    table = wide[:, 3:9]
+@pytest.mark.parametrize("first,columns", [(3, 20), (4, 20), (8, 14), (4, 17)])
+def test_rows_of_a_wider_table(kv_pages, first, columns):
+    """A table cut to the pages in use, at any alignment, and what lies beside it, which
+    stays."""
+    width = 6 if first % 2 else 8
+    wide = torch.full((4, columns + 3), 77, dtype=torch.int32, device="cuda")[:, :columns]
+    table = wide[:, first:first + width]
     table.fill_(-1)
-    pool, plain, want = kv_pages.PagePool(30, 16), Plain(30, 16, range(29, -1, -1), 30), np.full((4, 6), -1)
+    pool, plain, want = kv_pages.PagePool(30, 16), Plain(30, 16, range(29, -1, -1), 30), np.full((4, table.shape[1]), -1)
     lengths, new = [0] * 4, [90, 17, 96, 0]
     step = pool.extend(table, ints(lengths), ints(new), 203)
     compare(pool, plain, table, want, step, plain.extend(want, lengths, new, 203))
     pool.release(table, ints([16, 17, 50, 0]))
     plain.release(want, [16, 17, 50, 0])
     compare(pool, plain, table, want)
-    assert (wide[:, :3] == 77).all() and (wide[:, 9:] == 77).all()
+    assert (wide[:, :first] == 77).all() and (wide[:, first + table.shape[1]:] == 77).all()
 
 
 def test_empty_calls(kv_pages):

@@ -230,9 +230,11 @@ def test_pages_that_are_none_and_keys_that_are_not_finite(kv):
     n = torch.full((3,), 80 * 16 - 7, dtype=torch.int32, device="cuda")
     q = torch.randn(3, 4, 64, device="cuda", generator=gen(4)).bfloat16()
     more = torch.cat((table, torch.full((3, 200), -1, dtype=torch.int32, device="cuda")), 1)  # scored apart
+    many = torch.randn(3, 2 * 11, 64, device="cuda", generator=gen(5)).bfloat16()  # by the matrix cores
     for count in (2, 3, 5, 30, 39, 41, 60, 79):
         compare(c, q, table, n, count, 1, 1)
         compare(c, q, more, n, count, 1, 1)
+        compare(c, many, table, n, count, 1, 1)
     c.bounds.fill_(math.nan)  # none has been made: by index
     compare(c, q, table, n, 9, 0, 2)
 

@@ -124,13 +124,21 @@ def test_release_refuses(kv_pages, lib):
     p = pool(kv_pages)
     need = lib.vramc_pages_release_workspace(p, 8, 3)
     assert need == 16
-    ok = [p, P, 12, 8, P, 3, P, need, None]
+    ok = [p, P, 12, 8, at(0x30000), 3, P, need, None]
     for i, value, code in ((0, None, EARG), (1, None, EARG), (2, 7, EARG), (3, -1, EARG), (3, 1 << 26, EARG),
                            (4, None, EARG), (5, -1, EARG), (5, 4097, EARG), (6, None, EWORKSPACE),
                            (6, at(0x10004), EARG), (7, need - 1, EWORKSPACE)):
         bad = list(ok)
         bad[i] = value
         assert lib.vramc_pages_release(*bad) == code, (i, value)
+    table, size = 0x200000, 4 * (2 * 12 + 8)
+    for name, first, n in (("lengths", None, 12), ("free", 0x100000, 256), ("count", 0x110000, 4)):
+        for near in (0, n - 4, -size + 4):
+            args = list(ok)
+            args[1] = at((first or table) + near)
+            if first is None:
+                args[4] = at(table)
+            assert lib.vramc_pages_release(*args) == EARG, name
     for i in (3, 5):  # nothing to give back
         none = list(ok)
         none[i] = 0
@@ -229,6 +237,25 @@ def test_bound_and_select_refuse(kv, lib):
         assert lib.vramc_kv_select(*bad) == code, (i, value)
     ok[10] = 0  # no sequences
     assert lib.vramc_kv_select(*ok) == 0
+
+
+def test_select_writes_nothing_that_it_reads(kv, lib):
+    """Three sequences of two heads, 900 entries in rows 1000 apart, 8 pages each: some
+    workgroups write while others read."""
+    table, lengths, chosen, held, work = 0x100000, 0x200000, 0x300000, 0x400000, 0x500000
+    c, need = cache(kv), 3 * 2 * 900 * 8
+
+    def call(chosen=chosen, held=held):
+        return lib.vramc_kv_select(c, P, P, 512, 128, 4, at(table), 1000, 900, at(lengths), 3, 8, 1, 1, at(chosen),
+                                   at(held), at(work), need, None)
+    for first, n in ((table, 4 * 2900), (lengths, 12)):
+        for at_chosen in (first, first + n - 4, first - 6 * 8 * 4 + 4):
+            assert call(chosen=at_chosen) == EARG
+        for at_held in (first, first + n - 4, first - 6 * 4 + 4):
+            assert call(held=at_held) == EARG
+    assert call(held=chosen + 6 * 8 * 4 - 4) == EARG
+    if not torch.cuda.is_available():  # touching is not overlapping
+        assert call(chosen=lengths + 12) > 0 and call(held=table + 4 * 2900) > 0 and call(held=chosen + 6 * 8 * 4) > 0
 
 
 def test_fails_loudly_without_gpu(kv_pages, rotary):

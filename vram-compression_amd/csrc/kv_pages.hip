@@ -165,10 +165,77 @@ __device__ __forceinline__ int sum_of(int x, int* waves) {
     return sum;
 }
 
-// A workgroup to a row: how many pages it gives back, and then, in a second launch,
-// those behind what the rows before it do.  One workgroup that takes a small table
-// whole is no faster (one row of 8 entries 3.8 us against 3.6, 64 of 512 12.6 against
-// 4.7): it waits for its own reads.
+// Small tables by one workgroup: pieces of 256 entries of a row, up to kPieces to each
+// of its waves, four neighbouring entries to a lane, read once, counted, and then put
+// behind what the waves before have.  With extend, of one token each: a row of 512
+// entries 5.7 us, and 7.2 where two launches give pages back, 16 rows 7.8 and 9.3, 64
+// rows of 256 11.4 and 10.7, where a launch less is worth more to a host that is waited
+// for (2.7 us); 64 of 512, with twice the pieces, 14.5 and 11.0.
+constexpr int kAll = 1024, kAllWaves = kAll / 64, kPieces = 4;
+
+__global__ void __launch_bounds__(kAll) release_kernel(Release r) {
+    __shared__ int waves[kAllWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per_row = (r.width + 255) / 256, all = per_row * r.batch, each = (all + kAllWaves - 1) / kAllWaves;
+    const int first = min(wave * each, all - 1), mine = min(each, all - wave * each);
+    const int b0 = first / per_row, c0 = first - b0 * per_row;
+    const int have = min(max(*r.p.count, 0), r.p.pages);
+    using Four = vec<int, 4>;
+    Four x[kPieces];
+    int kept[kPieces];
+    const auto over = [&](auto f) {  // f(u, row, first of the lane's entries)
+        int b = b0, c = c0;
+#pragma unroll
+        for (int u = 0; u < kPieces; u++) {
+            if (u < mine) f(u, b, 256 * c + 4 * lane);
+            if (++c == per_row) c = 0, b++;
+        }
+    };
+    over([&](int u, int b, int i) {
+        x[u] = *reinterpret_cast<const Four*>(r.table + b * r.table_row + min(i, r.width - 4));
+        kept[u] = r.kept(b);
+    });
+    int n = 0;
+    over([&](int u, int, int i) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) n += __popcll(__ballot((i < r.width) & (i + e >= kept[u]) & r.is_page(x[u][e])));
+    });
+    if (lane == 0) waves[wave] = n;
+    __syncthreads();
+    int at = have, total = have;
+#pragma unroll
+    for (int w = 0; w < kAllWaves; w++) {
+        at += w < wave ? waves[w] : 0;
+        total += waves[w];
+    }
+    over([&](int u, int b, int i) {
+        Four y = x[u];
+        uint32_t to = at;
+        bool goes[4], changes = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool behind = (i < r.width) & (i + e >= kept[u]);
+            goes[e] = behind & r.is_page(x[u][e]);
+            changes |= behind & (x[u][e] != -1);
+            y[e] = behind ? -1 : x[u][e];
+            const uint64_t mask = __ballot(goes[e]);
+            to = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, to));
+            at += __popcll(mask);
+        }
+        if (!__any(changes)) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (goes[e]) {
+                if (to < (uint32_t)r.p.pages) r.p.free[to] = x[u][e];
+                to++;
+            }
+        if (changes) *reinterpret_cast<Four*>(r.table + b * r.table_row + i) = y;
+    });
+    if (threadIdx.x == 0) *r.p.count = min(total, r.p.pages);
+}
+
+// Larger tables, a workgroup to a row: how many pages it gives back, and then, in a
+// second launch, those behind what the rows before it do.
 __global__ void __launch_bounds__(kThreads) release_count_kernel(Release r) {
     __shared__ int waves[kWaves];
     const int b = blockIdx.x;
@@ -242,6 +309,12 @@ int check_table(const vramc_pages* p, int64_t table_row, int table_width, int ba
     return 0;
 }
 
+// Whether one workgroup takes the table.
+bool one_launch(const int32_t* table, int64_t table_row, int table_width, int batch) {
+    return ((uintptr_t)table % 16 | table_row % 4 | table_width % 4) == 0 &&
+           (int64_t)((table_width + 255) / 256) * batch <= kAllWaves * kPieces;
+}
+
 // Whether `bytes` at a and n integers at b share memory.
 bool overlap(const void* a, int64_t bytes, const int32_t* b, int64_t n) {
     return b && n > 0 && bytes > 0 && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)a + bytes;
@@ -286,11 +359,19 @@ extern "C" int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t
     if (const int rc = check_table(p, table_row, table_width, batch)) return rc;
     if (batch == 0 || table_width == 0) return 0;
     if (!table || !lengths) return RANS_EARG;
+    const int64_t entries = table_row * (batch - 1) + table_width;
+    if (overlap(table, 4 * entries, lengths, batch) || overlap(table, 4 * entries, p->free, p->pages) ||
+        overlap(table, 4 * entries, p->count, 1))
+        return RANS_EARG;
     if (!workspace || workspace_bytes < vramc_pages_release_workspace(p, table_width, batch)) return RANS_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return RANS_EARG;
     auto* counts = static_cast<int32_t*>(workspace);
     const Release r{*p, __builtin_ctz(p->page_size), table, table_row, table_width, lengths, batch, counts,
                     counts + batch};
+    if (one_launch(table, table_row, table_width, batch)) {
+        hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kAll), 0, stream, r);
+        return (int)hipGetLastError();
+    }
     hipLaunchKernelGGL(release_count_kernel, dim3((unsigned)batch), dim3(kThreads), 0, stream, r);
     if (const int rc = (int)hipGetLastError()) return rc;
     hipLaunchKernelGGL(release_rows_kernel, dim3((unsigned)batch), dim3(kThreads), 0, stream, r);

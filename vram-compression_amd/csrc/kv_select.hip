@@ -597,6 +597,11 @@ int select(const Select& a, int dim, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
+// Whether n integers at a share memory with m at b.
+bool overlap(const int32_t* a, int64_t n, const int32_t* b, int64_t m) {
+    return n > 0 && m > 0 && (uintptr_t)a < (uintptr_t)(b + m) && (uintptr_t)b < (uintptr_t)(a + n);
+}
+
 template <typename T, bool MX>
 int bound(const Bound& a, hipStream_t stream) {
     const int64_t blocks = (a.n + kWaves * a.each - 1) / (kWaves * a.each) * a.c.kv_heads;
@@ -653,6 +658,14 @@ extern "C" int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, cons
         return RANS_EARG;
     if (need && (!workspace || workspace_bytes < need)) return RANS_EWORKSPACE;
     if (need && (uintptr_t)workspace % 16) return RANS_EARG;
+    // Workgroups read these while others write.
+    const int64_t rows = (int64_t)batch * c->kv_heads, step = table_row * (batch - 1);
+    const int32_t* entries = table + (step < 0 ? step : 0);
+    const int64_t n = table_width ? (step < 0 ? -step : step) + table_width : 0;
+    if (overlap(chosen, rows * count, lengths, batch) || overlap(held, rows, lengths, batch) ||
+        overlap(chosen, rows * count, entries, n) || overlap(held, rows, entries, n) ||
+        overlap(chosen, rows * count, held, rows))
+        return RANS_EARG;
     const Select a{bounds, q, q_seq, q_head, q_heads / c->kv_heads, c->kv_heads, c->pages,
                    __builtin_ctz(c->page_size), table, table_row, table_width, lengths, batch, count, first, last,
                    (int)chunks_of(c->head_dim, q_heads / c->kv_heads, table_width), static_cast<uint64_t*>(workspace), chosen, held};
