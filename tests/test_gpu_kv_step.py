@@ -145,6 +145,28 @@ def test_sequences_come_and_go(bench):
     assert torch.equal(stack.step(h), fresh.step(h))
 
 
+def test_rows_used_again_are_evicted_in_time(bench):
+    """Prompts in rows that others have left: the budget holds for what a row holds now,
+    not for all that it ever has, and no token is refused."""
+    stack = bench.AttentionStack(layers=1, batch=2, budget=64, slack=16, recent=8, page=16, mx=False, pooled=True)
+    torch.manual_seed(5)
+    prompt = torch.randn(120, 1536, device="cuda").bfloat16()
+    for _ in range(3):
+        stack.write(prompt[:90], [60, 30])
+        stack.finish([0])
+        stack.write(prompt[:60], [60, 0])
+        stack.finish([0, 1])
+    assert stack.held == 0 and int(stack.pool.count) == stack.pool.pages
+    stack.write(prompt, [60, 60])
+    want = 60
+    for step in range(60):
+        stack.step(prompt[:2])
+        want = 64 if want == 79 else want + 1
+        assert stack.lengths.tolist() == [want] * 2 and stack.held == want
+    assert stack.seen.tolist() == [120] * 2
+    pages_are_whole(stack)
+
+
 def test_a_step_in_a_graph(bench):
     """A whole step of two layers, captured once and replayed with other tokens, lengths
     and pages, between eager work, against the same calls made eagerly."""

@@ -801,7 +801,8 @@ class AttentionStack:
         self.rows = torch.arange(batch, device="cuda")
         self.lengths = torch.zeros(batch, dtype=torch.int32, device="cuda")
         self.seen = torch.zeros(batch, dtype=torch.int32, device="cuda")
-        self.held = 0  # tokens of the longest sequence, as the host knows them
+        self.each = [0] * batch  # tokens of the sequences, as the host knows them,
+        self.held = 0            # and of the longest
         self.pool = None
         if pooled:
             self.pool = kv_pages.PagePool(batch * width, page)
@@ -825,13 +826,17 @@ class AttentionStack:
         """Prompts: new[b] (a list) tokens of each sequence, h (their sum, hidden), whose
         keys and values every layer keeps (what a prompt's tokens attend to is not
         computed).  No sequence may then hold more than the budget."""
-        self.held += max(new)
+        self.each = [n + m for n, m in zip(self.each, new)]
+        self.held = max(self.each)
         room = self._room(torch.tensor(new, dtype=torch.int32, device="cuda"), h.shape[0])
         for layer in self.layers:
             layer.write(h, *room)
 
     def finish(self, sequences):
-        """Ends sequences (rows); their pages are free again."""
+        """Ends sequences (a list of rows); their pages are free again."""
+        for s in sequences:
+            self.each[s] = 0
+        self.held = max(self.each)
         self.lengths[sequences] = 0
         self.seen[sequences] = 0
         self.pool.release(self.table, self.lengths)
@@ -848,13 +853,15 @@ class AttentionStack:
             self.seen += 1
         else:
             slots, positions, filled = self._room(self.one, self.batch)
-        self.held += 1
+        self.each = [n + 1 for n in self.each]
+        self.held = max(self.each)
         for layer in self.layers:
             h = layer(h, self.table, self.lengths, slots, positions, filled)
-        if self.held == self.budget + self.slack:
+        if self.held >= self.budget + self.slack:
             for layer in self.layers:
                 left = layer.cache.evict(self.table, self.lengths, self.seen, self.budget, self.recent)
-            self.lengths, self.held = left, self.budget
+            self.lengths, self.each = left, [min(n, self.budget) for n in self.each]
+            self.held = max(self.each)
             if self.pool is not None:
                 self.pool.release(self.table, self.lengths)
             for layer in self.layers:
