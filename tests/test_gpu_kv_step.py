@@ -167,6 +167,16 @@ def test_rows_used_again_are_evicted_in_time(bench):
     pages_are_whole(stack)
 
 
+def test_chosen_pages_need_filled(bench):
+    """A layer that chooses pages by bounds is told which pages became full."""
+    stack = bench.AttentionStack(layers=1, batch=1, budget=64, slack=16, page=16, mx=False, pooled=True, count=2)
+    layer, h = stack.layers[0], torch.zeros(1, 1536, device="cuda", dtype=torch.bfloat16)
+    room = stack.pool.extend(stack.table, stack.lengths, stack.one, 1)
+    with pytest.raises(ValueError, match="filled"):
+        layer(h, stack.table, room.lengths, room.slots, room.positions)
+    assert not layer.cache.k.any() and not layer.cache.v.any()
+
+
 def test_a_step_in_a_graph(bench):
     """A whole step of two layers, captured once and replayed with other tokens, lengths
     and pages, between eager work, against the same calls made eagerly."""

@@ -769,7 +769,10 @@ class AttentionLayer(torch.nn.Module):
 
     def forward(self, h, table, lengths, slots, positions, filled=None):
         """One new token of each sequence: h (sequences, hidden) in the cache's
-        dtype; lengths counts the new tokens, slots and positions are theirs."""
+        dtype; lengths counts the new tokens, slots and positions are theirs, filled
+        (where pages are chosen) the pages that they make full."""
+        if self.count and filled is None:
+            raise ValueError("pages are chosen by their bounds, which the layer keeps by filled")
         c, q = self.cache, self.write(h, slots, positions, filled)
         if self.count:
             out = c.attend_selected(q, *c.select(q, table, lengths, self.count))
