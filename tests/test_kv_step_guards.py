@@ -120,6 +120,21 @@ def test_extend_next_to_what_it_reads(kv_pages, lib):
         assert extend(kv_pages, lib, **kw) > 0, kw
 
 
+@pytest.mark.parametrize("name,size", [("lengths", 12), ("fresh", 12), ("seen", 12), ("free", 256), ("count", 4),
+                                       ("ticket", 4)])
+def test_extend_writes_no_table_that_it_reads_besides(kv_pages, lib, name, size):
+    table, end = EXTEND["table"], EXTEND["table"] + 4 * (2 * 12 + 8)
+    for address in (table, end - 4, table - size + 4):
+        kw = {name: address}
+        assert (extend(kv_pages, lib, **kw) if name in EXTEND else extend(kv_pages, lib, kw)) == EARG, hex(address)
+
+
+def test_release_reads_no_lengths_where_it_writes(kv_pages, lib):
+    for first, n in ((0x100000, 256), (0x110000, 4)):
+        for address in (first, first + n - 4, first - 12 + 4):
+            assert lib.vramc_pages_release(pool(kv_pages), P, 12, 8, at(address), 3, at(0x300000), 16, None) == EARG
+
+
 def test_release_refuses(kv_pages, lib):
     p = pool(kv_pages)
     need = lib.vramc_pages_release_workspace(p, 8, 3)

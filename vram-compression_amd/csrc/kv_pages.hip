@@ -335,6 +335,10 @@ extern "C" int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t 
         {slots, tokens * 8}, {positions, tokens * 4}, {filled, tokens * 4},
         {starts, 4 * ((int64_t)batch + 1)}, {new_lengths, 4 * (int64_t)batch}};
     const int64_t entries = batch ? table_row * (batch - 1) + table_width : 0;
+    const int64_t size = 4 * entries;
+    if (overlap(table, size, lengths, batch) || overlap(table, size, fresh, batch) || overlap(table, size, seen, batch) ||
+        overlap(table, size, p->free, p->pages) || overlap(table, size, p->count, 1) || overlap(table, size, p->ticket, 1))
+        return RANS_EARG;
     for (const auto& o : outs)
         if (overlap(o.at, o.bytes, lengths, batch) || overlap(o.at, o.bytes, fresh, batch) ||
             overlap(o.at, o.bytes, seen, batch) || overlap(o.at, o.bytes, table, entries) ||
@@ -361,7 +365,8 @@ extern "C" int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t
     if (!table || !lengths) return RANS_EARG;
     const int64_t entries = table_row * (batch - 1) + table_width;
     if (overlap(table, 4 * entries, lengths, batch) || overlap(table, 4 * entries, p->free, p->pages) ||
-        overlap(table, 4 * entries, p->count, 1))
+        overlap(table, 4 * entries, p->count, 1) || overlap(lengths, 4 * (int64_t)batch, p->free, p->pages) ||
+        overlap(lengths, 4 * (int64_t)batch, p->count, 1))
         return RANS_EARG;
     if (!workspace || workspace_bytes < vramc_pages_release_workspace(p, table_width, batch)) return RANS_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return RANS_EARG;
