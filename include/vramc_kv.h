@@ -119,10 +119,13 @@ int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, voi
  * all of them where there are at most `count`, or else the first `first`, the last
  * `last` and those of the largest score,
  *   score = max over the kv head's query heads of sum_d max(q_d lo_d, q_d hi_d),
- * which no q . k of the page exceeds, lo and hi its bounds; in 64 bits, ties to the
- * lower index, a score that is not a number before all others, an entry that is no
- * page behind all (any pages where a query is not finite).  0 <= first, 1 <= last, first + last <= count.  lengths are cut
- * to 0 and table_width * page_size.
+ * which no q . k of the page exceeds, lo and hi its bounds; ties to the lower index, a
+ * score that is not a number before all others, an entry that is no page behind all
+ * (any pages where a query is not finite).  Sums are in 64 bits and of the larger
+ * products alone, in one order for all pages of a call: pages with the same products
+ * tie, others whose scores differ by less than that rounding may change places.
+ * 0 <= first, 1 <= last, first + last <= count.  lengths are cut to 0 and
+ * table_width * page_size.
  * chosen[b*kv_heads + h][count]: the pages in order of the sequence's, page * kv_heads
  * + h (a page of the same tensors taken as a cache of pages * kv_heads pages of one
  * head), -1 for an entry that is none and behind the last; held[b*kv_heads + h]: the

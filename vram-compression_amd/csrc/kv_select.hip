@@ -228,8 +228,9 @@ __device__ __forceinline__ double row_sum(double x, int lanes) {
 }
 
 // Few query heads: a wave scores two pages on each row of its lanes, eight columns a
-// lane.  q_d lo_d or q_d hi_d is q_d (hi_d + lo_d) / 2 + |q_d| (hi_d - lo_d) / 2
-// whatever the sign: two multiply-adds a column and query head.
+// lane.  q_d lo_d or q_d hi_d is min(q_d, 0) lo_d + max(q_d, 0) hi_d, of which one is a
+// zero: what a query does not point to leaves no rounding behind, so that pages alike
+// where it points have the same score to the bit.
 template <typename T>
 struct Few {
     const Select& a;
@@ -264,15 +265,12 @@ struct Few {
         }
     }
     __device__ __forceinline__ void score(const double* query, double (&best)[kSets]) const {
-        double sum[kSets][kPer], gap[kSets][kPer];
+        double low[kSets][kPer], high[kSets][kPer];
 #pragma unroll
         for (int s = 0; s < kSets; s++) {
-            const auto low = __builtin_bit_cast(vec<T, kPer>, raw[s][0]), high = __builtin_bit_cast(vec<T, kPer>, raw[s][1]);
+            const auto x = __builtin_bit_cast(vec<T, kPer>, raw[s][0]), y = __builtin_bit_cast(vec<T, kPer>, raw[s][1]);
 #pragma unroll
-            for (int j = 0; j < kPer; j++) {
-                sum[s][j] = wide(high[j]) + wide(low[j]);
-                gap[s][j] = wide(high[j]) - wide(low[j]);
-            }
+            for (int j = 0; j < kPer; j++) low[s][j] = wide(x[j]), high[s][j] = wide(y[j]);
             best[s] = -__builtin_inf();
         }
         const int at = inside ? seg : 0;
@@ -283,12 +281,14 @@ struct Few {
             for (int p = 0; p < kPer / 2; p++) {
                 const auto v = *reinterpret_cast<const vec<double, 2>*>(query + ((g * (kPer / 2) + p) * per_row + at) * 2);
 #pragma unroll
-                for (int s = 0; s < kSets; s++)
+                for (int i = 0; i < 2; i++) {  // of halves: the query's value or 0, exactly
+                    const double below = v[i] - __builtin_fabs(v[i]), above = v[i] + __builtin_fabs(v[i]);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        x[s] = __builtin_fma(v[i], sum[s][2 * p + i], x[s]);
-                        y[s] = __builtin_fma(__builtin_fabs(v[i]), gap[s][2 * p + i], y[s]);
+                    for (int s = 0; s < kSets; s++) {
+                        x[s] = __builtin_fma(below, low[s][2 * p + i], x[s]);
+                        y[s] = __builtin_fma(above, high[s][2 * p + i], y[s]);
                     }
+                }
             }
 #pragma unroll
             for (int s = 0; s < kSets; s++) {
