@@ -918,7 +918,8 @@ def serve(layers=2, batch=4, longest=32768, count=64, steps=64):
     def step():  # what a graph replays: lengths in place
         room, x = stack.pool.extend(stack.table, lengths, stack.one, batch, seen), h
         for layer in stack.layers:
-            x = layer(x, stack.table, room.lengths, room.slots, room.positions, room.filled)
+            x = layer(x, stack.table, room.lengths, room.slots, room.positions,
+                      room.filled if layer.count else None)  # all pages need no bounds
         seen.add_(room.lengths - lengths)
         lengths.copy_(room.lengths)
         return x
@@ -926,6 +927,8 @@ def serve(layers=2, batch=4, longest=32768, count=64, steps=64):
     def timed(count):
         for layer in stack.layers:
             layer.count = count
+            if count:  # of pages that have become full without
+                layer.cache.bound(stack.table)
         step()
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
