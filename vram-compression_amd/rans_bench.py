@@ -828,12 +828,20 @@ class AttentionStack:
     def write(self, h, new):
         """Prompts: new[b] (a list) tokens of each sequence, h (their sum, hidden), whose
         keys and values every layer keeps (what a prompt's tokens attend to is not
-        computed).  No sequence may then hold more than the budget."""
-        self.each = [n + m for n, m in zip(self.each, new)]
-        self.held = max(self.each)
+        computed).  A sequence then holds fewer than budget + slack tokens, so that the
+        next step's has a place.  Returns the rows (a list) whose prompt got no room, as
+        their pages are not in the pool: they hold what they held."""
+        if len(new) != self.batch or any(m < 0 for m in new) or sum(new) != h.shape[0]:
+            raise ValueError(f"prompts of {new} tokens, {h.shape[0]} rows of them and {self.batch} sequences")
+        most = max(n + m for n, m in zip(self.each, new))
+        if most >= self.budget + self.slack:
+            raise ValueError(f"a sequence of {most} tokens and a next one: the row has {self.budget + self.slack}")
         room = self._room(torch.tensor(new, dtype=torch.int32, device="cuda"), h.shape[0])
         for layer in self.layers:
             layer.write(h, *room)
+        before, self.each = self.each, self.lengths.tolist()
+        self.held = max(self.each)
+        return [b for b, m in enumerate(new) if self.each[b] != before[b] + m]
 
     def finish(self, sequences):
         """Ends sequences (a list of rows); their pages are free again."""
