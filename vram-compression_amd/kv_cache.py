@@ -89,8 +89,8 @@ def _check(ok, message):
 def _failed(name, rc):
     """Raises what a return value of the library says."""
     if rc < 0:
-        raise ValueError(f"{name}: refused by the library ({rc}): more than one launch holds, or a tensor "
-                         "less aligned than the kernels read")
+        raise ValueError(f"{name}: refused by the library ({rc}): more than one launch holds, a tensor less "
+                         "aligned than the kernels read, or one that is written in the memory of another")
     raise RuntimeError(f"{name}: HIP error {rc}")
 
 
