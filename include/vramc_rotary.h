@@ -43,16 +43,17 @@ typedef struct vramc_rotary_rows {
 } vramc_rotary_rows;
 
 /* q_out, k_out: [tokens][heads][head_dim] of dtype, 16-byte aligned, sharing no
- * memory with each other or what is read (RANS_EARG).  Everything is computed in f32 (the angle in 64 bits up
- * to its whole turns) and rounded once; the norm of a head whose squares leave f32 is
- * no number of use. */
+ * memory with each other or what is read (RANS_EARG).  Everything is computed in f32
+ * (the angle in 64 bits up to its whole turns) and rounded once; the norm of a head
+ * whose squares leave f32 is no number of use. */
 int vramc_rotary_apply(const vramc_rotary* r, const vramc_rotary_rows* x, void* q_out, void* k_out,
                        hipStream_t stream);
 
 /* The same, with the keys rounded to dtype and written, as vramc_kv_append writes
  * them, into the slots of a cache of the same dtype, head_dim and k_heads heads,
  * with the values v; where it has them, the slot's mass becomes 0 and its position
- * the token's.  k of x stays as it is. */
+ * the token's.  k of x stays as it is.  The cache's tensors share no memory with what
+ * is read or q_out (RANS_EARG). */
 int vramc_rotary_append(const vramc_rotary* r, const vramc_rotary_rows* x, const vramc_kv_cache* c,
                         const void* v, int64_t v_token, int64_t v_head, const int64_t* slots,
                         void* q_out, hipStream_t stream);

@@ -1,7 +1,11 @@
 """Calls whose outputs lie over what they read, without a GPU: refused by the library
 before any HIP call, with a message that says so."""
+import ctypes
+
 import pytest
 import torch
+
+EARG = -4
 
 pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="a GPU is present, and the memory is none of its own")
 
@@ -29,3 +33,88 @@ def test_what_is_refused_is_named(host):
     for call in (lambda: pool.extend(table, table[1, :3], n, 5), lambda: pool.release(table, table[1, :3])):
         with pytest.raises(ValueError, match="memory"):
             call()
+
+
+# Addresses 1 MiB apart, in the order of their names; never dereferenced.
+def places(*names):
+    return {name: 0x10000000 + (i << 20) for i, name in enumerate(names)}
+
+
+def each_pair(call, written, read):
+    """Every output over every input, at its first and its last bytes, is refused; next
+    to it, it gets as far as a HIP call.  written, read: bytes by name."""
+    assert call() > 0
+    for out, size in written.items():
+        for name, n in read.items():
+            if name == out:
+                continue
+            first = at[name]
+            for address in (first, first + n - 16, first - size + 16):
+                assert call(**{out: address & -16}) == EARG, (out, name, hex(address - first))
+            for address in (first + n + 16, first - size):
+                assert call(**{out: address & -16}) > 0, (out, name, "beside")
+
+
+TOKENS, Q_HEADS, K_HEADS, DIM = 10, 4, 2, 64
+at = places("q", "k", "v", "q_weight", "k_weight", "positions", "turns", "slots", "q_out", "k_out", "pages_k",
+            "pages_v", "scales_k", "scales_v", "mass", "place", "bounds", "list", "table", "lengths", "chosen", "held",
+            "work", "free", "count", "ticket", "fresh", "seen", "filled", "starts", "grown")
+# q and k are columns of one projection, as far as its last row's
+ROWS = {"q": ((TOKENS - 1) * 400 + Q_HEADS * DIM) * 2, "k": ((TOKENS - 1) * 400 + K_HEADS * DIM) * 2, "q_weight": DIM * 4,
+        "k_weight": DIM * 4, "positions": TOKENS * 4, "turns": 16 * 8}
+PAGES, PAGE = 8, 16
+CACHE = {"pages_k": PAGES * K_HEADS * PAGE * DIM * 2, "pages_v": PAGES * K_HEADS * PAGE * DIM * 2,
+         "mass": PAGES * K_HEADS * PAGE * 4, "place": PAGES * K_HEADS * PAGE * 4}
+CACHE_MX = {**CACHE, "pages_k": PAGES * K_HEADS * PAGE * DIM // 2, "pages_v": PAGES * K_HEADS * PAGE * DIM // 2,
+            "scales_k": PAGES * K_HEADS * PAGE * DIM // 32, "scales_v": PAGES * K_HEADS * PAGE * DIM // 32}
+
+
+def rotation(rotary, kw):
+    a = {**at, **kw}
+    r = rotary.RotaryDesc(DIM, 16, 0, 1.0, a["turns"])
+    x = rotary.RowsDesc(a["q"], a["k"], 400, DIM, 400, DIM, Q_HEADS, K_HEADS, a["q_weight"], a["k_weight"], 1, 0, 1e-6,
+                        a["positions"], TOKENS)  # bf16, weights of f32
+    return a, ctypes.byref(r), ctypes.byref(x)
+
+
+def cache_of(kv_cache, a, mx):
+    return ctypes.byref(kv_cache.KvCacheDesc(
+        pages=PAGES, kv_heads=K_HEADS, page_size=PAGE, head_dim=DIM, dtype=1, mx=int(mx), k=a["pages_k"], v=a["pages_v"],
+        k_scale=a["scales_k"] if mx else None, v_scale=a["scales_v"] if mx else None, mass=a["mass"],
+        position=a["place"]))
+
+
+def test_rotate_writes_nothing_that_it_reads(host, lib):
+    import rotary
+
+    def call(**kw):
+        a, r, x = rotation(rotary, kw)
+        return lib.vramc_rotary_apply(r, x, a["q_out"], a["k_out"], None)
+    out = {"q_out": TOKENS * Q_HEADS * DIM * 2, "k_out": TOKENS * K_HEADS * DIM * 2}
+    each_pair(call, out, {**ROWS, **out})
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_append_writes_nothing_that_it_reads(host, lib, mx):
+    """The queries, and every tensor of the cache."""
+    import kv_cache
+    import rotary
+
+    def call(**kw):
+        a, r, x = rotation(rotary, kw)
+        return lib.vramc_rotary_append(r, x, cache_of(kv_cache, a, mx), a["v"], 400, DIM, a["slots"], a["q_out"], None)
+    read = {**ROWS, "v": ((TOKENS - 1) * 400 + K_HEADS * DIM) * 2, "slots": TOKENS * 8}
+    pages = CACHE_MX if mx else CACHE
+    each_pair(call, {"q_out": TOKENS * Q_HEADS * DIM * 2}, {**read, **pages})
+    each_pair(call, pages, read)
+
+
+def test_append_of_the_cache_s_own_rows(host):
+    cache, _, turn = host
+    x, n = torch.zeros(8, 2, 64), torch.zeros(8, dtype=torch.int32)
+    slots, own = torch.arange(8), cache.v[:, :, 3]
+    for q, k, v in ((x, x, own), (x, own, x), (own, x, x)):
+        with pytest.raises(ValueError, match="memory"):
+            turn.append(cache, q, k, v, slots, n)
+    with pytest.raises(ValueError, match="memory"):
+        turn.append(cache, x, x, x, slots, cache.position.view(-1)[:8])

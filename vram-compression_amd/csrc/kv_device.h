@@ -134,6 +134,41 @@ inline int check_cache(const vramc_kv_cache* c) {
     return 0;
 }
 
+// Memory that a call reads or writes; no address or no bytes: none.
+struct Span {
+    const void* at;
+    int64_t bytes;
+};
+inline bool overlap(Span a, Span b) {
+    return a.at && b.at && a.bytes > 0 && b.bytes > 0 && (uintptr_t)a.at < (uintptr_t)b.at + b.bytes &&
+           (uintptr_t)b.at < (uintptr_t)a.at + a.bytes;
+}
+template <size_t N, size_t M>
+bool overlap(const Span (&a)[N], const Span (&b)[M]) {
+    for (const Span& x : a)
+        for (const Span& y : b)
+            if (overlap(x, y)) return true;
+    return false;
+}
+
+// Values of rows, rows x[t * token + h * head] of `dim`, strides not negative.
+inline Span span_of(const void* x, int64_t token, int64_t head, int64_t tokens, int64_t heads, int64_t dim, int64_t size) {
+    return {x, tokens && heads ? ((tokens - 1) * token + (heads - 1) * head + dim) * size : 0};
+}
+
+// The tensors of a cache.
+struct CacheSpans {
+    Span of[6];
+};
+inline CacheSpans spans_of(const vramc_kv_cache& c) {
+    const int64_t pages = (int64_t)c.pages * c.kv_heads, most = INT64_MAX >> 20;  // more do not exist
+    const int64_t tokens = (pages < most ? pages : most) * c.page_size;
+    const int64_t values = tokens * c.head_dim, size = c.dtype == RANS_X_F32 ? 4 : 2;
+    const int64_t held = c.mx ? values / 2 : values * size, scales = c.mx ? values / 32 : 0;
+    return {{{c.k, held}, {c.v, held}, {c.k_scale, scales}, {c.v_scale, scales}, {c.mass, 4 * tokens},
+             {c.position, 4 * tokens}}};
+}
+
 }  // namespace
 
 #endif  // VRAMC_KV_DEVICE_H

@@ -233,12 +233,17 @@ int check(const vramc_rotary* r, const vramc_rotary_rows* x) {
     return 0;
 }
 
-// Whether a dense output shares memory with rows that are read.
-bool overlap(const void* out, int64_t bytes, const void* x, int64_t token, int64_t head, int64_t tokens, int64_t heads,
-             int64_t dim, int64_t size) {
-    if (!bytes || !tokens || !heads) return false;
-    const int64_t all = ((tokens - 1) * token + (heads - 1) * head + dim) * size;
-    return (uintptr_t)out < (uintptr_t)x + all && (uintptr_t)x < (uintptr_t)out + bytes;
+int64_t size_of(int dtype) { return dtype == RANS_X_F32 ? 4 : 2; }
+
+// What both calls read.
+struct RowsSpans {
+    Span of[6];
+};
+RowsSpans spans_of(const vramc_rotary& r, const vramc_rotary_rows& x) {
+    const int64_t dim = r.head_dim, size = size_of(x.dtype), weight = dim * size_of(x.weight_dtype);
+    return {{span_of(x.q, x.q_token, x.q_head, x.tokens, x.q_heads, dim, size),
+             span_of(x.k, x.k_token, x.k_head, x.tokens, x.k_heads, dim, size),
+             {x.q_weight, weight}, {x.k_weight, weight}, {x.positions, x.tokens * 4}, {r.turns, r.pairs * (int64_t)8}}};
 }
 
 template <typename T>
@@ -296,14 +301,9 @@ extern "C" int vramc_rotary_apply(const vramc_rotary* r, const vramc_rotary_rows
     if (const int rc = check(r, x)) return rc;
     if (x->tokens == 0) return 0;
     if ((x->q_heads && !q_out) || (x->k_heads && !k_out) || ((uintptr_t)q_out | (uintptr_t)k_out) % 16) return RANS_EARG;
-    const int64_t size = x->dtype == RANS_X_F32 ? 4 : 2, dim = r->head_dim;
-    const struct { const void* at; int64_t bytes; } outs[] = {{q_out, x->tokens * x->q_heads * dim * size},
-                                                              {k_out, x->tokens * x->k_heads * dim * size}};
-    if (overlap(q_out, outs[0].bytes, k_out, x->k_heads * dim, dim, x->tokens, x->k_heads, dim, size)) return RANS_EARG;
-    for (const auto& o : outs)
-        if (overlap(o.at, o.bytes, x->q, x->q_token, x->q_head, x->tokens, x->q_heads, dim, size) ||
-            overlap(o.at, o.bytes, x->k, x->k_token, x->k_head, x->tokens, x->k_heads, dim, size))
-            return RANS_EARG;
+    const int64_t value = size_of(x->dtype) * r->head_dim;
+    const Span out[] = {{q_out, x->tokens * x->q_heads * value}, {k_out, x->tokens * x->k_heads * value}};
+    if (overlap(out[0], out[1]) || overlap(out, spans_of(*r, *x).of)) return RANS_EARG;
     const auto go = [&](auto fn) { return fn(*r, *x, nullptr, nullptr, 0, 0, nullptr, q_out, k_out, stream); };
     if (x->dtype == RANS_X_F32) return go(launch<float, kTensor>);
     return x->dtype == RANS_X_BF16 ? go(launch<__bf16, kTensor>) : go(launch<_Float16, kTensor>);
@@ -318,10 +318,13 @@ extern "C" int vramc_rotary_append(const vramc_rotary* r, const vramc_rotary_row
         return RANS_EARG;
     if (x->tokens == 0) return 0;
     if (!v || !slots || (x->q_heads && !q_out) || (uintptr_t)q_out % 16) return RANS_EARG;
-    const int64_t size = x->dtype == RANS_X_F32 ? 4 : 2, dim = r->head_dim, bytes = x->tokens * x->q_heads * dim * size;
-    if (overlap(q_out, bytes, x->q, x->q_token, x->q_head, x->tokens, x->q_heads, dim, size) ||
-        overlap(q_out, bytes, x->k, x->k_token, x->k_head, x->tokens, x->k_heads, dim, size) ||
-        overlap(q_out, bytes, v, v_token, v_head, x->tokens, x->k_heads, dim, size))
+    const Span out[] = {{q_out, x->tokens * x->q_heads * size_of(x->dtype) * r->head_dim}};
+    const Span more[] = {span_of(v, v_token, v_head, x->tokens, x->k_heads, r->head_dim, size_of(x->dtype)),
+                         {slots, x->tokens * 8}};
+    const auto read = spans_of(*r, *x);
+    const auto pages = spans_of(*c);
+    if (overlap(out, read.of) || overlap(out, more) || overlap(out, pages.of) || overlap(pages.of, read.of) ||
+        overlap(pages.of, more))
         return RANS_EARG;
     const auto go = [&](auto fn) { return fn(*r, *x, c, v, v_token, v_head, slots, q_out, nullptr, stream); };
     if (x->dtype == RANS_X_F32) return go(launch<float, kPlain>);

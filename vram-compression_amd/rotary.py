@@ -163,7 +163,8 @@ class Rotary(kv_cache.Calls):
     def append(self, cache, q, k, v, slots, positions, q_weight=None, k_weight=None, eps=1e-6):
         """rotate, with the keys and the values v (as k, any strides) written into slots
         (int64) of a cache, as PagedCache.append writes them; a tracked one takes the
-        positions too.  Returns the queries, also of tokens without a slot (-1)."""
+        positions too.  Returns the queries, also of tokens without a slot (-1).  What is
+        read lies in none of the cache's tensors."""
         if cache.head_dim != self.head_dim or cache.dtype is not q.dtype or cache._index != self._index:
             raise ValueError(f"a cache of {cache.dtype} heads of {cache.head_dim} on {cache.device} takes no "
                              f"{q.dtype} of {self.head_dim} on {self.device}")
