@@ -111,7 +111,8 @@ int vramc_kv_evict(const vramc_kv_cache* c, const int32_t* table, int64_t table_
 /* The smallest and largest key of each column of n pages (a number that is no page
  * of the cache is skipped): bounds[page][kv_head][0 and 1][head_dim] of dtype,
  * 16-byte aligned, over all places of the page; NaN in both where a column has a
- * key that is not finite. */
+ * key that is not finite.  They share no memory with the cache's tensors or the list
+ * (RANS_EARG). */
 int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, void* bounds,
                    hipStream_t stream);
 
@@ -129,9 +130,10 @@ int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, voi
  * chosen[b*kv_heads + h][count]: the pages in order of the sequence's, page * kv_heads
  * + h (a page of the same tensors taken as a cache of pages * kv_heads pages of one
  * head), -1 for an entry that is none and behind the last; held[b*kv_heads + h]: the
- * tokens in them, so that vramc_kv_attend takes both as table and lengths; neither
- * shares memory with the other, lengths or table (RANS_EARG).
- * workspace: vramc_kv_select_workspace bytes, no content expected, 16-byte aligned. */
+ * tokens in them, so that vramc_kv_attend takes both as table and lengths.
+ * workspace: vramc_kv_select_workspace bytes, no content expected, 16-byte aligned,
+ * private to the call until its kernels have run.  chosen, held and the workspace share
+ * no memory with one another or with what is read (RANS_EARG). */
 int64_t vramc_kv_select_workspace(const vramc_kv_cache* c, int q_heads, int table_width, int batch,
                                   int count);
 int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, const void* q, int64_t q_seq,

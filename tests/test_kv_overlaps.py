@@ -118,3 +118,32 @@ def test_append_of_the_cache_s_own_rows(host):
             turn.append(cache, q, k, v, slots, n)
     with pytest.raises(ValueError, match="memory"):
         turn.append(cache, x, x, x, slots, cache.position.view(-1)[:8])
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_bound_writes_nothing_that_it_reads(host, lib, mx):
+    import kv_cache
+
+    def call(**kw):
+        a = {**at, **kw}
+        return lib.vramc_kv_bound(cache_of(kv_cache, a, mx), a["list"], 12, a["bounds"], None)
+    each_pair(call, {"bounds": PAGES * K_HEADS * 2 * DIM * 2}, {"list": 48, **(CACHE_MX if mx else CACHE)})
+
+
+@pytest.mark.parametrize("turned", [False, True])
+def test_select_writes_nothing_that_it_reads(host, lib, turned):
+    """Three sequences, 900 entries in rows 1000 apart, scored in a launch of their own;
+    the queries' sequences may come in either order."""
+    import kv_cache
+    need = lib.vramc_kv_select_workspace(cache_of(kv_cache, at, False), Q_HEADS, 900, 3, 8)
+    assert need == 3 * K_HEADS * 900 * 8
+    last = 2 * 400 if turned else 0
+
+    def call(**kw):
+        a = {**at, **kw}
+        return lib.vramc_kv_select(cache_of(kv_cache, a, False), a["bounds"], a["q"] + 2 * last, -400 if turned else 400,
+                                   DIM, Q_HEADS, a["table"], 1000, 900, a["lengths"], 3, 8, 1, 1, a["chosen"], a["held"],
+                                   a["work"], need, None)
+    out = {"chosen": 3 * K_HEADS * 8 * 4, "held": 3 * K_HEADS * 4, "work": need}
+    each_pair(call, out, {"bounds": PAGES * K_HEADS * 2 * DIM * 2, "q": (2 * 400 + Q_HEADS * DIM) * 2,
+                          "table": (2 * 1000 + 900) * 4, "lengths": 12, **out})

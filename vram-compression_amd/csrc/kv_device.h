@@ -151,9 +151,19 @@ bool overlap(const Span (&a)[N], const Span (&b)[M]) {
     return false;
 }
 
-// Values of rows, rows x[t * token + h * head] of `dim`, strides not negative.
+// Rows of `dim` values of `size` bytes each, x[t * token + h * head].
 inline Span span_of(const void* x, int64_t token, int64_t head, int64_t tokens, int64_t heads, int64_t dim, int64_t size) {
-    return {x, tokens && heads ? ((tokens - 1) * token + (heads - 1) * head + dim) * size : 0};
+    if (!x || tokens <= 0 || heads <= 0 || dim <= 0) return {};
+    const int64_t far[] = {(tokens - 1) * token, (heads - 1) * head};
+    int64_t first = 0, end = dim;
+    for (const int64_t f : far) (f < 0 ? first : end) += f;
+    return {static_cast<const char*>(x) + first * size, (end - first) * size};
+}
+
+// Pages of a cache's heads; more than these do not exist.
+inline int64_t head_pages(const vramc_kv_cache& c) {
+    const int64_t n = (int64_t)c.pages * c.kv_heads, most = INT64_MAX >> 20;
+    return n < most ? n : most;
 }
 
 // The tensors of a cache.
@@ -161,8 +171,7 @@ struct CacheSpans {
     Span of[6];
 };
 inline CacheSpans spans_of(const vramc_kv_cache& c) {
-    const int64_t pages = (int64_t)c.pages * c.kv_heads, most = INT64_MAX >> 20;  // more do not exist
-    const int64_t tokens = (pages < most ? pages : most) * c.page_size;
+    const int64_t tokens = head_pages(c) * c.page_size;
     const int64_t values = tokens * c.head_dim, size = c.dtype == RANS_X_F32 ? 4 : 2;
     const int64_t held = c.mx ? values / 2 : values * size, scales = c.mx ? values / 32 : 0;
     return {{{c.k, held}, {c.v, held}, {c.k_scale, scales}, {c.v_scale, scales}, {c.mass, 4 * tokens},

@@ -597,11 +597,6 @@ int select(const Select& a, int dim, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
-// Whether n integers at a share memory with m at b.
-bool overlap(const int32_t* a, int64_t n, const int32_t* b, int64_t m) {
-    return n > 0 && m > 0 && (uintptr_t)a < (uintptr_t)(b + m) && (uintptr_t)b < (uintptr_t)(a + n);
-}
-
 template <typename T, bool MX>
 int bound(const Bound& a, hipStream_t stream) {
     const int64_t blocks = (a.n + kWaves * a.each - 1) / (kWaves * a.each) * a.c.kv_heads;
@@ -617,6 +612,10 @@ int bound(const Bound& a, hipStream_t stream) {
     return (int)hipGetLastError();
 }
 
+Span span_of_bounds(const vramc_kv_cache& c, const void* bounds) {
+    return {bounds, head_pages(c) * 2 * c.head_dim * (c.dtype == RANS_X_F32 ? 4 : 2)};
+}
+
 }  // namespace
 
 extern "C" int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int64_t n, void* bounds,
@@ -625,6 +624,9 @@ extern "C" int vramc_kv_bound(const vramc_kv_cache* c, const int32_t* pages, int
     if (n < 0 || n > INT64_MAX / 65536) return RANS_EARG;
     if (n == 0) return 0;
     if (!pages || !bounds || (uintptr_t)bounds % 16) return RANS_EARG;
+    // Waves read these while others write.
+    const Span out[] = {span_of_bounds(*c, bounds)};
+    if (overlap(out[0], Span{pages, n * 4}) || overlap(out, spans_of(*c).of)) return RANS_EARG;
     const Bound a{*c, __builtin_ctz(c->page_size), lanes_of(c->head_dim), pages, n, bounds,
                   (n * c->kv_heads + kBoundWaves - 1) / kBoundWaves};
     if (c->dtype == RANS_X_F32) return bound<float, false>(a, stream);
@@ -659,12 +661,12 @@ extern "C" int vramc_kv_select(const vramc_kv_cache* c, const void* bounds, cons
     if (need && (!workspace || workspace_bytes < need)) return RANS_EWORKSPACE;
     if (need && (uintptr_t)workspace % 16) return RANS_EARG;
     // Workgroups read these while others write.
-    const int64_t rows = (int64_t)batch * c->kv_heads, step = table_row * (batch - 1);
-    const int32_t* entries = table + (step < 0 ? step : 0);
-    const int64_t n = table_width ? (step < 0 ? -step : step) + table_width : 0;
-    if (overlap(chosen, rows * count, lengths, batch) || overlap(held, rows, lengths, batch) ||
-        overlap(chosen, rows * count, entries, n) || overlap(held, rows, entries, n) ||
-        overlap(chosen, rows * count, held, rows))
+    const int64_t rows = (int64_t)batch * c->kv_heads;
+    const Span out[] = {{chosen, rows * count * 4}, {held, rows * 4}, {workspace, need}};
+    const Span read[] = {
+        span_of_bounds(*c, bounds), {lengths, batch * (int64_t)4}, span_of(table, table_row, 0, batch, 1, table_width, 4),
+        span_of(q, q_seq, q_head, batch, q_heads, c->head_dim, c->dtype == RANS_X_F32 ? 4 : 2)};
+    if (overlap(out, read) || overlap(out[0], out[1]) || overlap(out[0], out[2]) || overlap(out[1], out[2]))
         return RANS_EARG;
     const Select a{bounds, q, q_seq, q_head, q_heads / c->kv_heads, c->kv_heads, c->pages,
                    __builtin_ctz(c->page_size), table, table_row, table_width, lengths, batch, count, first, last,
