@@ -42,8 +42,9 @@ typedef struct vramc_pages {
  * and whose pages, with those that sequences before it want, are all in the pool.
  * New pages come from the top of the stack in order and are written behind the
  * ceil(length / page_size) entries that the length takes up.  Negative numbers
- * count as 0, lengths beyond the row as its end.  Outputs and the table share no
- * memory with what is read, rows of the table none with each other (RANS_EARG). */
+ * count as 0, lengths beyond the row as its end.  Outputs, the table and the pool's
+ * tensors share no memory with one another or with what is read, rows of the table
+ * none with each other (RANS_EARG). */
 int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t table_row, int table_width,
                        const int32_t* lengths, const int32_t* fresh, const int32_t* seen, int batch,
                        int64_t tokens, int64_t* slots, int32_t* positions, int32_t* filled,
@@ -52,9 +53,9 @@ int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t table_row, 
 /* Puts the pages of entries at ceil(lengths[b] / page_size) and behind on the stack,
  * in order of the sequences and entries, and -1 in their place.  Entries that are
  * no page become -1 and go nowhere; what would not fit the stack (a page given back
- * twice) is dropped.  Table, lengths and pool share no memory (RANS_EARG).
- * workspace: vramc_pages_release_workspace bytes, no content
- * expected, 16-byte aligned, private to the call until its kernels have run. */
+ * twice) is dropped.  Table, lengths, workspace and the pool's tensors share no memory
+ * (RANS_EARG).  workspace: vramc_pages_release_workspace bytes, no content expected,
+ * 16-byte aligned, private to the call until its kernels have run. */
 int64_t vramc_pages_release_workspace(const vramc_pages* p, int table_width, int batch);
 int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t table_row, int table_width,
                         const int32_t* lengths, int batch, void* workspace, int64_t workspace_bytes,

@@ -49,7 +49,7 @@ def each_pair(call, written, read):
             if name == out:
                 continue
             first = at[name]
-            for address in (first, first + n - 16, first - size + 16):
+            for address in (first, first + max(n - 16, 0), first - max(size - 16, 0)):
                 assert call(**{out: address & -16}) == EARG, (out, name, hex(address - first))
             for address in (first + n + 16, first - size):
                 assert call(**{out: address & -16}) > 0, (out, name, "beside")
@@ -147,3 +147,47 @@ def test_select_writes_nothing_that_it_reads(host, lib, turned):
     out = {"chosen": 3 * K_HEADS * 8 * 4, "held": 3 * K_HEADS * 4, "work": need}
     each_pair(call, out, {"bounds": PAGES * K_HEADS * 2 * DIM * 2, "q": (2 * 400 + Q_HEADS * DIM) * 2,
                           "table": (2 * 1000 + 900) * 4, "lengths": 12, **out})
+
+
+# Three sequences in rows of 8 entries, 12 apart, 40 rows of tokens, 64 pages.
+POOL = {"free": 64 * 4, "count": 4, "ticket": 4}
+TABLE = {"table": (2 * 12 + 8) * 4}
+
+
+def pool_of(kv_pages, a):
+    return ctypes.byref(kv_pages.PagesDesc(64, 16, a["free"], a["count"], a["ticket"]))
+
+
+def test_extend_writes_nothing_twice(host, lib):
+    """Outputs, the table and the pool's tensors over what is read and over each other."""
+    import kv_pages
+
+    def call(**kw):
+        a = {**at, **kw}
+        return lib.vramc_pages_extend(pool_of(kv_pages, a), a["table"], 12, 8, a["lengths"], a["fresh"], a["seen"], 3, 40,
+                                      a["slots"], a["positions"], a["filled"], a["starts"], a["grown"], None)
+    out = {"slots": 320, "positions": 160, "filled": 160, "starts": 16, "grown": 12, **TABLE, **POOL}
+    each_pair(call, out, {"lengths": 12, "fresh": 12, "seen": 12, **out})
+
+
+def test_release_writes_nothing_twice(host, lib):
+    import kv_pages
+
+    def call(**kw):
+        a = {**at, **kw}
+        return lib.vramc_pages_release(pool_of(kv_pages, a), a["table"], 12, 8, a["lengths"], 3, a["work"], 16, None)
+    out = {"work": 16, **TABLE, **POOL}
+    each_pair(call, out, {"lengths": 12, **out})
+
+
+def test_a_pool_of_one_tensor(host):
+    """Free pages and their count in the same memory."""
+    import kv_pages
+    pool = host[1]
+    free = torch.arange(8, dtype=torch.int32)
+    table, n = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    pool._desc = kv_pages.PagesDesc(8, 16, free.data_ptr(), free[7:].data_ptr(), pool._ticket.data_ptr())
+    pool._ref = ctypes.byref(pool._desc)
+    for call in (lambda: pool.extend(table, n, n, 5), lambda: pool.release(table, n)):
+        with pytest.raises(ValueError, match="memory"):
+            call()

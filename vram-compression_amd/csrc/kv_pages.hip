@@ -315,9 +315,21 @@ bool one_launch(const int32_t* table, int64_t table_row, int table_width, int ba
            (int64_t)((table_width + 255) / 256) * batch <= kAllWaves * kPieces;
 }
 
-// Whether `bytes` at a and n integers at b share memory.
-bool overlap(const void* a, int64_t bytes, const int32_t* b, int64_t n) {
-    return b && n > 0 && bytes > 0 && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)a + bytes;
+// A pool's tensors.
+struct PoolSpans {
+    Span of[3];
+};
+PoolSpans spans_of(const vramc_pages& p) {
+    return {{{p.free, (int64_t)p.pages * 4}, {p.count, 4}, {p.ticket, 4}}};
+}
+
+// Whether some of these share memory with one another.
+template <size_t N>
+bool overlap(const Span (&a)[N]) {
+    for (size_t i = 0; i < N; i++)
+        for (size_t j = 0; j < i; j++)
+            if (overlap(a[i], a[j])) return true;
+    return false;
 }
 
 }  // namespace
@@ -331,20 +343,13 @@ extern "C" int vramc_pages_extend(const vramc_pages* p, int32_t* table, int64_t 
     if (tokens < 0 || tokens > INT32_MAX - 1 || !starts) return RANS_EARG;
     if (batch && (!lengths || !fresh || !new_lengths || (table_width && !table))) return RANS_EARG;
     if (tokens && (!slots || !positions || !filled)) return RANS_EARG;
-    const struct { const void* at; int64_t bytes; } outs[] = {
-        {slots, tokens * 8}, {positions, tokens * 4}, {filled, tokens * 4},
-        {starts, 4 * ((int64_t)batch + 1)}, {new_lengths, 4 * (int64_t)batch}};
-    const int64_t entries = batch ? table_row * (batch - 1) + table_width : 0;
-    const int64_t size = 4 * entries;
-    if (overlap(table, size, lengths, batch) || overlap(table, size, fresh, batch) || overlap(table, size, seen, batch) ||
-        overlap(table, size, p->free, p->pages) || overlap(table, size, p->count, 1) || overlap(table, size, p->ticket, 1))
+    const Span out[] = {{slots, tokens * 8}, {positions, tokens * 4}, {filled, tokens * 4},
+                        {starts, 4 * ((int64_t)batch + 1)}, {new_lengths, 4 * (int64_t)batch},
+                        span_of(table, table_row, 0, batch, 1, table_width, 4)};
+    const Span read[] = {{lengths, 4 * (int64_t)batch}, {fresh, 4 * (int64_t)batch}, {seen, 4 * (int64_t)batch}};
+    const auto pool = spans_of(*p);
+    if (overlap(out) || overlap(out, read) || overlap(out, pool.of) || overlap(pool.of) || overlap(pool.of, read))
         return RANS_EARG;
-    for (const auto& o : outs)
-        if (overlap(o.at, o.bytes, lengths, batch) || overlap(o.at, o.bytes, fresh, batch) ||
-            overlap(o.at, o.bytes, seen, batch) || overlap(o.at, o.bytes, table, entries) ||
-            overlap(o.at, o.bytes, p->free, p->pages) || overlap(o.at, o.bytes, p->count, 1) ||
-            overlap(o.at, o.bytes, p->ticket, 1))
-            return RANS_EARG;
     const Extend e{*p, __builtin_ctz(p->page_size), table, table_row, table_width, lengths, fresh, seen, batch,
                    (int)tokens, slots, positions, filled, starts, new_lengths};
     const int64_t blocks = (tokens + kThreads - 1) / kThreads;
@@ -363,13 +368,13 @@ extern "C" int vramc_pages_release(const vramc_pages* p, int32_t* table, int64_t
     if (const int rc = check_table(p, table_row, table_width, batch)) return rc;
     if (batch == 0 || table_width == 0) return 0;
     if (!table || !lengths) return RANS_EARG;
-    const int64_t entries = table_row * (batch - 1) + table_width;
-    if (overlap(table, 4 * entries, lengths, batch) || overlap(table, 4 * entries, p->free, p->pages) ||
-        overlap(table, 4 * entries, p->count, 1) || overlap(lengths, 4 * (int64_t)batch, p->free, p->pages) ||
-        overlap(lengths, 4 * (int64_t)batch, p->count, 1))
-        return RANS_EARG;
     if (!workspace || workspace_bytes < vramc_pages_release_workspace(p, table_width, batch)) return RANS_EWORKSPACE;
     if ((uintptr_t)workspace % 16) return RANS_EARG;
+    const Span out[] = {span_of(table, table_row, 0, batch, 1, table_width, 4), {workspace, 4 * ((int64_t)batch + 1)}};
+    const Span read[] = {{lengths, 4 * (int64_t)batch}};
+    const auto pool = spans_of(*p);
+    if (overlap(out) || overlap(out, read) || overlap(out, pool.of) || overlap(pool.of) || overlap(pool.of, read))
+        return RANS_EARG;
     auto* counts = static_cast<int32_t*>(workspace);
     const Release r{*p, __builtin_ctz(p->page_size), table, table_row, table_width, lengths, batch, counts,
                     counts + batch};
