@@ -14,7 +14,8 @@
 // A workgroup takes some tokens of one kind (queries, keys or values) with all
 // their heads.  The angles are the same for all heads of a token: one thread makes
 // each, to LDS.  position * turns is the angle in full turns, so that what it has
-// of whole ones falls away exactly in 64 bits, and 32 hold the rest.
+// of whole ones falls away exactly in 64 bits, and 32 hold the rest, for f32 rows with
+// a first-order step for the bits beyond.
 #include "kv_device.h"
 
 #include "../../include/vramc_rotary.h"
@@ -97,8 +98,14 @@ __global__ void __launch_bounds__(kThreads) rotate_kernel(Rotate a) {
         for (int i = thread; i < tokens * a.pairs; i += kThreads) {
             const int t = i / a.pairs, j = i - t * a.pairs;
             const double turn = (double)a.positions[first + t] * a.turns[j];
+            const double rest = turn - __builtin_rint(turn);
             float sine, cosine;
-            sincospif(2.f * (float)(turn - __builtin_rint(turn)), &sine, &cosine);
+            sincospif(2.f * (float)rest, &sine, &cosine);
+            if constexpr (std::is_same_v<T, float>) {  // what the rest's rounding left, no 16-bit type sees
+                const float more = (float)(rest - (double)(float)rest) * 6.28318531f, before = cosine;
+                cosine -= more * sine;
+                sine += more * before;
+            }
             angles[2 * t * a.pairs + j] = cosine * a.amplitude;
             angles[(2 * t + 1) * a.pairs + j] = sine * a.amplitude;
         }
