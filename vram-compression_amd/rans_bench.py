@@ -797,6 +797,8 @@ class AttentionStack:
         import kv_cache
         import kv_pages
         import rotary
+        if budget < 1 or slack < 1:
+            raise ValueError(f"budget {budget}, slack {slack}: a row at its budget takes one more token")
         torch.manual_seed(seed)
         width = -(-(budget + slack) // page)
         self.budget, self.slack, self.recent, self.batch = budget, slack, recent, batch
