@@ -818,6 +818,10 @@ class AttentionStack:
                                                                    bounds=count > 0),
                                       bits=bits, turn=turn, count=count) for _ in range(layers)]
 
+    def _pooled(self):
+        if self.pool is None:
+            raise ValueError("prompts and endings take a stack whose pages come from a pool: pooled=True")
+
     def _room(self, new, tokens):
         """Slots, positions and filled pages of new tokens, which lengths and seen then
         count."""
@@ -833,6 +837,7 @@ class AttentionStack:
         computed).  A sequence then holds fewer than budget + slack tokens, so that the
         next step's has a place.  Returns the rows (a list) whose prompt got no room, as
         their pages are not in the pool: they hold what they held."""
+        self._pooled()
         if len(new) != self.batch or any(m < 0 for m in new) or sum(new) != h.shape[0]:
             raise ValueError(f"prompts of {new} tokens, {h.shape[0]} rows of them and {self.batch} sequences")
         most = max(n + m for n, m in zip(self.each, new))
@@ -847,6 +852,7 @@ class AttentionStack:
 
     def finish(self, sequences):
         """Ends sequences (a list of rows); their pages are free again."""
+        self._pooled()
         for s in sequences:
             self.each[s] = 0
         self.held = max(self.each)
