@@ -23,7 +23,7 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMostShift = 5;  // tokens of a workgroup, whose angles then take 32 KB of LDS at most
+constexpr int kMostShift = 5;  // tokens of a workgroup, whose angles then take 8 KB of LDS at most
 
 // Rows of one kind: `heads` of each token; how workgroups take them.
 struct Kind {
