@@ -44,8 +44,8 @@ typedef struct vramc_rotary_rows {
 
 /* q_out, k_out: [tokens][heads][head_dim] of dtype, 16-byte aligned, sharing no
  * memory with each other or what is read (RANS_EARG).  Everything is computed in f32
- * (the angle in 64 bits up to its whole turns, for f32 to its sine) and rounded once; the norm of a head
- * whose squares leave f32 is no number of use. */
+ * (the angle in 64 bits up to its whole turns, for f32 rows up to its sine) and rounded
+ * once; the norm of a head whose squares leave f32 is no number of use. */
 int vramc_rotary_apply(const vramc_rotary* r, const vramc_rotary_rows* x, void* q_out, void* k_out,
                        hipStream_t stream);
 

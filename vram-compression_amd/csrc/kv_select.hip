@@ -9,11 +9,11 @@
 // select scores in 64 bits, so that a choice does not hang on the rounding of 32-bit
 // sums.  Vector instructions bound it: 16 sequences of 512 pages of 8 heads, 5 query
 // heads each, 16 us where their bounds are read in 6; the multiply-adds are a fifth of
-// the instructions, the rest sums over lanes, conversions and addresses.  A second launch, a workgroup to a kv head of
-// a sequence, finds the border by radix over the scores' bits, from the highest in
-// which they differ, and writes the pages in their order by counts of ballot bits (5
-// to 7 us: reads, digits, lists, one after the other); for small tables it makes the
-// scores too.
+// the instructions, the rest sums over lanes, conversions and addresses.  A second
+// launch, a workgroup to a kv head of a sequence, finds the border by radix over the
+// scores' bits, from the highest in which they differ, and writes the pages in their
+// order by counts of ballot bits (5 to 7 us: reads, digits, lists, one after the other);
+// for small tables it makes the scores too.
 #include "kv_device.h"
 
 #include <limits>
